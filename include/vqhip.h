@@ -33,6 +33,7 @@ extern "C" {
 
 #define VQHIP_F32  0
 #define VQHIP_BF16 1
+#define VQHIP_F16  2            /* taken by the beam, norm and gradient entry points at the end of this header only */
 
 #define VQHIP_EUCLID 0
 #define VQHIP_COSINE 1          /* l2-normalise the rows in the kernel prologue, then max dot product */
@@ -539,6 +540,51 @@ int vqhip_assign_rowwise(const float *x, int64_t N, int D, int64_t ldx, const fl
                          int64_t *idx_out, void *stream);
 
 int vqhip_row_sumsq(const void *x, int x_dtype, int64_t N, int D, int64_t ldx, float *out, void *stream);
+
+/* ---- beam search: selection -----------------------------------------------------------------------
+ * The selection of a beam search over codes (ResidualVQ.forward(beam_size=), rvq.py:493-562) or over any vocabulary:
+ *   c[b, j, v] = scores[b, j] + (logits[b, j, v] - log sum_v exp logits[b, j, v])     normalize != 0
+ *   c[b, j, v] = scores[b, j] + logits[b, j, v]                                       normalize == 0
+ * and per batch entry the K largest c in descending order, equal ones by ascending j * V + v.  What `mask` leaves out counts as -inf
+ * and takes no part in the sum (its logits may hold anything); a c that is not a number counts as -inf, so a beam whose log-sum is
+ * not finite has no continuation; a finished beam has one, c = scores[b, j] at end_token, its logits are not used.  Where fewer than K
+ * continuations are above -inf, -inf ones follow, by ascending j * V + v.  c is compared in 64 bits and returned rounded to fp32.
+ *   logits   [B, J, V] of dtype F32 / BF16 / F16, continuations contiguous, beams stride_j and batch entries stride_b elements apart
+ *   scores   nullable (zeros) [B, J] fp32        mask      nullable [B, J, V] bytes at byte strides mask_stride_b / _j (0: shared)
+ *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out: the log-sums, which the backward reads
+ *   out_scores / parents / tokens  [B, K]        workspace vqhip_beam_select_workspace_bytes(B, J, V, K) bytes, 16-byte aligned
+ * J, K <= VQHIP_BEAM_MAX, J * V < 2^31, K <= J * V (VQHIP_EDIM beyond).
+ * vqhip_beam_select_bwd: the gradients of out_scores (grad [B, K]) with the fields of the forward call, its outputs among them:
+ *   d_scores[b, j] (nullable [B, J] fp32) = sum of grad over the kept continuations of beam j,
+ *   d_logits (nullable [B, J, V] contiguous, dtype) = sum of grad over those with token v - (normalize) d_scores softmax(logits).
+ * A kept continuation of score -inf passes nothing on; masked places and finished beams get zeros in d_logits. */
+#define VQHIP_BEAM_MAX 64
+typedef struct {
+    const void *logits; int64_t dtype; int64_t B; int64_t J; int64_t V; int64_t stride_b; int64_t stride_j;
+    const float *scores;
+    const uint8_t *mask; int64_t mask_stride_b; int64_t mask_stride_j;
+    const uint8_t *finished; int64_t end_token;
+    int64_t normalize; int64_t K;
+    float *out_scores; int64_t *parents; int64_t *tokens; double *lse;
+    void *workspace; size_t workspace_bytes;
+} vqhip_beam_select_t;
+size_t vqhip_beam_select_workspace_bytes(int64_t B, int64_t J, int64_t V, int64_t K);
+int vqhip_beam_select(const vqhip_beam_select_t *step, void *stream);
+int vqhip_beam_select_bwd(const vqhip_beam_select_t *step, const float *grad, void *d_logits, float *d_scores, void *stream);
+
+/* ---- beam search: the states follow their beams ------------------------------------------------------
+ * dst[b, i] = src[b, parents[b, i]] for n <= VQHIP_BEAM_STATES states in one launch (`pick`, the gathers of rvq.py:533-562).  A state's row is
+ * `pieces` runs of piece_bytes contiguous bytes, piece_stride bytes apart; rows lie stride_j, batch entries stride_b bytes apart; dst is
+ * contiguous [B, K, pieces * piece_bytes] and overlaps no src.  parents [B, K] int64; one outside [0, J) gives a row of zeros.
+ * vqhip_beam_reorder_bwd: dst[b, j] = sum of src[b, i] over parents[b, i] == j, summed in fp32 by ascending i and rounded once; src
+ * (the gradients [B, K, row]) and dst ([B, J, row]) contiguous, element types dtypes[n] F32 / BF16 / F16; the strides are not read. */
+#define VQHIP_BEAM_STATES 32
+typedef struct {
+    const void *src; void *dst; int64_t stride_b; int64_t stride_j; int64_t pieces; int64_t piece_stride; int64_t piece_bytes;
+} vqhip_beam_state_t;
+int vqhip_beam_reorder(const vqhip_beam_state_t *states, int64_t n, const int64_t *parents, int64_t B, int64_t J, int64_t K, void *stream);
+int vqhip_beam_reorder_bwd(const vqhip_beam_state_t *states, const int64_t *dtypes, int64_t n, const int64_t *parents, int64_t B,
+                           int64_t J, int64_t K, void *stream);
 
 #ifdef __cplusplus
 }

@@ -6,5 +6,7 @@ from .vector_quantize import VectorQuantize, LossBreakdown
 from .residual_vq import ResidualVQ, GroupedResidualVQ
 from .sim_vq import SimVQ, ResidualSimVQ
 from .callers import HierarchicalVQ, RandomProjectionQuantizer
+from .beam import BeamStep, beam_reorder, beam_select
 
-__all__ = ["VectorQuantize", "ResidualVQ", "GroupedResidualVQ", "SimVQ", "ResidualSimVQ", "RandomProjectionQuantizer", "HierarchicalVQ", "Codebook", "LossBreakdown"]
+__all__ = ["VectorQuantize", "ResidualVQ", "GroupedResidualVQ", "SimVQ", "ResidualSimVQ", "RandomProjectionQuantizer", "HierarchicalVQ", "Codebook", "LossBreakdown",
+           "BeamStep", "beam_select", "beam_reorder"]

@@ -15,7 +15,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("VQHIP_SO", os.path.join(_HERE, "csrc", "libvqhip.so"))   # VQHIP_SO: A/B experiments only
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2                 # (F16: the operators of beam.py, norms.py and grads.py only)
 EUCLID, COSINE, COSINE_PRENORM = 0, 1, 2
 ASSIGN_ROWS_PER_BLOCK = 128
 
@@ -156,6 +156,16 @@ def lib():
     L.vqhip_vq_step_chunk_rows.restype = i64
     L.vqhip_vq_train_step.argtypes = [vp, vp]
     L.vqhip_vq_train_step.restype = i32
+    L.vqhip_beam_select_workspace_bytes.argtypes = [i64, i64, i64, i64]
+    L.vqhip_beam_select_workspace_bytes.restype = ctypes.c_size_t
+    L.vqhip_beam_select.argtypes = [vp, vp]
+    L.vqhip_beam_select.restype = i32
+    L.vqhip_beam_select_bwd.argtypes = [vp, vp, vp, vp, vp]
+    L.vqhip_beam_select_bwd.restype = i32
+    L.vqhip_beam_reorder.argtypes = [vp, i64, vp, i64, i64, i64, vp]
+    L.vqhip_beam_reorder.restype = i32
+    L.vqhip_beam_reorder_bwd.argtypes = [vp, vp, i64, vp, i64, i64, i64, vp]
+    L.vqhip_beam_reorder_bwd.restype = i32
     for name in ("vqhip_pack_codebook", "vqhip_assign", "vqhip_reduce_partials", "vqhip_ema_accumulate",
                  "vqhip_ema_finalize", "vqhip_decode_sum", "vqhip_row_sumsq", "vqhip_assign_rowwise", "vqhip_score_indices", "vqhip_topk", "vqhip_expire_scatter", "vqhip_kmeans_update", "vqhip_route_fwd", "vqhip_route_bwd", "vqhip_rvq_route", "vqhip_ema_renormalize_shard", "vqhip_scores_lse"):
         getattr(L, name).restype = i32
@@ -172,7 +182,8 @@ EXPORTS = ("vqhip_version", "vqhip_last_error", "vqhip_packed_bytes", "vqhip_pac
            "vqhip_route_fwd_gather", "vqhip_route_bwd_gather", "vqhip_ema_accumulate_prezeroed",
            "vqhip_ema_batched_ws_stride", "vqhip_ema_accumulate_batched", "vqhip_ema_finalize_batched",
            "vqhip_ema_accumulate_stages", "vqhip_rvq_chain_chunk_rows", "vqhip_rvq_chain_ws_stride", "vqhip_rvq_chain_forward",
-           "vqhip_ema_finalize_table", "vqhip_decode_sum_range")
+           "vqhip_ema_finalize_table", "vqhip_decode_sum_range",
+           "vqhip_beam_select_workspace_bytes", "vqhip_beam_select", "vqhip_beam_select_bwd", "vqhip_beam_reorder", "vqhip_beam_reorder_bwd")
 
 
 def _check(rc, what):
@@ -211,6 +222,17 @@ def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return BF16
     raise VQHipError(f"unsupported dtype {t.dtype}: the HIP path takes float32 or bfloat16")
+
+
+_ELEM_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+def _elem_code(t: torch.Tensor, what: str) -> int:
+    """the element code of the entry points that take float16 as well"""
+    code = _ELEM_CODES.get(t.dtype)
+    if code is None:
+        raise VQHipError(f"{what}: unsupported dtype {t.dtype}, takes float32, bfloat16 or float16")
+    return code
 
 
 def _need_gpu(*ts):

@@ -1,0 +1,304 @@
+"""Beam search over codes, or over any vocabulary: the selection over beams and continuations (`beam_select`) and the reordering of
+the beams' states (`beam_reorder`), both differentiable.  `ResidualVQ.forward(beam_size=)` runs on them (reference: rvq.py:493-562).
+
+    logits = model(tokens, caches)                                        # [b, beams, vocabulary]
+    step = beam_select(logits, scores, beam_size, finished=finished, end_token=end)
+    caches = beam_reorder(caches, step.parents)                           # every state [b, beams, ...] follows its beam
+    scores, tokens = step.scores, step.tokens                             # [b, beam_size]
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _lib as L
+
+BEAM_MAX = 64            # VQHIP_BEAM_MAX: beams before and after a selection
+_STATES = 32             # VQHIP_BEAM_STATES: states of one launch
+
+_i64, _vp = ctypes.c_int64, ctypes.c_void_p
+
+
+class BeamStep(NamedTuple):
+    """the survivors of a selection, best first: accumulated scores (fp32), the beams they continue and the chosen continuations"""
+    scores: torch.Tensor
+    parents: torch.Tensor
+    tokens: torch.Tensor
+
+
+class _Select(ctypes.Structure):                         # vqhip_beam_select_t
+    _fields_ = [("logits", _vp), ("dtype", _i64), ("B", _i64), ("J", _i64), ("V", _i64), ("stride_b", _i64), ("stride_j", _i64),
+                ("scores", _vp), ("mask", _vp), ("mask_stride_b", _i64), ("mask_stride_j", _i64), ("finished", _vp), ("end_token", _i64),
+                ("normalize", _i64), ("K", _i64), ("out_scores", _vp), ("parents", _vp), ("tokens", _vp), ("lse", _vp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class _State(ctypes.Structure):                          # vqhip_beam_state_t
+    _fields_ = [("src", _vp), ("dst", _vp), ("stride_b", _i64), ("stride_j", _i64), ("pieces", _i64), ("piece_stride", _i64),
+                ("piece_bytes", _i64)]
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _table(t: torch.Tensor, b: int, j: int, v: int) -> torch.Tensor:
+    """t [..., j, v] as [b, j, v] with contiguous continuations, without a copy where the layout allows it"""
+    t = t.reshape(b, j, v)
+    return t if t.stride(-1) == 1 or v == 1 else t.contiguous()
+
+
+@L._on_device
+def _select(logits, scores, mask, finished, beam_size, end_token, normalize, want_lse):
+    b, j, v = logits.shape
+    dev = logits.device
+    out = torch.empty(b, beam_size, dtype=torch.float32, device=dev)
+    parents, tokens = torch.empty(2, b, beam_size, dtype=torch.int64, device=dev).unbind(0)
+    lse = torch.empty(b, j, dtype=torch.float64, device=dev) if want_lse else None
+    nws = L.lib().vqhip_beam_select_workspace_bytes(b, j, v, beam_size)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    s = _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse)
+    s.workspace, s.workspace_bytes = _addr(ws), nws
+    L._check(L.lib().vqhip_beam_select(ctypes.byref(s), L._stream()), "vqhip_beam_select")
+    return out, parents, tokens, lse
+
+
+def _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse):
+    b, j, v = logits.shape
+    return _Select(logits=_addr(logits), dtype=L._ELEM_CODES[logits.dtype], B=b, J=j, V=v, stride_b=logits.stride(0), stride_j=logits.stride(1),
+                   scores=_addr(scores), mask=_addr(mask), mask_stride_b=0 if mask is None else mask.stride(0),
+                   mask_stride_j=0 if mask is None else mask.stride(1), finished=_addr(finished), end_token=end_token,
+                   normalize=int(normalize), K=out.shape[1], out_scores=_addr(out), parents=_addr(parents), tokens=_addr(tokens), lse=_addr(lse))
+
+
+@L._on_device
+def _select_bwd(grad, logits, mask, finished, end_token, normalize, out, parents, tokens, lse, want_logits, want_scores):
+    b, j, v = logits.shape
+    d_logits = torch.empty(b, j, v, dtype=logits.dtype, device=logits.device) if want_logits else None
+    d_scores = torch.empty(b, j, dtype=torch.float32, device=logits.device) if want_scores else None
+    s = _struct(logits, None, mask, finished, end_token, normalize, out, parents, tokens, lse)
+    L._check(L.lib().vqhip_beam_select_bwd(ctypes.byref(s), _addr(grad), _addr(d_logits), _addr(d_scores), L._stream()), "vqhip_beam_select_bwd")
+    return d_logits, d_scores
+
+
+class _SelectFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, scores, mask, finished, beam_size, end_token, normalize):
+        out, parents, tokens, lse = _select(logits, scores, mask, finished, beam_size, end_token, normalize, normalize)
+        ctx.save_for_backward(logits, mask, finished, out, parents, tokens, lse)
+        ctx.end_token, ctx.normalize = end_token, normalize
+        ctx.mark_non_differentiable(parents, tokens)
+        ctx.set_materialize_grads(False)
+        return out, parents, tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _parents, _tokens):
+        if grad is None:
+            return (None,) * 7
+        logits, mask, finished, out, parents, tokens, lse = ctx.saved_tensors
+        d_logits, d_scores = _select_bwd(grad.contiguous(), logits, mask, finished, ctx.end_token, ctx.normalize, out, parents, tokens, lse,
+                                         ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return d_logits, d_scores, None, None, None, None, None
+
+
+def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size: int, *, mask: Optional[torch.Tensor] = None,
+                finished: Optional[torch.Tensor] = None, end_token: Optional[int] = None, normalize: bool = True) -> BeamStep:
+    """The `beam_size` best of all continuations of all beams.
+
+    logits [..., beams, vocabulary] (float32 / bfloat16 / float16), scores [..., beams] float32 (None: zeros): continuation v of beam j
+    scores `scores[j] + log_softmax(logits[j])[v]`, or `scores[j] + logits[j, v]` with normalize=False (negative errors of codes, say).
+    -> BeamStep(scores, parents, tokens), each [..., beam_size], best first; equal scores by ascending beam, then ascending token.
+
+    mask      bool, broadcastable to logits: False leaves a continuation out -- of the softmax as well; its logits may hold anything
+    finished  bool [..., beams]: such a beam is kept as it is, as its own only continuation `end_token`
+    A score that is not a number counts as -inf: a beam whose logits hold NaN or +inf, or whose mask leaves nothing, has no
+    continuation (normalize=True).  Where fewer than beam_size continuations are left, the last survivors have a score of -inf.
+    Gradients reach logits and scores through the returned scores; survivors of score -inf pass none on."""
+    L._elem_code(logits, "beam_select")
+    if logits.ndim < 2:
+        raise L.VQHipError(f"beam_select: logits {tuple(logits.shape)}, expected [..., beams, vocabulary]")
+    *lead, j, v = logits.shape
+    rows = tuple(logits.shape[:-1])
+    if scores is not None and (tuple(scores.shape) != rows or scores.dtype != torch.float32):
+        raise L.VQHipError(f"beam_select: scores {tuple(scores.shape)} {scores.dtype}, expected {rows} float32")
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise L.VQHipError(f"beam_select: mask of {mask.dtype}, expected bool")
+        try:
+            mask = mask.expand(logits.shape)
+        except RuntimeError:
+            raise L.VQHipError(f"beam_select: mask {tuple(mask.shape)} does not broadcast to {tuple(logits.shape)}") from None
+    if finished is not None:
+        if tuple(finished.shape) != rows or finished.dtype != torch.bool:
+            raise L.VQHipError(f"beam_select: finished {tuple(finished.shape)} {finished.dtype}, expected {rows} bool")
+        if end_token is None or not 0 <= end_token < v:
+            raise L.VQHipError(f"beam_select: finished beams need an end_token in [0, {v}), got {end_token}")
+    if j < 1 or v < 1 or j > BEAM_MAX or not 1 <= beam_size <= min(BEAM_MAX, j * v):
+        raise L.VQHipError(f"beam_select: {beam_size} survivors of {j} x {v} continuations: takes 1 to {BEAM_MAX} beams and survivors, "
+                           "no more survivors than continuations")
+    L._need_gpu(logits, scores, mask, finished)
+    n = 1
+    for d in lead:
+        n *= d
+    lg = _table(logits, n, j, v)
+    sc = None if scores is None else scores.reshape(n, j).contiguous()
+    mk = None if mask is None else _table(mask, n, j, v).view(torch.uint8)
+    fin = None if finished is None else finished.reshape(n, j).contiguous().view(torch.uint8)
+    end = 0 if finished is None else int(end_token)
+    if torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad)):
+        out, parents, tokens = _SelectFn.apply(lg, sc, mk, fin, beam_size, end, bool(normalize))
+    else:
+        out, parents, tokens, _ = _select(lg, sc, mk, fin, beam_size, end, bool(normalize), False)
+    if len(lead) != 1:
+        out, parents, tokens = (t.view(*lead, beam_size) for t in (out, parents, tokens))
+    return BeamStep(out, parents, tokens)
+
+
+# ---- states ---------------------------------------------------------------------------------------------------------------------
+def _collapse(sizes, strides):
+    """(count, stride) of dims that lie behind each other like one, None where they do not"""
+    n, st = 1, 0
+    for d, s in zip(reversed(sizes), reversed(strides)):
+        if d == 1:
+            continue
+        if n == 1:
+            n, st = d, s
+        elif s == n * st:
+            n *= d
+        else:
+            return None
+    return n, st
+
+
+def _layout(t: torch.Tensor, nlead: int):
+    """t [*lead, beams, ...] -> (t or its contiguous copy, batch stride, beam stride, pieces, piece stride, elements of a piece)"""
+    shape, strides = t.shape, t.stride()
+    lead = _collapse(shape[:nlead], strides[:nlead])
+    inner, inner_st = list(shape[nlead + 1:]), list(strides[nlead + 1:])
+    run = 1
+    while inner and (inner[-1] == 1 or inner_st[-1] == run):
+        run *= inner.pop()
+        inner_st.pop()
+    pieces = _collapse(inner, inner_st)
+    if lead is None or pieces is None:
+        return _layout(t.contiguous(), nlead)
+    return t, lead[1], strides[nlead], pieces[0], pieces[1], run
+
+
+def _extent(t):
+    """[first byte, behind the last byte) of a tensor's memory"""
+    span = sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + span * t.element_size()
+
+
+@L._on_device
+def _reorder(parents, states, outs):
+    nlead, k = parents.ndim - 1, parents.shape[-1]
+    n = parents.numel() // k
+    keep, table, j = [], [], states[0].shape[nlead]
+    for s, o in zip(states, outs):
+        if s.numel() == 0:
+            continue
+        t, sb, sj, pieces, ps, run = _layout(s, nlead)
+        keep.append(t)
+        es = t.element_size()
+        table.append((t.data_ptr(), o.data_ptr(), sb * es, sj * es, pieces, ps * es, run * es))
+    for i in range(0, len(table), _STATES):
+        part = table[i:i + _STATES]
+        arr = (_State * len(part))(*part)
+        L._check(L.lib().vqhip_beam_reorder(arr, len(part), _addr(parents), n, j, k, L._stream()), "vqhip_beam_reorder")
+
+
+@L._on_device
+def _reorder_bwd(parents, j, grads):
+    nlead, k = parents.ndim - 1, parents.shape[-1]
+    n = parents.numel() // k
+    lead = parents.shape[:-1]
+    grads = [None if g is None else g.contiguous() for g in grads]
+    outs = [None if g is None else torch.empty(*lead, j, *g.shape[nlead + 1:], dtype=g.dtype, device=g.device) for g in grads]
+    some = [(g, o) for g, o in zip(grads, outs) if g is not None and o.numel()]
+    for i in range(0, len(some), _STATES):
+        part = some[i:i + _STATES]
+        arr = (_State * len(part))(*[(g.data_ptr(), o.data_ptr(), 0, 0, 1, 0, g.element_size() * (g.numel() // (n * k))) for g, o in part])
+        dts = (_i64 * len(part))(*[L._ELEM_CODES[g.dtype] for g, _ in part])
+        L._check(L.lib().vqhip_beam_reorder_bwd(arr, dts, len(part), _addr(parents), n, j, k, L._stream()), "vqhip_beam_reorder_bwd")
+    return outs
+
+
+class _ReorderFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, parents, *states):
+        nlead, k = parents.ndim - 1, parents.shape[-1]
+        outs = tuple(torch.empty(*parents.shape, *s.shape[nlead + 1:], dtype=s.dtype, device=s.device) for s in states)
+        _reorder(parents, states, outs)
+        ctx.save_for_backward(parents)
+        ctx.beams = states[0].shape[nlead]
+        ctx.mark_non_differentiable(*[o for o, s in zip(outs, states) if not s.requires_grad])
+        ctx.set_materialize_grads(False)
+        return outs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        parents, = ctx.saved_tensors
+        need = ctx.needs_input_grad[1:]
+        return (None, *_reorder_bwd(parents, ctx.beams, [g if w else None for g, w in zip(grads, need)]))
+
+
+def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None) -> list:
+    """states: tensors [..., beams, *] of any types and shapes behind the beams (caches, residuals, token histories); parents [..., k]
+    int64 -> a list of [..., k, *]: row i of every result is row parents[i] of its state, all of them in one launch.  A parent outside
+    [0, beams) gives a row of zeros.  States are read in place where their rows are evenly spaced runs (a cache cut to the positions in
+    use, `cache[..., :length, :]`), otherwise from a contiguous copy.
+
+    out: contiguous tensors that take the results (the other half of a double buffer); they may not share memory with a state or with
+    each other, and no state may require a gradient.  Without it, gradients reach float32, bfloat16 and float16 states: beams continued
+    by several rows get the sum, accumulated in 32 bits."""
+    states = list(states)
+    if parents.dtype != torch.int64 or parents.ndim < 1 or parents.shape[-1] < 1:
+        raise L.VQHipError(f"beam_reorder: parents {tuple(parents.shape)} {parents.dtype}, expected int64 [..., k]")
+    if not states:
+        return []
+    nlead = parents.ndim - 1
+    j = states[0].shape[nlead] if states[0].ndim > nlead else 0
+    for s in states:
+        if s.device != parents.device:
+            raise L.VQHipError(f"beam_reorder: tensors on different devices ({parents.device} and {s.device})")
+        if s.ndim <= nlead or s.shape[:nlead] != parents.shape[:-1] or s.shape[nlead] != j or j < 1:
+            raise L.VQHipError(f"beam_reorder: state {tuple(s.shape)}, expected {tuple(parents.shape[:-1])} + ({j or 'beams'}, ...)")
+    grad = torch.is_grad_enabled() and any(s.requires_grad for s in states)
+    if out is None:
+        if grad:
+            for s in states:
+                if s.requires_grad:
+                    L._elem_code(s, "beam_reorder: state with a gradient")
+        L._need_gpu(parents, *states)
+        parents = parents.contiguous()
+        if grad:
+            return list(_ReorderFn.apply(parents, *states))
+        out = [torch.empty(*parents.shape, *s.shape[nlead + 1:], dtype=s.dtype, device=s.device) for s in states]
+    else:
+        out = list(out)
+        if grad:
+            raise L.VQHipError("beam_reorder: out= with states that require a gradient")
+        if len(out) != len(states):
+            raise L.VQHipError(f"beam_reorder: {len(out)} results for {len(states)} states")
+        for s, o in zip(states, out):
+            if o.shape != (*parents.shape, *s.shape[nlead + 1:]) or o.dtype != s.dtype or o.device != s.device or not o.is_contiguous():
+                raise L.VQHipError(f"beam_reorder: out {tuple(o.shape)} {o.dtype}, expected contiguous "
+                                   f"{(*parents.shape, *s.shape[nlead + 1:])} {s.dtype} on {s.device}")
+        taken = sorted([(*_extent(t), w) for w, ts in ((0, [*states, parents]), (1, out)) for t in ts if t.numel()])
+        end = end_out = -1                                       # behind the last byte of any tensor, of any result so far
+        for first, behind, is_out in taken:
+            if first < (end if is_out else end_out):
+                raise L.VQHipError("beam_reorder: out shares memory with a state, the parents or another result")
+            end = max(end, behind)
+            end_out = max(end_out, behind) if is_out else end_out
+        L._need_gpu(parents, *states)
+        parents = parents.contiguous()
+    if parents.numel():
+        _reorder(parents, states, out)
+    return out
