@@ -586,6 +586,42 @@ int vqhip_beam_reorder(const vqhip_beam_state_t *states, int64_t n, const int64_
 int vqhip_beam_reorder_bwd(const vqhip_beam_state_t *states, const int64_t *dtypes, int64_t n, const int64_t *parents, int64_t B,
                            int64_t J, int64_t K, void *stream);
 
+/* ---- group norm with an activation, channels last ----------------------------------------------------
+ * y = act((x - mean) rstd weight + bias) on rows [B, N, C] as the quantizers read them (a feature map's positions are its rows); mean and
+ * the biased variance over the live rows and the C / groups channels of a group, rstd = 1 / sqrt(variance + eps).
+ *   x       [B, N, C], channels contiguous, rows stride_n and batch entries stride_b elements apart; y contiguous, x's dtype
+ *   weight, bias  nullable [C] of param_dtype        lens nullable [B] int64: rows n < lens[b] are live; mask nullable [B, N] bytes,
+ *           0 = padding (one of the two).  Padding rows may hold anything; their y, and their dx, are zero
+ *   mean, rstd    [B, groups] fp32 out, which the backward reads         act VQHIP_ACT_NONE / VQHIP_ACT_SILU (z sigmoid(z))
+ *   workspace     vqhip_group_norm_workspace_bytes bytes, 16-byte aligned, for either call
+ * vqhip_group_norm_bwd: from grad (y's gradient, [B, N, C] contiguous) dx (contiguous, x's dtype), dweight and dbias (param_dtype), each
+ * nullable; the sums over rows and batch in 32 bits or more, in an order that depends on the sizes alone.
+ * C <= VQHIP_NORM_MAX_C. */
+#define VQHIP_ACT_NONE 0
+#define VQHIP_ACT_SILU 1
+#define VQHIP_NORM_MAX_C 8192
+typedef struct {
+    const void *x; int64_t dtype; int64_t B; int64_t N; int64_t C; int64_t stride_b; int64_t stride_n;
+    int64_t groups; const void *weight; const void *bias; int64_t param_dtype; double eps; int64_t activation;
+    const int64_t *lens; const uint8_t *mask;
+    float *mean; float *rstd;
+    void *workspace; size_t workspace_bytes;
+} vqhip_group_norm_t;
+size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t C, int64_t groups);
+int vqhip_group_norm(const vqhip_group_norm_t *norm, void *y, void *stream);
+int vqhip_group_norm_bwd(const vqhip_group_norm_t *norm, const void *grad, void *dx, void *dweight, void *dbias, void *stream);
+
+/* ---- the global norm of many gradients, and clipping ---------------------------------------------------
+ * norm[0] = sqrt(sum of squares over all `count` tensors), squares and sums in 64 bits; dst = src * min(1, max_norm / (norm + eps)) for
+ * every tensor with a dst (src itself, or memory that overlaps no tensor of the call).  A norm that is not finite goes through: the
+ * factor is 0 for an infinite one, NaN for NaN.  `grads` is host memory, read during the call; src and dst are device pointers to n
+ * contiguous elements of dtype F32 / BF16 / F16.  No tensor occurs twice.  workspace: vqhip_clip_grads_workspace_bytes bytes, 16-byte
+ * aligned.  No host read: capturable. */
+typedef struct { const void *src; void *dst; int64_t n; int64_t dtype; } vqhip_grad_t;
+size_t vqhip_clip_grads_workspace_bytes(const vqhip_grad_t *grads, int64_t count);
+int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double max_norm, double eps, float *norm, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

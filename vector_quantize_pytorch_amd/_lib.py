@@ -166,6 +166,16 @@ def lib():
     L.vqhip_beam_reorder.restype = i32
     L.vqhip_beam_reorder_bwd.argtypes = [vp, vp, i64, vp, i64, i64, i64, vp]
     L.vqhip_beam_reorder_bwd.restype = i32
+    L.vqhip_group_norm_workspace_bytes.argtypes = [i64, i64, i64, i64]
+    L.vqhip_group_norm_workspace_bytes.restype = ctypes.c_size_t
+    L.vqhip_group_norm.argtypes = [vp, vp, vp]
+    L.vqhip_group_norm.restype = i32
+    L.vqhip_group_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp]
+    L.vqhip_group_norm_bwd.restype = i32
+    L.vqhip_clip_grads_workspace_bytes.argtypes = [vp, i64]
+    L.vqhip_clip_grads_workspace_bytes.restype = ctypes.c_size_t
+    L.vqhip_clip_grads.argtypes = [vp, i64, f64, f64, vp, vp, ctypes.c_size_t, vp]
+    L.vqhip_clip_grads.restype = i32
     for name in ("vqhip_pack_codebook", "vqhip_assign", "vqhip_reduce_partials", "vqhip_ema_accumulate",
                  "vqhip_ema_finalize", "vqhip_decode_sum", "vqhip_row_sumsq", "vqhip_assign_rowwise", "vqhip_score_indices", "vqhip_topk", "vqhip_expire_scatter", "vqhip_kmeans_update", "vqhip_route_fwd", "vqhip_route_bwd", "vqhip_rvq_route", "vqhip_ema_renormalize_shard", "vqhip_scores_lse"):
         getattr(L, name).restype = i32
@@ -183,7 +193,8 @@ EXPORTS = ("vqhip_version", "vqhip_last_error", "vqhip_packed_bytes", "vqhip_pac
            "vqhip_ema_batched_ws_stride", "vqhip_ema_accumulate_batched", "vqhip_ema_finalize_batched",
            "vqhip_ema_accumulate_stages", "vqhip_rvq_chain_chunk_rows", "vqhip_rvq_chain_ws_stride", "vqhip_rvq_chain_forward",
            "vqhip_ema_finalize_table", "vqhip_decode_sum_range",
-           "vqhip_beam_select_workspace_bytes", "vqhip_beam_select", "vqhip_beam_select_bwd", "vqhip_beam_reorder", "vqhip_beam_reorder_bwd")
+           "vqhip_beam_select_workspace_bytes", "vqhip_beam_select", "vqhip_beam_select_bwd", "vqhip_beam_reorder", "vqhip_beam_reorder_bwd",
+           "vqhip_group_norm_workspace_bytes", "vqhip_group_norm", "vqhip_group_norm_bwd", "vqhip_clip_grads_workspace_bytes", "vqhip_clip_grads")
 
 
 def _check(rc, what):
@@ -240,6 +251,13 @@ def _need_gpu(*ts):
         if t is not None and not t.is_cuda:
             raise VQHipError("vector_quantize_pytorch_amd runs on MI355X only: got a CPU tensor "
                              "(there is no CPU fallback; move the module and input to 'cuda')")
+
+
+def _written(tensors):
+    """tells autograd that the library wrote into tensors of the caller (a graph that saved one then refuses its backward)"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _ptr(t):

@@ -301,4 +301,5 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         parents = parents.contiguous()
     if parents.numel():
         _reorder(parents, states, out)
+        L._written(out)
     return out

@@ -1,0 +1,125 @@
+// vq_grads.hip -- the global norm of many gradients, and their clipping.
+#include "vq_elem.h"
+
+#include <math.h>
+
+// norm = sqrt(sum of all squares): squares and sums in 64 bits, so that neither 1e30 nor 1e-30 leaves the range.  The tensors travel as
+// kernel arguments, TENSORS of a launch; a tensor is cut into chunks, one workgroup and one partial sum each.
+#define GRAD_TENSORS 100
+#define GRAD_CHUNK 16384
+struct GradTensor { const void *src; void *dst; int64_t n; unsigned first; int dtype; };        // first: its first workgroup in the launch
+struct GradArgs { GradTensor t[GRAD_TENSORS]; int count; };
+
+__device__ __forceinline__ const GradTensor &grad_tensor(const GradArgs &a, unsigned block)
+{
+    int lo = 0, hi = a.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.t[mid].first <= block) lo = mid; else hi = mid - 1;
+    }
+    return a.t[lo];
+}
+
+__device__ double grad_block_sum(double v)
+{
+    __shared__ double red[4];
+    v = vq_wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+template <typename T> __device__ double grad_sumsq(const GradTensor &t, int64_t at, int64_t end)
+{
+    double s = 0.0;
+    for (int64_t i = at + threadIdx.x; i < end; i += 256) { const double v = (double)(float)((const T *)t.src)[i]; s = fma(v, v, s); }
+    return s;
+}
+
+__global__ void __launch_bounds__(256) vq_grad_norm_kernel(const GradArgs a, double *partial)
+{
+    const GradTensor &t = grad_tensor(a, blockIdx.x);
+    const int64_t at = (int64_t)(blockIdx.x - t.first) * GRAD_CHUNK, end = at + GRAD_CHUNK < t.n ? at + GRAD_CHUNK : t.n;
+    double s = t.dtype == VQHIP_F32 ? grad_sumsq<float>(t, at, end) : t.dtype == VQHIP_BF16 ? grad_sumsq<__bf16>(t, at, end) : grad_sumsq<_Float16>(t, at, end);
+    s = grad_block_sum(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// norm and coef = min(1, max_norm / (norm + eps)): (float) each behind the partial sums
+__global__ void __launch_bounds__(256) vq_grad_coef_kernel(const double *partial, int64_t n, double max_norm, double eps, float *norm, float *coef)
+{
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 256) s += partial[i];
+    s = sqrt(grad_block_sum(s));
+    if (threadIdx.x == 0) {
+        const double c = max_norm / (s + eps);
+        norm[0] = (float)s;
+        coef[0] = c > 1.0 ? 1.f : (float)c;             // (a norm that is not a number: neither comparison holds, NaN goes through)
+    }
+}
+
+template <typename T> __device__ void grad_scale(const GradTensor &t, int64_t at, int64_t end, float coef)
+{
+    for (int64_t i = at + threadIdx.x; i < end; i += 256) ((T *)t.dst)[i] = (T)((float)((const T *)t.src)[i] * coef);
+}
+
+__global__ void __launch_bounds__(256) vq_grad_scale_kernel(const GradArgs a, const float *coef_p)
+{
+    const GradTensor &t = grad_tensor(a, blockIdx.x);
+    const float coef = *coef_p;
+    if (coef == 1.f && t.src == t.dst) return;          // in place and nothing to clip: g * 1 is g
+    const int64_t at = (int64_t)(blockIdx.x - t.first) * GRAD_CHUNK, end = at + GRAD_CHUNK < t.n ? at + GRAD_CHUNK : t.n;
+    if (t.dtype == VQHIP_F32) grad_scale<float>(t, at, end, coef);
+    else if (t.dtype == VQHIP_BF16) grad_scale<__bf16>(t, at, end, coef);
+    else grad_scale<_Float16>(t, at, end, coef);
+}
+
+static int64_t grad_blocks(const vqhip_grad_t *g, int64_t count)
+{
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; ++i) n += g[i].n > 0 ? (g[i].n + GRAD_CHUNK - 1) / GRAD_CHUNK : 0;
+    return n;
+}
+
+extern "C" size_t vqhip_clip_grads_workspace_bytes(const vqhip_grad_t *grads, int64_t count)
+{
+    return grads && count > 0 ? (size_t)grad_blocks(grads, count) * 8 + 16 : 16;
+}
+
+extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double max_norm, double eps, float *norm, void *workspace,
+                                size_t workspace_bytes, void *stream)
+{
+    if (count < 0 || (count > 0 && !grads) || !norm || !workspace) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: %lld tensors, null pointer", (long long)count);
+    if (!(max_norm >= 0.0) || !(eps >= 0.0)) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: max_norm %g, eps %g", max_norm, eps);
+    bool write = false;
+    for (int64_t i = 0; i < count; ++i) {
+        if (!vq_elem_bytes(grads[i].dtype) || grads[i].n < 0 || grads[i].n > ((int64_t)1 << 44)) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: tensor %lld: dtype %lld, %lld elements", (long long)i, (long long)grads[i].dtype, (long long)grads[i].n);
+        if (grads[i].n > 0 && !grads[i].src) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: tensor %lld: null pointer", (long long)i);
+        write |= grads[i].n > 0 && grads[i].dst;
+    }
+    const int64_t blocks = grad_blocks(grads, count);
+    if (blocks > 0x7fffffff) VQ_FAIL(VQHIP_EDIM, "vqhip_clip_grads: too many elements");
+    if (workspace_bytes < (size_t)blocks * 8 + 16) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: workspace of %zu bytes", workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    float *coef = (float *)workspace;
+    double *partial = (double *)((char *)workspace + 16);
+    for (int pass = 0; pass < (write ? 2 : 1); ++pass) {
+        int64_t done = 0;
+        for (int64_t i = 0; i < count;) {
+            GradArgs a;
+            a.count = 0;
+            unsigned nb = 0;
+            for (; i < count && a.count < GRAD_TENSORS; ++i)
+                if (grads[i].n > 0 && (pass == 0 || grads[i].dst)) {
+                    a.t[a.count++] = GradTensor{grads[i].src, grads[i].dst, grads[i].n, nb, (int)grads[i].dtype};
+                    nb += (unsigned)((grads[i].n + GRAD_CHUNK - 1) / GRAD_CHUNK);
+                }
+            if (!nb) continue;
+            if (pass == 0) vq_grad_norm_kernel<<<dim3(nb), 256, 0, st>>>(a, partial + done);
+            else vq_grad_scale_kernel<<<dim3(nb), 256, 0, st>>>(a, coef);
+            done += nb;
+        }
+        if (pass == 0) vq_grad_coef_kernel<<<1, 256, 0, st>>>(partial, done, max_norm, eps, norm, coef);
+    }
+    return vq_launch_status("vqhip_clip_grads");
+}

@@ -18,6 +18,7 @@ import torch.distributed as dist
 from torch import Tensor, nn
 
 from . import _lib as L
+from .beam import BEAM_MAX, beam_reorder, beam_select
 from .vector_quantize import VectorQuantize, _rows_of, other_float_dtypes_as_fp32
 
 
@@ -544,46 +545,54 @@ class ResidualVQ(nn.Module):
         return quantized_out, idx, losses
 
     # ---- beam search over the quantizers (rvq.py:445-590): every stage keeps the `beam_size` best partial code
-    #      sequences by accumulated (weighted) negative commit loss; the per-stage top-k comes from the dense-score path ----
+    #      sequences by accumulated (weighted) negative commit loss; the per-stage top-k comes from the dense-score path.  The J x K
+    #      continuations of a row are never formed: the survivors are selected from their losses (beam_select), then the states of
+    #      their beams and the codes they continue with are gathered (beam_reorder, one launch each) ----
     def _forward_beam(self, x, mask, sample_codebook_temp, freeze_codebook, beam_size, drop_at):
         lead = x.shape[:-1]
-        J = 1
-        scores = torch.zeros(*lead, 1, device=x.device, dtype=x.dtype)
+        scores = torch.zeros(*lead, 1, device=x.device, dtype=torch.float32)                # [b, n, J]
         residual = x[..., None, :]                                  # [b, n, J, d]
         out = torch.zeros_like(residual)
-        inputs = torch.empty(*lead, 1, 0, x.shape[-1], device=x.device, dtype=x.dtype)     # [b, n, J, l, d] stage inputs
-        idxs = torch.empty(*lead, 1, 0, device=x.device, dtype=torch.long)                  # [b, n, J, l]
-        losses = torch.empty(*lead, 1, 0, device=x.device, dtype=torch.float32)             # [b, n, J, l]
+        idxs, losses, inputs = [], [], []                           # per stage so far: [b, n, J] | [b, n, J] | [b, n, J, d] (stage inputs)
         last = (len(self.layers) - 1) if drop_at is None else drop_at
+        want_inputs = self.training and self.shared_codebook and self.layers[0]._codebook.has_dead_code_replacement
 
-        def pick(t, sel):                                           # t [b, n, J', ...] -> rows `sel` [b, n, keep] of the beam axis
-            extra = t.ndim - sel.ndim
-            s_ = sel.reshape(*sel.shape, *([1] * extra)).expand(*sel.shape, *t.shape[sel.ndim:])
-            return t.gather(sel.ndim - 1, s_)
-
-        for qi, vq in enumerate(self.layers):
-            if drop_at is not None and qi > drop_at:
-                idxs = torch.nn.functional.pad(idxs, (0, 1), value=-1)
-                losses = torch.nn.functional.pad(losses, (0, 1), value=0.)
-                continue
-            inputs = torch.cat((inputs, residual[..., None, :]), dim=-2)
+        for qi, vq in enumerate(self.layers[:last + 1]):
             quantized, ind, loss = vq(residual, mask=mask, sample_codebook_temp=sample_codebook_temp,
                                       freeze_codebook=freeze_codebook, topk=beam_size)       # [b,n,J,K,d], [b,n,J,K], [b,n,J,K]
-            K = ind.shape[-1]
-            scores = (scores[..., None] - loss * self.beam_score_weights[qi]).flatten(-2)   # [b, n, J K]
-            step = quantized.detach() if self.quant_grad_frac <= 0 else (
-                self.quant_grad_frac * quantized + (1. - self.quant_grad_frac) * quantized.detach())
-            residual = (residual[..., None, :] - step).flatten(-3, -2)
-            out = (out[..., None, :] + quantized).flatten(-3, -2)
-            inputs = inputs[..., None, :, :].expand(*inputs.shape[:-2], K, *inputs.shape[-2:]).flatten(-4, -3)
-            idxs = torch.cat((idxs[..., None, :].expand(*idxs.shape[:-1], K, idxs.shape[-1]), ind[..., None]), dim=-1).flatten(-3, -2)
-            losses = torch.cat((losses[..., None, :].expand(*losses.shape[:-1], K, losses.shape[-1]), loss[..., None].float()), dim=-1).flatten(-3, -2)
+            if loss.shape != ind.shape:
+                raise RuntimeError("ResidualVQ: beam search scores codes by their commitment loss, which exists in training and with "
+                                   "commitment_weight > 0 only")
+            J, K = ind.shape[-2:]
+            gain = -(loss.detach().float() * self.beam_score_weights[qi])                    # [b, n, J, K]
             keep = beam_size if qi != last else 1
-            if scores.shape[-1] > keep:
-                scores, sel = scores.topk(keep, dim=-1)
-                residual, out, idxs, losses, inputs = (pick(t, sel) for t in (residual, out, idxs, losses, inputs))
+            if J * K <= keep:                                       # everything survives, in place
+                scores = (scores[..., None] + gain).flatten(-2)
+                at = torch.arange(J * K, device=x.device).expand(*lead, J * K)
+                parents = at // K
+            elif max(J, keep) <= BEAM_MAX:
+                scores, parents, tokens = beam_select(gain, scores, keep, normalize=False)
+                at = parents * K + tokens
+            else:
+                scores, at = (scores[..., None] + gain).flatten(-2).topk(keep, dim=-1)
+                parents = at // K
+            if want_inputs:
+                inputs.append(residual)
+            n = len(idxs)
+            residual, out, *rest = beam_reorder([residual, out, *idxs, *losses, *inputs], parents)
+            idxs, losses, inputs = rest[:n], rest[n:2 * n], rest[2 * n:]
+            code, ind, loss = beam_reorder([quantized.flatten(-3, -2), ind.flatten(-2), loss.float().flatten(-2)], at)
+            step = code.detach() if self.quant_grad_frac <= 0 else (
+                self.quant_grad_frac * code + (1. - self.quant_grad_frac) * code.detach())
+            residual = residual - step
+            out = out + code
+            idxs.append(ind)
+            losses.append(loss)
 
-        out, idxs, losses, inputs = out[..., 0, :], idxs[..., 0, :], losses[..., 0, :], inputs[..., 0, :, :]
+        dropped = len(self.layers) - len(idxs)
+        out = out[..., 0, :]
+        idxs = torch.nn.functional.pad(torch.stack([t[..., 0] for t in idxs], dim=-1), (0, dropped), value=-1)
+        losses = torch.nn.functional.pad(torch.stack([t[..., 0] for t in losses], dim=-1), (0, dropped), value=0.)
         if mask is not None:
             losses = torch.where(mask[..., None], losses, torch.zeros_like(losses))
             losses = losses.flatten(0, -2).sum(0) / mask.sum().clamp_min(1e-4)
@@ -593,12 +602,13 @@ class ResidualVQ(nn.Module):
             # rvq.py:574, 586-589.  REFERENCE QUIRK, replicated for parity: `all_residuals[..., 0, :]` selects stage 0 (not beam 0)
             # of the [.., beam, stage, d] tensor, the following unbind runs over the beam axis (length 1), and the zip therefore
             # stops after the FIRST quantizer: only layer 0 receives EMA statistics after a beam search.
-            self.layers[0].update_indices(inputs[..., 0, :], idxs[..., 0], mask=mask)
+            self.layers[0].update_indices(x, idxs[..., 0], mask=mask)                        # (stage 0's input is x)
             if self.shared_codebook:
                 shared = self.layers[0]
                 if self.vq_is_ema_updating:
                     shared._codebook.update_ema()
                 if shared._codebook.has_dead_code_replacement:
+                    inputs = torch.stack([t[..., 0, :] for t in inputs], dim=-2)             # [b, n, l, d]
                     shared.expire_codes_(inputs.reshape(inputs.shape[0], -1, inputs.shape[-1]))
         return out, idxs, losses
 

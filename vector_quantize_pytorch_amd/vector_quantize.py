@@ -21,6 +21,7 @@ from torch import Tensor, nn
 
 from . import _lib as L
 from .codebook import Codebook
+from .grads import clip_grad_norm_
 
 LossBreakdown = namedtuple('LossBreakdown', ['commitment', 'codebook_diversity', 'orthogonal_reg', 'inplace_optimize'])
 
@@ -372,8 +373,11 @@ class VectorQuantize(nn.Module):
         return_zeros_for_masked_padding=True,
         route_gradients_to_input=True,
         shard_codebook=False,
+        in_place_codebook_max_grad_norm: Optional[float] = None,
     ):
-        """Constructor keywords = the reference's (vqp.py:803-849) plus ONE extension: `shard_codebook=True` partitions the
+        """Constructor keywords = the reference's (vqp.py:803-849) plus two extensions.  `in_place_codebook_max_grad_norm` clips the
+        gradients that the in-place optimizer steps on to this global 2-norm (after their all-reduce over the ranks; `clip_grad_norm_`,
+        no host read).  `shard_codebook=True` partitions the
         codebook over the ranks of the default process group (rank p owns codes [p C/P, (p+1) C/P)): every
         rank searches its shard with the HIP kernels and ONE RCCL all-reduce(MAX) of packed (score, index) keys picks the
         global winner with the reference's tie rule (parallel.ShardedVectorQuantize).  EMA codebooks with heads == 1 only."""
@@ -496,6 +500,9 @@ class VectorQuantize(nn.Module):
         self.in_place_codebook_optimizer = in_place_codebook_optimizer(self._codebook.parameters()) \
             if in_place_codebook_optimizer is not None else None
         self.manual_in_place_optimizer_update = manual_in_place_optimizer_update
+        assert in_place_codebook_max_grad_norm is None or (in_place_codebook_optimizer is not None and in_place_codebook_max_grad_norm >= 0.), \
+            'in_place_codebook_max_grad_norm bounds the gradients of an in_place_codebook_optimizer'
+        self.in_place_codebook_max_grad_norm = in_place_codebook_max_grad_norm
         self.register_buffer('zero', torch.tensor(0.), persistent=False)
 
     # ---- reference-compatible accessors (vqp.py:978-1022) -----------------------------------------
@@ -544,6 +551,8 @@ class VectorQuantize(nn.Module):
                 if param.grad is not None:
                     dist.all_reduce(param.grad)
                     param.grad /= dist.get_world_size()
+        if self.in_place_codebook_max_grad_norm is not None:
+            clip_grad_norm_(self._codebook.parameters(), self.in_place_codebook_max_grad_norm)
         self.in_place_codebook_optimizer.step()
         self.in_place_codebook_optimizer.zero_grad()
 
