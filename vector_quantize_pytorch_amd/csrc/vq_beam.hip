@@ -8,6 +8,10 @@
 // c[b, j, v] = s[b, j] + (l[b, j, v] - lse[b, j]) (normalize) or s + l; a finished beam has one continuation, c = s at end_token; what
 // the mask leaves out, and every sum that is not a number, is -inf.  Out: the K largest c of a batch entry, equal ones by ascending
 // j * V + v.  Sums and comparisons are 64-bit: two continuations of different beams may be closer than fp32 resolves.
+//
+// Within a row c grows with l, so the K best of a row are the K largest l.  Two launches: vq_beam_rows_kernel reads every logit once
+// (its tile stays in registers), and leaves of each tile the log-sum's maximum and sum and its K largest logits; vq_beam_merge_kernel
+// joins the tiles of a batch entry's rows.  Bound by the read of the logits.  vq_beam_small_kernel does small entries in one launch.
 struct SelArgs {
     const void *logits; int64_t lb, lj;                 // element strides of batch and beam
     const float *scores;                                // [B, J] or null (zeros)
@@ -15,6 +19,8 @@ struct SelArgs {
     const uint8_t *finished;                            // [B, J] or null
     float *scores_out; int64_t *parents_out, *tokens_out; double *lse_out;
     int64_t B; int J, V, K, end_token, normalize;
+    // per (row, tile): the K largest (logit, token), unused ones -inf; maximum and sum of exp(l - maximum)
+    int2 *part; double *part_sum; float *part_max; int tiles;
 };
 
 __device__ __forceinline__ double sel_sum(double score, double x)
@@ -23,80 +29,380 @@ __device__ __forceinline__ double sel_sum(double score, double x)
     return c != c ? -INFINITY : c;
 }
 
-template <typename T> __global__ void __launch_bounds__(256) vq_beam_select_kernel(const SelArgs a)
+__device__ __forceinline__ bool sel_before(double c, int i, double d, int k) { return c > d || (c == d && i < k); }
+
+// the entry's last survivors where fewer than K continuations are above -inf: the first places, by number, that are not among the `found`
+// ones.  One thread.
+__device__ void sel_fill(const SelArgs &a, int64_t b, int found)
 {
-    extern __shared__ double smem[];
-    double *lse = smem, *red = smem + a.J;              // [J], [256]
-    int *redi = (int *)(red + 256);                     // [256]
-    const int64_t b = blockIdx.x;
-    const int t = threadIdx.x, J = a.J, V = a.V;
-    const T *lg = (const T *)a.logits + b * a.lb;
-    const uint8_t *mk = a.mask ? a.mask + b * a.mb : nullptr;
-    for (int j = 0; j < J; ++j) {
-        double out = 0.0;
-        if (a.normalize) {
-            const T *row = lg + j * a.lj;
-            const uint8_t *m = mk ? mk + j * a.mj : nullptr;
-            double mx = -INFINITY;
-            for (int v = t; v < V; v += 256)
-                if (!m || m[v]) mx = fmax(mx, (double)(float)row[v]);
-            red[t] = mx;
-            __syncthreads();
-            for (int o = 128; o; o >>= 1) {
-                if (t < o) red[t] = fmax(red[t], red[t + o]);
-                __syncthreads();
-            }
-            mx = red[0];
-            __syncthreads();
-            double s = 0.0;
-            for (int v = t; v < V; v += 256)
-                if (!m || m[v]) s += exp((double)(float)row[v] - mx);
-            red[t] = s;
-            __syncthreads();
-            for (int o = 128; o; o >>= 1) {
-                if (t < o) red[t] += red[t + o];
-                __syncthreads();
-            }
-            out = mx + log(red[0]);
-            __syncthreads();
+    int place = 0;
+    for (int r = found; r < a.K; ++r, ++place) {
+        for (bool taken = true; taken;) {
+            taken = false;
+            for (int i = 0; i < found; ++i)
+                if (a.parents_out[b * a.K + i] * a.V + a.tokens_out[b * a.K + i] == place) taken = true;
+            if (taken) ++place;
         }
-        if (t == 0) {
-            lse[j] = out;
-            if (a.lse_out) a.lse_out[b * J + j] = out;
+        a.scores_out[b * a.K + r] = -INFINITY;
+        a.parents_out[b * a.K + r] = place / a.V;
+        a.tokens_out[b * a.K + r] = place % a.V;
+    }
+}
+
+// ---- small entries: J * V <= 64, W = a power of two >= J * V lanes of a wave each, one continuation a lane.  A survivor's rank is the
+// number of continuations before it.  Bound by the launch.
+template <typename T> __global__ void __launch_bounds__(256) vq_beam_small_kernel(const SelArgs a, int W)
+{
+    const int lane = threadIdx.x & 63, i = lane & (W - 1), base = lane - i, J = a.J, V = a.V;
+    const int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
+    const bool in = b < a.B && i < J * V;
+    const int64_t bb = b < a.B ? b : 0;
+    const int j = in ? i / V : 0, v = in ? i - j * V : 0;
+    double x = -INFINITY, s = 0.0;
+    bool fin = false;
+    if (in) {
+        if (a.scores) s = a.scores[bb * J + j];
+        fin = a.finished && a.finished[bb * J + j];
+        if (!fin && (!a.mask || a.mask[bb * a.mb + j * a.mj + v])) x = (double)(float)((const T *)a.logits)[bb * a.lb + j * a.lj + v];
+    }
+    if (a.normalize) {
+        const int row = base + j * V;
+        double m = -INFINITY, e = 0.0;
+        for (int t = 0; t < V; ++t) m = fmax(m, __shfl(x, row + t, 64));
+        const double mine = exp(x - m);
+        for (int t = 0; t < V; ++t) e += __shfl(mine, row + t, 64);
+        const double lse = m + log(e);
+        if (in && v == 0 && a.lse_out) a.lse_out[bb * J + j] = lse;
+        x -= lse;
+    }
+    if (fin) x = v == a.end_token ? 0.0 : -INFINITY;
+    const double c = in ? sel_sum(s, x) : -INFINITY;
+    int rank = 0;
+    for (int t = 0; t < J * V; ++t) rank += sel_before(__shfl(c, base + t, 64), t, c, i) ? 1 : 0;
+    if (in && rank < a.K) {
+        a.scores_out[b * a.K + rank] = (float)c;
+        a.parents_out[b * a.K + rank] = j;
+        a.tokens_out[b * a.K + rank] = v;
+    }
+}
+
+// ---- rows -------------------------------------------------------------------------------------------------------------------------
+#define SEL_CAP 512            // continuations of a tile that the first bound lets through before it is made exact
+
+__device__ __forceinline__ unsigned sel_order(float f)       // ascending like f; NaN never gets here
+{
+    const unsigned u = __float_as_uint(f + 0.f);              // (-0 + 0 = 0: the zeros are equal)
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// exp(x) for x <= 0 to about one step of fp32: v_exp_f32 takes 2^t, and the rounding of t = x log2(e), which grows with |x|, is put back
+// to first order
+__device__ __forceinline__ float sel_exp(float x)
+{
+    x = fmaxf(x, -100.f);                                     // (nothing below counts; -inf would make the correction NaN)
+    const float t = x * 1.44269504f;
+    const float r = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0.693147181f, e);
+}
+
+// NT threads hold a tile of NT * E logits in registers, 8 consecutive ones of every NT * 8 each.  The K best:
+//   1. a bound: the threads form 64 groups; the K-th largest of the groups' maxima has at least K logits at or above it;
+//   2. what reaches the bound is collected (on unordered data about K + K^2 / 128);
+//   3. where more than SEL_CAP do (ties, runs), the K-th largest is found by bisection over value and place, and exactly K collected;
+//   4. each collected one's rank is the number of those before it.
+template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bounds__(NT) vq_beam_rows_kernel(const SelArgs a)
+{
+    constexpr int NW = NT / 64, NU = E / 8;
+    __shared__ float group_max[64];
+    __shared__ double wave_sum[NW];
+    __shared__ int wave_cnt[NW], found;
+    __shared__ int2 list[SEL_CAP];
+    const int t = threadIdx.x, V = a.V, K = a.K;
+    const unsigned tile = blockIdx.x % a.tiles;
+    const int64_t row = blockIdx.x / a.tiles, b = row / a.J;
+    const int j = (int)(row - b * a.J);
+    // a finished beam's logits are not used, nor are those of a beam without a score: the merge knows
+    if (a.finished && a.finished[row]) return;
+    if (a.scores && !(a.scores[row] > -INFINITY)) return;
+    const T *lg = (const T *)a.logits + b * a.lb + j * a.lj;
+    const uint8_t *mk = MASKED ? a.mask + b * a.mb + j * a.mj : nullptr;
+    const int64_t first = (int64_t)tile * (NT * E);
+    float x[E];
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int64_t at = first + (int64_t)(u * NT + t) * 8;
+        unsigned long long live = ~0ull;
+        if (MASKED && at + 8 <= V) {
+            const VqVec<uint8_t, 8> m = vq_ldv<uint8_t, 8>(mk + at);
+            __builtin_memcpy(&live, &m, 8);
+        }
+        if (at + 8 <= V) {
+            if (!MASKED || live) {
+                const VqVec<T, 8> r = vq_ldv<T, 8>(lg + at);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u * 8 + i] = !MASKED || ((live >> (8 * i)) & 0xff) ? (float)r.v[i] : -INFINITY;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u * 8 + i] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[u * 8 + i] = at + i < V && (!MASKED || mk[at + i]) ? (float)lg[at + i] : -INFINITY;
+        }
+    }
+    float mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        bad |= x[i] != x[i];
+        mine = fmaxf(mine, x[i]);                             // (a NaN is passed over)
+    }
+    // 1. 64 groups of NT / 64 threads; lane g of every wave ranks group g
+    float gm = mine;
+#pragma unroll
+    for (int o = 1; o < NT / 64; o <<= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
+    if (t % (NT / 64) == 0) group_max[t / (NT / 64)] = gm;
+    if (t == 0) found = 0;
+    __syncthreads();
+    gm = group_max[t & 63];
+    int place = 0;
+#pragma unroll
+    for (int k = 0; k < 64; ++k) {
+        const float o = group_max[k];
+        place += o > gm || (o == gm && k < (t & 63)) ? 1 : 0;
+    }
+    const float bound = __shfl(gm, __builtin_ctzll(__ballot(place == K - 1)), 64), mx = __shfl(gm, __builtin_ctzll(__ballot(place == 0)), 64);
+    // 2. and the log-sum: sums of 8 in 32 bits, the rest in 64
+    if (mine >= bound && mine > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (x[i] >= bound && x[i] > -INFINITY) {
+                const int at = atomicAdd(&found, 1);
+                if (at < SEL_CAP) list[at] = make_int2(__float_as_int(x[i]), (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8));
+            }
+    }
+    if (a.normalize) {
+        double s = bad ? (double)NAN : 0.0;
+        if (mx > -INFINITY && mx < INFINITY) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                float q = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q += sel_exp(x[u * 8 + i] - mx);
+                s += q;
+            }
+        } else if (mx == INFINITY) s = NAN;                   // a log-sum of +inf: no continuation
+        s = vq_wave_sum(s);
+        if ((t & 63) == 0) wave_sum[t >> 6] = s;
+    }
+    __syncthreads();
+    int n = found;
+    if (n > SEL_CAP) {
+        // 3. the K-th largest value, then the last place among those equal to it
+        auto count = [&](auto &&pred) {
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) c += pred(x[i], (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8)) ? 1 : 0;
+            c = vq_wave_sum(c);
+            __syncthreads();
+            if ((t & 63) == 0) wave_cnt[t >> 6] = c;
+            __syncthreads();
+            c = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) c += wave_cnt[w];
+            return c;
+        };
+        unsigned kth = 0;
+        for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
+            const unsigned want = kth | bit;
+            if (count([&](float f, int) { return f > -INFINITY && sel_order(f) >= want; }) >= K) kth = want;
+        }
+        const int above = count([&](float f, int) { return f > -INFINITY && sel_order(f) > kth; });
+        unsigned lo = (unsigned)first, hi = (unsigned)(first + NT * E - 1 < V - 1 ? first + NT * E - 1 : V - 1);
+        while (lo < hi) {                                     // the least place with `above` + (equal ones up to it) >= K
+            const unsigned mid = lo + (hi - lo) / 2;
+            if (above + count([&](float f, int p) { return f > -INFINITY && sel_order(f) == kth && (unsigned)p <= mid; }) >= K) hi = mid; else lo = mid + 1;
+        }
+        __syncthreads();
+        if (t == 0) found = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int p = (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8);
+            const unsigned u = sel_order(x[i]);
+            if (x[i] > -INFINITY && (u > kth || (u == kth && (unsigned)p <= lo))) list[atomicAdd(&found, 1)] = make_int2(__float_as_int(x[i]), p);
+        }
+        __syncthreads();
+        n = found;
+    }
+    // 4.
+    int2 *out = a.part + (int64_t)blockIdx.x * K;
+    for (int i = t; i < n; i += NT) {
+        const int2 me = list[i];
+        const float f = __int_as_float(me.x);
+        int rank = 0;
+        for (int k = 0; k < n; ++k) {
+            const int2 o = list[k];
+            const float g = __int_as_float(o.x);
+            rank += g > f || (g == f && o.y < me.y) ? 1 : 0;
+        }
+        if (rank < K) out[rank] = me;
+    }
+    for (int i = n + t; i < K; i += NT) out[i] = make_int2(__float_as_int(-INFINITY), 0);
+    if (t == 0) {
+        double s = 0.0;
+        if (a.normalize)
+            for (int w = 0; w < NW; ++w) s += wave_sum[w];
+        a.part_max[blockIdx.x] = mx;
+        a.part_sum[blockIdx.x] = s;
+    }
+}
+
+// ---- merge: one workgroup per batch entry -------------------------------------------------------------------------------------------
+// The rows' log-sums from their tiles (16 lanes a row), then the K best of J * tiles * K (and the finished beams') by the same bound and
+// ranks in 64 bits; where ties let more than SEL_CAP through, K rounds that each find the next one.  Bound by latency.
+__global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
+{
+    __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], group_max[64], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
+    __shared__ int ps[SEL_CAP], found;
+    __shared__ uint8_t fin[VQHIP_BEAM_MAX];
+    __shared__ double rc[4];
+    __shared__ int rp[4];
+    const int t = threadIdx.x, J = a.J, S = a.tiles, K = a.K;
+    const int64_t b = blockIdx.x;
+    for (int j = t >> 4; j < J; j += 16) {
+        const int64_t row = b * J + j;
+        const double s = a.scores ? (double)a.scores[row] : 0.0;
+        const bool f = a.finished && a.finished[row], live = !f && s > -INFINITY;
+        double lse = 0.0;
+        if (live && a.normalize) {
+            float m = -INFINITY;
+            for (int q = t & 15; q < S; q += 16) m = fmaxf(m, a.part_max[row * S + q]);
+            for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            double sum = 0.0;
+            for (int q = t & 15; q < S; q += 16) {
+                const float pm = a.part_max[row * S + q];
+                const double p = a.part_sum[row * S + q];
+                sum += p == 0.0 ? 0.0 : p * exp((double)pm - (double)m);
+            }
+            for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            lse = (double)m + log(sum);                        // (no logit admitted: -inf, and NaN below)
+        }
+        if ((t & 15) == 0) {
+            fin[j] = f;
+            base[j] = !live ? (f ? s : -INFINITY) : !(lse > -INFINITY && lse < INFINITY) ? -INFINITY : s;
+            if (live && a.normalize && !(lse > -INFINITY && lse < INFINITY)) lse = INFINITY;
+            if (a.lse_out) a.lse_out[row] = lse;
+            log_sum[j] = lse;
+        }
+    }
+    if (t == 0) found = 0;
+    __syncthreads();
+    const int per = S * K, total = J * per;
+    // candidate i: list entry i % per of row i / per; a finished beam's first entry is its only continuation
+    auto at = [&](int i, int &place) -> double {
+        const int j = i / per, e = i - j * per;
+        const double s = base[j];
+        if (fin[j]) {
+            place = j * a.V + a.end_token;
+            return e ? -INFINITY : sel_sum(s, 0.0);
+        }
+        if (!(s > -INFINITY)) { place = 0; return -INFINITY; }
+        const int2 q = a.part[(b * J + j) * (int64_t)per + e];
+        place = j * a.V + q.y;
+        const double l = (double)__int_as_float(q.x);
+        return l > -INFINITY ? sel_sum(s, l - log_sum[j]) : -INFINITY;
+    };
+    int place;
+    double best = -INFINITY;
+    for (int i = t; i < total; i += 256) best = fmax(best, at(i, place));
+    best = fmax(best, __shfl_xor(best, 1, 64));
+    best = fmax(best, __shfl_xor(best, 2, 64));
+    if ((t & 3) == 0) group_max[t >> 2] = best;
+    __syncthreads();
+    best = group_max[t & 63];
+    int order = 0;
+#pragma unroll
+    for (int k = 0; k < 64; ++k) {
+        const double o = group_max[k];
+        order += o > best || (o == best && k < (t & 63)) ? 1 : 0;
+    }
+    const double bound = __shfl(best, __builtin_ctzll(__ballot(order == K - 1)), 64);
+    for (int i = t; i < total; i += 256) {
+        const double c = at(i, place);
+        if (c >= bound && c > -INFINITY) {
+            const int k = atomicAdd(&found, 1);
+            if (k < SEL_CAP) { cs[k] = c; ps[k] = place; }
         }
     }
     __syncthreads();
-    double last = INFINITY;
-    int lasti = -1;
-    const int total = J * V;
-    for (int k = 0; k < a.K; ++k) {
-        double best = -INFINITY;
-        int bi = 0x7fffffff;
-        for (int i = t; i < total; i += 256) {
-            const int j = i / V, v = i - j * V;
-            const double s = a.scores ? (double)a.scores[b * J + j] : 0.0;
-            double c;
-            if (a.finished && a.finished[b * J + j]) c = sel_sum(s, v == a.end_token ? 0.0 : -INFINITY);
-            else if (mk && !mk[j * a.mj + v]) c = -INFINITY;
-            else c = sel_sum(s, (double)(float)lg[j * a.lj + v] - lse[j]);
-            const bool open = c < last || (c == last && i > lasti);
-            if (open && (c > best || (c == best && i < bi))) { best = c; bi = i; }
+    int n = found;
+    if (n <= SEL_CAP) {
+        for (int i = t; i < n; i += 256) {
+            const double c = cs[i];
+            const int p = ps[i];
+            int rank = 0;
+            for (int k = 0; k < n; ++k) rank += sel_before(cs[k], ps[k], c, p) ? 1 : 0;
+            if (rank < K) {
+                a.scores_out[b * K + rank] = (float)c;
+                a.parents_out[b * K + rank] = p / a.V;
+                a.tokens_out[b * K + rank] = p % a.V;
+            }
         }
-        red[t] = best;
-        redi[t] = bi;
-        __syncthreads();
-        for (int o = 128; o; o >>= 1) {
-            if (t < o && (red[t + o] > red[t] || (red[t + o] == red[t] && redi[t + o] < redi[t]))) { red[t] = red[t + o]; redi[t] = redi[t + o]; }
+        n = n < K ? n : K;
+    } else {
+        double last = INFINITY;
+        int lastp = -1;
+        for (n = 0; n < K; ++n) {
+            double c = -INFINITY;
+            int p = 0x7fffffff;
+            for (int i = t; i < total; i += 256) {
+                const double d = at(i, place);
+                if (sel_before(last, lastp, d, place) && d > -INFINITY && sel_before(d, place, c, p)) { c = d; p = place; }
+            }
+            for (int o = 32; o; o >>= 1) {
+                const double d = __shfl_xor(c, o, 64);
+                const int q = __shfl_xor(p, o, 64);
+                if (sel_before(d, q, c, p)) { c = d; p = q; }
+            }
+            if ((t & 63) == 0) { rc[t >> 6] = c; rp[t >> 6] = p; }
             __syncthreads();
+            for (int w = 0; w < 4; ++w)
+                if (sel_before(rc[w], rp[w], c, p)) { c = rc[w]; p = rp[w]; }
+            __syncthreads();
+            if (!(c > -INFINITY)) break;
+            last = c; lastp = p;
+            if (t == 0) {
+                a.scores_out[b * K + n] = (float)c;
+                a.parents_out[b * K + n] = p / a.V;
+                a.tokens_out[b * K + n] = p % a.V;
+            }
         }
-        last = red[0];
-        lasti = redi[0];
-        __syncthreads();
-        if (t == 0) {
-            a.scores_out[b * a.K + k] = (float)last;
-            a.parents_out[b * a.K + k] = lasti / V;
-            a.tokens_out[b * a.K + k] = lasti % V;
-        }
+    }
+    __syncthreads();
+    if (t == 0 && n < K) sel_fill(a, b, n);
+}
+
+// tiles of the rows: one wave for rows of up to 512 logits; 8192 logits a workgroup where that gives each CU two, else 2048
+struct SelPlan { int small, threads, per_thread, tiles; };
+static SelPlan sel_plan(int64_t B, int64_t J, int64_t V)
+{
+    if (J * V <= 64) return SelPlan{1, 0, 0, 0};
+    if (V <= 512) return SelPlan{0, 64, 8, 1};
+    const bool big = B * J * ((V + 8191) / 8192) >= 512;
+    return SelPlan{0, 256, big ? 32 : 8, (int)(big ? (V + 8191) / 8192 : (V + 2047) / 2048)};
+}
+
+template <typename T> static void sel_rows(const SelArgs &a, const SelPlan &p, hipStream_t st)
+{
+    const dim3 grid((unsigned)(a.B * a.J * p.tiles));
+    if (p.threads == 64) {
+        if (a.mask) vq_beam_rows_kernel<T, 64, 8, true><<<grid, 64, 0, st>>>(a); else vq_beam_rows_kernel<T, 64, 8, false><<<grid, 64, 0, st>>>(a);
+    } else if (p.per_thread == 8) {
+        if (a.mask) vq_beam_rows_kernel<T, 256, 8, true><<<grid, 256, 0, st>>>(a); else vq_beam_rows_kernel<T, 256, 8, false><<<grid, 256, 0, st>>>(a);
+    } else {
+        if (a.mask) vq_beam_rows_kernel<T, 256, 32, true><<<grid, 256, 0, st>>>(a); else vq_beam_rows_kernel<T, 256, 32, false><<<grid, 256, 0, st>>>(a);
     }
 }
 
@@ -105,9 +411,9 @@ static int sel_check(const vqhip_beam_select_t *p, const char *what)
     if (!p) VQ_FAIL(VQHIP_EINVAL, "%s: null argument", what);
     if (!vq_elem_bytes(p->dtype)) VQ_FAIL(VQHIP_EINVAL, "%s: dtype %lld", what, (long long)p->dtype);
     if (p->B < 0 || p->J < 1 || p->V < 1 || p->K < 1) VQ_FAIL(VQHIP_EINVAL, "%s: B %lld, J %lld, V %lld, K %lld", what, (long long)p->B, (long long)p->J, (long long)p->V, (long long)p->K);
-    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->B > 0x7fffffff || p->V > 0x7fffffff / p->J || p->K > p->J * p->V)
-        VQ_FAIL(VQHIP_EDIM, "%s: %lld beams, %lld kept of %lld x %lld continuations: at most %d beams, %d kept, 2^31 - 1 continuations", what,
-                (long long)p->J, (long long)p->K, (long long)p->J, (long long)p->V, VQHIP_BEAM_MAX, VQHIP_BEAM_MAX);
+    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->V > (1 << 30) / p->J || p->K > p->J * p->V || p->B > 0x7fffffff / p->J / ((p->V + 2047) / 2048))
+        VQ_FAIL(VQHIP_EDIM, "%s: %lld entries, %lld kept of %lld x %lld continuations: at most %d beams, %d kept, 2^30 continuations an entry, 2^31 tiles in all",
+                what, (long long)p->B, (long long)p->K, (long long)p->J, (long long)p->V, VQHIP_BEAM_MAX, VQHIP_BEAM_MAX);
     if (p->finished && (p->end_token < 0 || p->end_token >= p->V)) VQ_FAIL(VQHIP_EINVAL, "%s: end token %lld outside [0, %lld)", what, (long long)p->end_token, (long long)p->V);
     if (p->B > 0 && (!p->logits || !p->parents || !p->tokens || !p->out_scores)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
     return 0;
@@ -115,8 +421,8 @@ static int sel_check(const vqhip_beam_select_t *p, const char *what)
 
 extern "C" size_t vqhip_beam_select_workspace_bytes(int64_t B, int64_t J, int64_t V, int64_t K)
 {
-    (void)B; (void)J; (void)V; (void)K;
-    return 0;
+    if (B <= 0 || J <= 0 || V <= 0 || K <= 0 || J > VQHIP_BEAM_MAX || V > (1 << 30) / J) return 0;
+    return (size_t)(B * J * sel_plan(B, J, V).tiles) * (size_t)(8 * K + 12);
 }
 
 extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
@@ -124,66 +430,126 @@ extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
     int rc = sel_check(p, "vqhip_beam_select");
     if (rc) return rc;
     if (p->B == 0) return 0;
+    const size_t need = vqhip_beam_select_workspace_bytes(p->B, p->J, p->V, p->K);
+    if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select: workspace of %zu bytes, needs %zu", p->workspace_bytes, need);
     SelArgs a;
     a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.scores = p->scores;
     a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j; a.finished = p->finished;
     a.scores_out = p->out_scores; a.parents_out = p->parents; a.tokens_out = p->tokens; a.lse_out = p->lse;
     a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.end_token = (int)p->end_token; a.normalize = p->normalize != 0;
-    const size_t sm = (size_t)(a.J + 256) * 8 + 256 * 4;
-    const dim3 grid((unsigned)p->B);
-    if (p->dtype == VQHIP_F32) vq_beam_select_kernel<float><<<grid, 256, sm, (hipStream_t)stream>>>(a);
-    else if (p->dtype == VQHIP_BF16) vq_beam_select_kernel<__bf16><<<grid, 256, sm, (hipStream_t)stream>>>(a);
-    else vq_beam_select_kernel<_Float16><<<grid, 256, sm, (hipStream_t)stream>>>(a);
+    const SelPlan plan = sel_plan(p->B, p->J, p->V);
+    hipStream_t st = (hipStream_t)stream;
+    if (plan.small) {
+        int W = 1;
+        while (W < a.J * a.V) W <<= 1;
+        const dim3 grid((unsigned)((a.B * W + 255) / 256));
+        if (p->dtype == VQHIP_F32) vq_beam_small_kernel<float><<<grid, 256, 0, st>>>(a, W);
+        else if (p->dtype == VQHIP_BF16) vq_beam_small_kernel<__bf16><<<grid, 256, 0, st>>>(a, W);
+        else vq_beam_small_kernel<_Float16><<<grid, 256, 0, st>>>(a, W);
+        return vq_launch_status("vqhip_beam_select");
+    }
+    const int64_t lists = a.B * a.J * plan.tiles;
+    a.tiles = plan.tiles;
+    a.part = (int2 *)p->workspace; a.part_sum = (double *)(a.part + lists * a.K); a.part_max = (float *)(a.part_sum + lists);
+    if (p->dtype == VQHIP_F32) sel_rows<float>(a, plan, st);
+    else if (p->dtype == VQHIP_BF16) sel_rows<__bf16>(a, plan, st);
+    else sel_rows<_Float16>(a, plan, st);
+    vq_beam_merge_kernel<<<dim3((unsigned)a.B), 256, 0, st>>>(a);
     return vq_launch_status("vqhip_beam_select");
 }
 
 // d_scores[b, j] = sum of g over the kept continuations of beam j; d_logits[b, j, v] = sum of g over those with token v, minus (normalize)
 // d_scores[b, j] * softmax(l)[b, j, v].  A continuation of score -inf is none: its g counts as 0.  Finished beams pass nothing on to logits.
+// One pass: a workgroup reads SEL_BWD logits of a row and writes their gradients; a row without a survivor is written and not read.
 struct SelBwdArgs {
     const void *logits; int64_t lb, lj;
     const uint8_t *mask; int64_t mb, mj;
     const uint8_t *finished; const double *lse;
     const float *scores_out; const int64_t *parents, *tokens; const float *grad;
     void *d_logits; float *d_scores;
-    int64_t B; int J, V, K, normalize;
+    int64_t B; int J, V, K, normalize, tiles;
 };
+#define SEL_BWD 4096
 
-template <typename T> __global__ void __launch_bounds__(256) vq_beam_select_bwd_kernel(const SelBwdArgs a)
+template <typename T, bool MASKED> __global__ void __launch_bounds__(256) vq_beam_select_bwd_kernel(const SelBwdArgs a)
 {
     __shared__ float g[VQHIP_BEAM_MAX];
-    __shared__ int tok[VQHIP_BEAM_MAX];
-    __shared__ int n;
-    __shared__ float onto;
-    const int64_t b = blockIdx.x / a.J;
-    const int j = blockIdx.x % a.J, t = threadIdx.x, V = a.V;
-    if (t == 0) {
-        int m = 0;
-        float s = 0.f;
-        for (int k = 0; k < a.K; ++k)
-            if (a.parents[b * a.K + k] == j && a.scores_out[b * a.K + k] > -INFINITY) {
-                g[m] = a.grad[b * a.K + k];
-                tok[m] = (int)a.tokens[b * a.K + k];
-                s += g[m++];
-            }
-        if (a.d_scores) a.d_scores[b * a.J + j] = s;
-        onto = s;
-        n = a.finished && a.finished[b * a.J + j] ? -1 : m;
+    __shared__ int tok[VQHIP_BEAM_MAX], n_s;
+    __shared__ float onto_s;
+    const unsigned tile = blockIdx.x % a.tiles;
+    const int64_t row = blockIdx.x / a.tiles, b = row / a.J;
+    const int j = (int)(row - b * a.J), t = threadIdx.x, V = a.V;
+    const int first = (int)tile * SEL_BWD, last = V - first < SEL_BWD ? V : first + SEL_BWD;
+    if (t < 64) {                                             // lane k looks at survivor k; the list keeps this tile's
+        const int64_t k = b * a.K + t;
+        const bool mine = t < a.K && a.parents[k] == j && a.scores_out[k] > -INFINITY;
+        const float gk = mine ? a.grad[k] : 0.f;
+        const int tk = mine ? (int)a.tokens[k] : -1;
+        const bool here = mine && tk >= first && tk < last;
+        const unsigned long long hs = __ballot(here);
+        if (here) {
+            const int at = __popcll(hs & ((1ull << t) - 1));
+            g[at] = gk;
+            tok[at] = tk;
+        }
+        const float onto = vq_wave_sum(gk);
+        const bool any = __ballot(mine) != 0;
+        if (t == 0) {
+            if (a.d_scores && tile == 0) a.d_scores[row] = onto;
+            onto_s = onto;
+            n_s = (a.finished && a.finished[row]) || !any ? -1 : __popcll(hs);
+        }
     }
     __syncthreads();
     if (!a.d_logits) return;
-    const T *row = (const T *)a.logits + b * a.lb + j * a.lj;
-    const uint8_t *mk = a.mask ? a.mask + b * a.mb + j * a.mj : nullptr;
-    T *out = (T *)a.d_logits + (b * a.J + j) * (int64_t)V;
-    const double lse = a.normalize ? a.lse[b * a.J + j] : 0.0;
-    for (int v = t; v < V; v += 256) {
-        float d = 0.f;
-        if (n > 0 && (!mk || mk[v])) {
-            for (int i = 0; i < n; ++i)
-                if (tok[i] == v) d += g[i];
-            if (a.normalize) d -= onto * (float)exp((double)(float)row[v] - lse);
+    const int n = n_s;
+    const float onto = onto_s;
+    const T *lg = (const T *)a.logits + b * a.lb + j * a.lj;
+    const uint8_t *mk = MASKED ? a.mask + b * a.mb + j * a.mj : nullptr;
+    T *out = (T *)a.d_logits + row * V;
+    const double lse = a.normalize && n >= 0 ? a.lse[row] : 0.0;
+    const float lh = (float)lse, ll = (float)(lse - (double)lh);             // l - lse in two steps of 32 bits
+#pragma unroll
+    for (int u = 0; u < SEL_BWD / 2048; ++u) {
+        const int at = first + (u * 256 + t) * 8;
+        if (at >= last) break;
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = 0.f;
+        const int have = last - at < 8 ? last - at : 8;
+        if (n >= 0) {
+            if (a.normalize) {
+                VqVec<T, 8> r;
+                if (have == 8) r = vq_ldv<T, 8>(lg + at);
+                else
+                    for (int i = 0; i < 8; ++i) r.v[i] = i < have ? lg[at + i] : (T)0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = -onto * sel_exp(((float)r.v[i] - lh) - ll);
+            }
+            for (int k = 0; k < n; ++k) {
+                const int w = tok[k] - at;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] += w == i ? g[k] : 0.f;
+            }
+            if (MASKED)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = i < have && mk[at + i] ? d[i] : 0.f;
         }
-        out[v] = (T)d;
+        if (have == 8) {
+            VqVec<T, 8> o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.v[i] = (T)d[i];
+            vq_stv<T, 8>(out + at, o);
+        } else
+            for (int i = 0; i < have; ++i) out[at + i] = (T)d[i];
     }
+}
+
+template <typename T> static void sel_bwd(const SelBwdArgs &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)(a.B * a.J * a.tiles));
+    if (a.mask) vq_beam_select_bwd_kernel<T, true><<<grid, 256, 0, st>>>(a);
+    else vq_beam_select_bwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
 }
 
 extern "C" int vqhip_beam_select_bwd(const vqhip_beam_select_t *p, const float *grad, void *d_logits, float *d_scores, void *stream)
@@ -192,16 +558,16 @@ extern "C" int vqhip_beam_select_bwd(const vqhip_beam_select_t *p, const float *
     if (rc) return rc;
     if (p->B == 0 || (!d_logits && !d_scores)) return 0;
     if (!grad || (p->normalize && d_logits && !p->lse)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select_bwd: null pointer");
-    if (p->B * p->J > 0x7fffffff) VQ_FAIL(VQHIP_EDIM, "vqhip_beam_select_bwd: %lld x %lld rows", (long long)p->B, (long long)p->J);
     SelBwdArgs a;
     a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j;
     a.finished = p->finished; a.lse = p->lse; a.scores_out = p->out_scores; a.parents = p->parents; a.tokens = p->tokens; a.grad = grad;
     a.d_logits = d_logits; a.d_scores = d_scores;
     a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.normalize = p->normalize != 0;
-    const dim3 grid((unsigned)(p->B * p->J));
-    if (p->dtype == VQHIP_F32) vq_beam_select_bwd_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-    else if (p->dtype == VQHIP_BF16) vq_beam_select_bwd_kernel<__bf16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-    else vq_beam_select_bwd_kernel<_Float16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    a.tiles = d_logits ? (a.V + SEL_BWD - 1) / SEL_BWD : 1;
+    hipStream_t st = (hipStream_t)stream;
+    if (p->dtype == VQHIP_F32) sel_bwd<float>(a, st);
+    else if (p->dtype == VQHIP_BF16) sel_bwd<__bf16>(a, st);
+    else sel_bwd<_Float16>(a, st);
     return vq_launch_status("vqhip_beam_select_bwd");
 }
 
