@@ -95,16 +95,12 @@ __device__ __forceinline__ unsigned sel_order(float f)       // ascending like f
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// exp(x) for x <= 0 to about one step of fp32: v_exp_f32 takes 2^t, and the rounding of t = x log2(e), which grows with |x|, is put back
-// to first order
-__device__ __forceinline__ float sel_exp(float x)
-{
-    x = fmaxf(x, -100.f);                                     // (nothing below counts; -inf would make the correction NaN)
-    const float t = x * 1.44269504f;
-    const float r = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.693147181f, e);
-}
+__device__ __forceinline__ float sel_value(unsigned u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+
+// exp(x) for x <= 0 (NaN stays NaN, -inf gives 0).  The product's rounding grows with |x|, but so falls the term: a term of weight e^-5
+// is off by 5 steps of fp32, e^-5 of one in the sum.  Measured on normal logits of deviation 1 to 4, 1000 to 131071 of them: log-sums off
+// by 2e-8 to 5e-8 rms, most of it the same for every row (the rounding of log2 e).
+__device__ __forceinline__ float sel_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // NT threads hold a tile of NT * E logits in registers, 8 consecutive ones of every NT * 8 each.  The K best:
 //   1. a bound: the threads form 64 groups; the K-th largest of the groups' maxima has at least K logits at or above it;
@@ -114,77 +110,79 @@ __device__ __forceinline__ float sel_exp(float x)
 template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bounds__(NT) vq_beam_rows_kernel(const SelArgs a)
 {
     constexpr int NW = NT / 64, NU = E / 8;
-    __shared__ float group_max[64];
+    __shared__ float group_max[64], bound_s;
     __shared__ double wave_sum[NW];
     __shared__ int wave_cnt[NW], found;
     __shared__ int2 list[SEL_CAP];
     const int t = threadIdx.x, V = a.V, K = a.K;
-    const unsigned tile = blockIdx.x % a.tiles;
-    const int64_t row = blockIdx.x / a.tiles, b = row / a.J;
-    const int j = (int)(row - b * a.J);
+    const unsigned row = blockIdx.x / (unsigned)a.tiles, tile = blockIdx.x - row * a.tiles, b = row / (unsigned)a.J, j = row - b * a.J;
     // a finished beam's logits are not used, nor are those of a beam without a score: the merge knows
     if (a.finished && a.finished[row]) return;
     if (a.scores && !(a.scores[row] > -INFINITY)) return;
     const T *lg = (const T *)a.logits + b * a.lb + j * a.lj;
     const uint8_t *mk = MASKED ? a.mask + b * a.mb + j * a.mj : nullptr;
-    const int64_t first = (int64_t)tile * (NT * E);
-    float x[E];
-    bool bad = false;
+    const int first = (int)tile * (NT * E);
+    // all loads first: whole vectors, the ones past the row's end moved back into it and put right below
+    VqVec<T, 8> raw[NU];
+    unsigned long long live[NU];
+    if (V >= 8) {
+        if (MASKED)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int at = first + (u * NT + t) * 8;
+                const VqVec<uint8_t, 8> m = vq_ldv<uint8_t, 8>(mk + (at < V - 8 ? at : V - 8));
+                __builtin_memcpy(&live[u], &m, 8);
+            }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int at = first + (u * NT + t) * 8;
+            if (!MASKED || live[u]) raw[u] = vq_ldv<T, 8>(lg + (at < V - 8 ? at : V - 8));
+        }
+    }
+    float x[E], most[NU];                                     // the logits, the largest of each 8
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u * 8 + i] = !MASKED || ((live[u] >> (8 * i)) & 0xff) ? (float)raw[u].v[i] : -INFINITY;
+    if (first + NT * E > V) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int at = first + (u * NT + t) * 8;
+            if (at + 8 > V)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u * 8 + i] = at + i < V && (!MASKED || mk[at + i]) ? (float)lg[at + i] : -INFINITY;
+        }
+    }
+    float gm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        const int64_t at = first + (int64_t)(u * NT + t) * 8;
-        unsigned long long live = ~0ull;
-        if (MASKED && at + 8 <= V) {
-            const VqVec<uint8_t, 8> m = vq_ldv<uint8_t, 8>(mk + at);
-            __builtin_memcpy(&live, &m, 8);
-        }
-        if (at + 8 <= V) {
-            if (!MASKED || live) {
-                const VqVec<T, 8> r = vq_ldv<T, 8>(lg + at);
+        most[u] = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[u * 8 + i] = !MASKED || ((live >> (8 * i)) & 0xff) ? (float)r.v[i] : -INFINITY;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[u * 8 + i] = -INFINITY;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[u * 8 + i] = at + i < V && (!MASKED || mk[at + i]) ? (float)lg[at + i] : -INFINITY;
-        }
+        for (int i = 0; i < 8; ++i) most[u] = fmaxf(most[u], x[u * 8 + i]);                 // (a NaN is passed over)
+        gm = fmaxf(gm, most[u]);
     }
-    float mine = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        bad |= x[i] != x[i];
-        mine = fmaxf(mine, x[i]);                             // (a NaN is passed over)
-    }
-    // 1. 64 groups of NT / 64 threads; lane g of every wave ranks group g
-    float gm = mine;
+    // 1. 64 groups of NT / 64 threads: each wave finds the largest of all, one of them the K-th
 #pragma unroll
     for (int o = 1; o < NT / 64; o <<= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
     if (t % (NT / 64) == 0) group_max[t / (NT / 64)] = gm;
     if (t == 0) found = 0;
     __syncthreads();
     gm = group_max[t & 63];
-    int place = 0;
+    float mx = gm;
 #pragma unroll
-    for (int k = 0; k < 64; ++k) {
-        const float o = group_max[k];
-        place += o > gm || (o == gm && k < (t & 63)) ? 1 : 0;
-    }
-    const float bound = __shfl(gm, __builtin_ctzll(__ballot(place == K - 1)), 64), mx = __shfl(gm, __builtin_ctzll(__ballot(place == 0)), 64);
-    // 2. and the log-sum: sums of 8 in 32 bits, the rest in 64
-    if (mine >= bound && mine > -INFINITY) {
+    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if (t >> 6 == NW - 1) {
+        // ranks by value with the lane in the low 6 bits, so that no two are equal; the bound is the value without them
+        const unsigned key = (sel_order(gm) & ~63u) | (unsigned)(t & 63);
+        int rank = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (x[i] >= bound && x[i] > -INFINITY) {
-                const int at = atomicAdd(&found, 1);
-                if (at < SEL_CAP) list[at] = make_int2(__float_as_int(x[i]), (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8));
-            }
+        for (int k = 0; k < 64; ++k) rank += (unsigned)__builtin_amdgcn_readlane((int)key, k) > key ? 1 : 0;
+        if (rank == K - 1) bound_s = gm > -INFINITY ? sel_value(key & ~63u) : -INFINITY;
     }
+    // the log-sum: 8 terms in 32 bits, the rest in 64; a logit of +inf or NaN makes it NaN
     if (a.normalize) {
-        double s = bad ? (double)NAN : 0.0;
-        if (mx > -INFINITY && mx < INFINITY) {
+        double s = 0.0;
+        if (mx > -INFINITY) {
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 float q = 0.f;
@@ -192,18 +190,50 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
                 for (int i = 0; i < 8; ++i) q += sel_exp(x[u * 8 + i] - mx);
                 s += q;
             }
-        } else if (mx == INFINITY) s = NAN;                   // a log-sum of +inf: no continuation
+        } else {                                              // no number at all: the sum is 0, or NaN where one is NaN
+#pragma unroll
+            for (int i = 0; i < E; ++i) s += x[i] != x[i] ? (double)NAN : 0.0;
+        }
         s = vq_wave_sum(s);
         if ((t & 63) == 0) wave_sum[t >> 6] = s;
     }
     __syncthreads();
+    // 2.
+    const float bound = bound_s;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        if (most[u] >= bound && most[u] > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (x[u * 8 + i] >= bound && x[u * 8 + i] > -INFINITY) {
+                    const int at = atomicAdd(&found, 1);
+                    if (at < SEL_CAP) list[at] = make_int2(__float_as_int(x[u * 8 + i]), first + (u * NT + t) * 8 + i);
+                }
+        }
+    __syncthreads();
     int n = found;
     if (n > SEL_CAP) {
-        // 3. the K-th largest value, then the last place among those equal to it
+        // 3. the K-th largest value, then the last place among those equal to it.  The logits are read again (from cache): kept in registers
+        // for this rare way they would cost every tile a third of the waves that fit a CU.
+        auto each = [&](auto &&f) {
+#pragma unroll 1
+            for (int u = 0; u < NU; ++u) {
+                const int at = first + (u * NT + t) * 8;
+                if (at >= V) break;
+                VqVec<T, 8> r;
+                if (at + 8 <= V) r = vq_ldv<T, 8>(lg + at);
+                else
+                    for (int i = 0; i < 8; ++i) r.v[i] = at + i < V ? lg[at + i] : (T)0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = at + i < V && (!MASKED || mk[at + i]) ? (float)r.v[i] : -INFINITY;
+                    if (v > -INFINITY) f(v, sel_order(v), (unsigned)(at + i));
+                }
+            }
+        };
         auto count = [&](auto &&pred) {
             int c = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) c += pred(x[i], (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8)) ? 1 : 0;
+            each([&](float, unsigned o, unsigned p) { c += pred(o, p) ? 1 : 0; });
             c = vq_wave_sum(c);
             __syncthreads();
             if ((t & 63) == 0) wave_cnt[t >> 6] = c;
@@ -216,28 +246,25 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
         unsigned kth = 0;
         for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
             const unsigned want = kth | bit;
-            if (count([&](float f, int) { return f > -INFINITY && sel_order(f) >= want; }) >= K) kth = want;
+            if (count([&](unsigned o, unsigned) { return o >= want; }) >= K) kth = want;
         }
-        const int above = count([&](float f, int) { return f > -INFINITY && sel_order(f) > kth; });
-        unsigned lo = (unsigned)first, hi = (unsigned)(first + NT * E - 1 < V - 1 ? first + NT * E - 1 : V - 1);
+        const int above = count([&](unsigned o, unsigned) { return o > kth; });
+        unsigned lo = (unsigned)first, hi = (unsigned)(first + NT * E < V ? first + NT * E : V) - 1;
         while (lo < hi) {                                     // the least place with `above` + (equal ones up to it) >= K
             const unsigned mid = lo + (hi - lo) / 2;
-            if (above + count([&](float f, int p) { return f > -INFINITY && sel_order(f) == kth && (unsigned)p <= mid; }) >= K) hi = mid; else lo = mid + 1;
+            if (above + count([&](unsigned o, unsigned p) { return o == kth && p <= mid; }) >= K) hi = mid; else lo = mid + 1;
         }
         __syncthreads();
         if (t == 0) found = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int p = (int)(first + (int64_t)((i / 8) * NT + t) * 8 + i % 8);
-            const unsigned u = sel_order(x[i]);
-            if (x[i] > -INFINITY && (u > kth || (u == kth && (unsigned)p <= lo))) list[atomicAdd(&found, 1)] = make_int2(__float_as_int(x[i]), p);
-        }
+        each([&](float v, unsigned o, unsigned p) {
+            if (o > kth || (o == kth && p <= lo)) list[atomicAdd(&found, 1)] = make_int2(__float_as_int(v), (int)p);
+        });
         __syncthreads();
         n = found;
     }
     // 4.
-    int2 *out = a.part + (int64_t)blockIdx.x * K;
+    int2 *out = a.part + blockIdx.x * (int64_t)K;
     for (int i = t; i < n; i += NT) {
         const int2 me = list[i];
         const float f = __int_as_float(me.x);
@@ -261,7 +288,9 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
 
 // ---- merge: one workgroup per batch entry -------------------------------------------------------------------------------------------
 // The rows' log-sums from their tiles (16 lanes a row), then the K best of J * tiles * K (and the finished beams') by the same bound and
-// ranks in 64 bits; where ties let more than SEL_CAP through, K rounds that each find the next one.  Bound by latency.
+// ranks in 64 bits; where ties let more than SEL_CAP through, K rounds that each find the next one.  Bound by latency: the first
+// SEL_HELD list entries of a thread are on their way while the log-sums are formed, and stay in registers.
+#define SEL_HELD 4
 __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
 {
     __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], group_max[64], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
@@ -271,70 +300,83 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
     __shared__ int rp[4];
     const int t = threadIdx.x, J = a.J, S = a.tiles, K = a.K;
     const int64_t b = blockIdx.x;
+    const int per = S * K, total = J * per;
+    const int2 *lists = a.part + b * total;                   // (rows that no workgroup listed hold anything: base tells)
+    int2 held[SEL_HELD];
+#pragma unroll
+    for (int h = 0; h < SEL_HELD; ++h) held[h] = h * 256 + t < total ? lists[h * 256 + t] : make_int2(0, 0);
     for (int j = t >> 4; j < J; j += 16) {
         const int64_t row = b * J + j;
         const double s = a.scores ? (double)a.scores[row] : 0.0;
         const bool f = a.finished && a.finished[row], live = !f && s > -INFINITY;
         double lse = 0.0;
-        if (live && a.normalize) {
+        if (a.normalize) {
             float m = -INFINITY;
-            for (int q = t & 15; q < S; q += 16) m = fmaxf(m, a.part_max[row * S + q]);
-            for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
             double sum = 0.0;
-            for (int q = t & 15; q < S; q += 16) {
+            for (int q = t & 15; q < S; q += 16) {            // running maximum and sum
                 const float pm = a.part_max[row * S + q];
                 const double p = a.part_sum[row * S + q];
+                if (pm > m) { sum = sum == 0.0 ? 0.0 : sum * exp((double)m - (double)pm); m = pm; }
                 sum += p == 0.0 ? 0.0 : p * exp((double)pm - (double)m);
             }
+            float top = m;
+            for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            sum = sum == 0.0 ? 0.0 : sum * exp((double)m - (double)top);
             for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-            lse = (double)m + log(sum);                        // (no logit admitted: -inf, and NaN below)
+            lse = (double)top + log(sum);                      // (no logit admitted: not finite)
         }
         if ((t & 15) == 0) {
             fin[j] = f;
-            base[j] = !live ? (f ? s : -INFINITY) : !(lse > -INFINITY && lse < INFINITY) ? -INFINITY : s;
-            if (live && a.normalize && !(lse > -INFINITY && lse < INFINITY)) lse = INFINITY;
-            if (a.lse_out) a.lse_out[row] = lse;
+            base[j] = f ? s : live && lse > -INFINITY && lse < INFINITY ? s : -INFINITY;
             log_sum[j] = lse;
+            if (a.lse_out) a.lse_out[row] = lse;
         }
     }
     if (t == 0) found = 0;
     __syncthreads();
-    const int per = S * K, total = J * per;
     // candidate i: list entry i % per of row i / per; a finished beam's first entry is its only continuation
-    auto at = [&](int i, int &place) -> double {
-        const int j = i / per, e = i - j * per;
+    auto value = [&](int i, int2 q, int &place) -> double {
+        const int j = i / per;
         const double s = base[j];
         if (fin[j]) {
             place = j * a.V + a.end_token;
-            return e ? -INFINITY : sel_sum(s, 0.0);
+            return i == j * per ? sel_sum(s, 0.0) : -INFINITY;
         }
-        if (!(s > -INFINITY)) { place = 0; return -INFINITY; }
-        const int2 q = a.part[(b * J + j) * (int64_t)per + e];
-        place = j * a.V + q.y;
         const double l = (double)__int_as_float(q.x);
-        return l > -INFINITY ? sel_sum(s, l - log_sum[j]) : -INFINITY;
+        place = j * a.V + q.y;
+        return s > -INFINITY && l > -INFINITY ? sel_sum(s, l - log_sum[j]) : -INFINITY;
     };
-    int place;
-    double best = -INFINITY;
-    for (int i = t; i < total; i += 256) best = fmax(best, at(i, place));
+    double c_held[SEL_HELD], best = -INFINITY;
+    int p_held[SEL_HELD], place;
+#pragma unroll
+    for (int h = 0; h < SEL_HELD; ++h) {
+        c_held[h] = h * 256 + t < total ? value(h * 256 + t, held[h], p_held[h]) : -INFINITY;
+        best = fmax(best, c_held[h]);
+    }
+    for (int i = SEL_HELD * 256 + t; i < total; i += 256) best = fmax(best, value(i, lists[i], place));
     best = fmax(best, __shfl_xor(best, 1, 64));
     best = fmax(best, __shfl_xor(best, 2, 64));
     if ((t & 3) == 0) group_max[t >> 2] = best;
     __syncthreads();
     best = group_max[t & 63];
     int order = 0;
-#pragma unroll
+#pragma unroll 16
     for (int k = 0; k < 64; ++k) {
         const double o = group_max[k];
         order += o > best || (o == best && k < (t & 63)) ? 1 : 0;
     }
     const double bound = __shfl(best, __builtin_ctzll(__ballot(order == K - 1)), 64);
-    for (int i = t; i < total; i += 256) {
-        const double c = at(i, place);
+    auto offer = [&](double c, int p) {
         if (c >= bound && c > -INFINITY) {
             const int k = atomicAdd(&found, 1);
-            if (k < SEL_CAP) { cs[k] = c; ps[k] = place; }
+            if (k < SEL_CAP) { cs[k] = c; ps[k] = p; }
         }
+    };
+#pragma unroll
+    for (int h = 0; h < SEL_HELD; ++h) offer(c_held[h], p_held[h]);
+    for (int i = SEL_HELD * 256 + t; i < total; i += 256) {
+        const double c = value(i, lists[i], place);
+        offer(c, place);
     }
     __syncthreads();
     int n = found;
@@ -358,7 +400,7 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
             double c = -INFINITY;
             int p = 0x7fffffff;
             for (int i = t; i < total; i += 256) {
-                const double d = at(i, place);
+                const double d = value(i, lists[i], place);
                 if (sel_before(last, lastp, d, place) && d > -INFINITY && sel_before(d, place, c, p)) { c = d; p = place; }
             }
             for (int o = 32; o; o >>= 1) {
@@ -574,50 +616,132 @@ extern "C" int vqhip_beam_select_bwd(const vqhip_beam_select_t *p, const float *
 // ---- reordering ------------------------------------------------------------------------------------------------------------------
 // out[b, i] = state[b, parents[b, i]] for every state of the call in one launch; a parent outside [0, J) gives zeros.  A state's row is
 // n1 pieces of `run` contiguous bytes, s1 bytes apart (a cache whose rows are cut to the positions in use); out is contiguous.
-struct ReorderState { const char *src; char *dst; int64_t sb, sj, s1, run; int64_t n1; };
+//
+// A copy, bound by HBM.  A piece is cut into units of 16 bytes (the largest power of two <= run where that is less); the last unit ends
+// with the piece and may overlap the one before it, so that no length needs a tail.  A workgroup moves REO_UNITS units that follow each
+// other over rows and pieces, whatever the rows' size; one 64-bit division finds its first row, 32-bit ones the rest.
+#define REO_PER_THREAD 4
+#define REO_UNITS (256 * REO_PER_THREAD)
+struct ReorderState {
+    const char *src; char *dst;
+    int64_t sb, sj, s1, run;
+    unsigned n1, per_piece, per_row, unit;              // pieces of a row; units of a piece, of a row; bytes of a unit
+    unsigned first;                                     // first workgroup in the launch
+};
 struct ReorderArgs {
     ReorderState s[VQHIP_BEAM_STATES];
     const int64_t *parents;
-    int64_t B; int J, K;
+    int64_t B; int J, K, n;
 };
+
+template <typename Args> __device__ __forceinline__ int reo_state(const Args &a, unsigned block)
+{
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.s[mid].first <= block) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <int BYTES> __device__ __forceinline__ void reo_move(const ReorderArgs &a, const ReorderState &s)
+{
+    using U = VqVec<uint8_t, BYTES>;
+    const int64_t rows = a.B * a.K;
+    const int64_t id0 = (int64_t)(blockIdx.x - s.first) * REO_UNITS, row0 = id0 / s.per_row;
+    const unsigned off0 = (unsigned)(id0 - row0 * s.per_row);
+    U v[REO_PER_THREAD];
+    char *dst[REO_PER_THREAD];
+#pragma unroll
+    for (int u = 0; u < REO_PER_THREAD; ++u) {
+        const unsigned off = off0 + u * 256 + threadIdx.x, skip = off / s.per_row, in_row = off - skip * s.per_row;
+        const int64_t row = row0 + skip;
+        dst[u] = nullptr;
+        if (row < rows) {
+            const unsigned piece = s.n1 == 1 ? 0 : in_row / s.per_piece;
+            int64_t at = (int64_t)(in_row - piece * s.per_piece) * BYTES;
+            at = at + BYTES <= s.run ? at : s.run - BYTES;
+            const int64_t b = (int64_t)((unsigned)row / (unsigned)a.K), p = a.parents[row];
+            dst[u] = s.dst + (row * s.n1 + piece) * s.run + at;
+            if (p >= 0 && p < a.J) v[u] = *(const U *)(s.src + b * s.sb + p * s.sj + piece * s.s1 + at);
+            else
+                for (int i = 0; i < BYTES; ++i) v[u].v[i] = 0;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < REO_PER_THREAD; ++u)
+        if (dst[u]) *(U *)dst[u] = v[u];
+}
 
 __global__ void __launch_bounds__(256) vq_beam_reorder_kernel(const ReorderArgs a)
 {
-    const ReorderState s = a.s[blockIdx.y];
-    const int64_t row = s.n1 * s.run, total = a.B * a.K * row;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / row, w = i - r * row, b = r / a.K, n = w / s.run;
-        const int64_t p = a.parents[r];
-        s.dst[i] = p < 0 || p >= a.J ? 0 : s.src[b * s.sb + p * s.sj + n * s.s1 + (w - n * s.run)];
+    const ReorderState &s = a.s[reo_state(a, blockIdx.x)];
+    switch (s.unit) {
+    case 16: reo_move<16>(a, s); break;
+    case 8: reo_move<8>(a, s); break;
+    case 4: reo_move<4>(a, s); break;
+    case 2: reo_move<2>(a, s); break;
+    default: reo_move<1>(a, s);
     }
 }
 
-// d_state[b, j] = sum of grad[b, i] over parents[b, i] == j, ascending i, in 32 bits and rounded once; both contiguous
-struct ReorderBwdState { const void *grad; void *out; int64_t row; int dtype; };
+// d_state[b, j] = sum of grad[b, i] over parents[b, i] == j, ascending i, in 32 bits and rounded once; both contiguous.  The same units,
+// now of 4 or 8 elements: an overlapping unit writes the same sums again.
+struct ReorderBwdState { const void *grad; void *out; int64_t row; unsigned per_row, unit, first; int dtype; };       // row, unit: elements
 struct ReorderBwdArgs {
     ReorderBwdState s[VQHIP_BEAM_STATES];
     const int64_t *parents;
-    int64_t B; int J, K;
+    int64_t B; int J, K, n;
 };
 
-template <typename T> __device__ __forceinline__ void reorder_bwd_at(const ReorderBwdArgs &a, const ReorderBwdState &s, int64_t i)
+template <typename T, int N> __device__ __forceinline__ void reo_sum(const ReorderBwdArgs &a, const ReorderBwdState &s)
 {
-    const int64_t r = i / s.row, w = i - r * s.row, b = r / a.J;
-    const int j = (int)(r - b * a.J);
-    float d = 0.f;
-    for (int k = 0; k < a.K; ++k)
-        if (a.parents[b * a.K + k] == j) d += (float)((const T *)s.grad)[(b * a.K + k) * s.row + w];
-    ((T *)s.out)[i] = (T)d;
+    const int64_t rows = a.B * a.J;
+    const int64_t id0 = (int64_t)(blockIdx.x - s.first) * REO_UNITS, row0 = id0 / s.per_row;
+    const unsigned off0 = (unsigned)(id0 - row0 * s.per_row);
+#pragma unroll
+    for (int u = 0; u < REO_PER_THREAD; ++u) {
+        const unsigned off = off0 + u * 256 + threadIdx.x, skip = off / s.per_row, in_row = off - skip * s.per_row;
+        const int64_t row = row0 + skip;
+        if (row >= rows) break;
+        int64_t at = (int64_t)in_row * N;
+        at = at + N <= s.row ? at : s.row - N;
+        const unsigned b = (unsigned)row / (unsigned)a.J;
+        const int64_t j = row - (int64_t)b * a.J, k0 = (int64_t)b * a.K;
+        const T *g = (const T *)s.grad + k0 * s.row + at;
+        float d[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] = 0.f;
+        for (int k = 0; k < a.K; k += 4) {                    // four parents at a time, their gradients loaded together
+            bool hit[4];
+            VqVec<T, N> v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) hit[q] = k + q < a.K && a.parents[k0 + k + q] == j;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (hit[q]) v[q] = vq_ldv<T, N>(g + (k + q) * s.row);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (hit[q])
+#pragma unroll
+                    for (int i = 0; i < N; ++i) d[i] += (float)v[q].v[i];
+        }
+        VqVec<T, N> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.v[i] = (T)d[i];
+        vq_stv<T, N>((T *)s.out + row * s.row + at, o);
+    }
 }
 
 __global__ void __launch_bounds__(256) vq_beam_reorder_bwd_kernel(const ReorderBwdArgs a)
 {
-    const ReorderBwdState s = a.s[blockIdx.y];
-    const int64_t total = a.B * a.J * s.row;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        if (s.dtype == VQHIP_F32) reorder_bwd_at<float>(a, s, i);
-        else if (s.dtype == VQHIP_BF16) reorder_bwd_at<__bf16>(a, s, i);
-        else reorder_bwd_at<_Float16>(a, s, i);
+    const ReorderBwdState &s = a.s[reo_state(a, blockIdx.x)];
+    if (s.dtype == VQHIP_F32) {
+        if (s.unit == 4) reo_sum<float, 4>(a, s); else reo_sum<float, 1>(a, s);
+    } else if (s.dtype == VQHIP_BF16) {
+        if (s.unit == 8) reo_sum<__bf16, 8>(a, s); else reo_sum<__bf16, 1>(a, s);
+    } else {
+        if (s.unit == 8) reo_sum<_Float16, 8>(a, s); else reo_sum<_Float16, 1>(a, s);
     }
 }
 
@@ -629,26 +753,42 @@ static int reorder_check(int64_t n, const void *states, const int64_t *parents, 
     return 0;
 }
 
+// workgroups of `rows` rows of per_row units; a launch takes fewer than 2^31
+static int reorder_blocks(int64_t rows, int64_t per_row, unsigned *first, unsigned *total, const char *what)
+{
+    if (per_row > 0x40000000 || rows > (((int64_t)1 << 62) / per_row)) VQ_FAIL(VQHIP_EDIM, "%s: rows of %lld units", what, (long long)per_row);
+    const int64_t blocks = (rows * per_row + REO_UNITS - 1) / REO_UNITS;
+    if (blocks > 0x7fffffff - (int64_t)*total) VQ_FAIL(VQHIP_EDIM, "%s: too many bytes", what);
+    *first = *total;
+    *total += (unsigned)blocks;
+    return 0;
+}
+
 extern "C" int vqhip_beam_reorder(const vqhip_beam_state_t *states, int64_t n, const int64_t *parents, int64_t B, int64_t J, int64_t K, void *stream)
 {
     int rc = reorder_check(n, states, parents, B, J, K, "vqhip_beam_reorder");
     if (rc) return rc;
     ReorderArgs a;
-    int m = 0;
-    int64_t most = 0;
+    unsigned total = 0;
+    a.n = 0;
     for (int64_t i = 0; i < n && B > 0; ++i) {
         const vqhip_beam_state_t &s = states[i];
         if (s.pieces < 0 || s.piece_bytes < 0) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_reorder: state %lld: %lld pieces of %lld bytes", (long long)i, (long long)s.pieces, (long long)s.piece_bytes);
         if (s.pieces == 0 || s.piece_bytes == 0) continue;
         if (!s.src || !s.dst) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_reorder: state %lld: null pointer", (long long)i);
-        a.s[m++] = ReorderState{(const char *)s.src, (char *)s.dst, s.stride_b, s.stride_j, s.piece_stride, s.piece_bytes, s.pieces};
-        const int64_t tot = B * K * s.pieces * s.piece_bytes;
-        if (tot > most) most = tot;
+        int unit = 16;
+        while (unit > s.piece_bytes) unit >>= 1;
+        const int64_t per_piece = (s.piece_bytes + unit - 1) / unit;
+        if (s.pieces > 0x40000000 || per_piece > 0x40000000) VQ_FAIL(VQHIP_EDIM, "vqhip_beam_reorder: state %lld: %lld pieces of %lld bytes", (long long)i, (long long)s.pieces, (long long)s.piece_bytes);
+        ReorderState &d = a.s[a.n];
+        d = ReorderState{(const char *)s.src, (char *)s.dst, s.stride_b, s.stride_j, s.piece_stride, s.piece_bytes, (unsigned)s.pieces, (unsigned)per_piece, (unsigned)(s.pieces * per_piece), (unsigned)unit, 0};
+        rc = reorder_blocks(B * K, s.pieces * per_piece, &d.first, &total, "vqhip_beam_reorder");
+        if (rc) return rc;
+        ++a.n;
     }
-    if (m == 0) return 0;
+    if (a.n == 0) return 0;
     a.parents = parents; a.B = B; a.J = (int)J; a.K = (int)K;
-    const int64_t blocks = (most + 256 * 16 - 1) / (256 * 16);
-    vq_beam_reorder_kernel<<<dim3((unsigned)(blocks > 65536 ? 65536 : blocks), (unsigned)m), 256, 0, (hipStream_t)stream>>>(a);
+    vq_beam_reorder_kernel<<<dim3(total), 256, 0, (hipStream_t)stream>>>(a);
     return vq_launch_status("vqhip_beam_reorder");
 }
 
@@ -658,21 +798,26 @@ extern "C" int vqhip_beam_reorder_bwd(const vqhip_beam_state_t *states, const in
     if (rc) return rc;
     if (n > 0 && !dtypes) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_reorder_bwd: null pointer");
     ReorderBwdArgs a;
-    int m = 0;
-    int64_t most = 0;
+    unsigned total = 0;
+    a.n = 0;
     for (int64_t i = 0; i < n && B > 0; ++i) {
         const vqhip_beam_state_t &s = states[i];
         const int eb = vq_elem_bytes(dtypes[i]);
         if (!eb || s.pieces < 0 || s.piece_bytes < 0 || s.piece_bytes % eb) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_reorder_bwd: state %lld: dtype %lld, %lld pieces of %lld bytes", (long long)i, (long long)dtypes[i], (long long)s.pieces, (long long)s.piece_bytes);
         if (s.pieces == 0 || s.piece_bytes == 0) continue;
         if (!s.src || !s.dst) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_reorder_bwd: state %lld: null pointer", (long long)i);
-        a.s[m++] = ReorderBwdState{s.src, s.dst, s.pieces * s.piece_bytes / eb, (int)dtypes[i]};
-        const int64_t tot = B * J * s.pieces * s.piece_bytes / eb;
-        if (tot > most) most = tot;
+        if (s.pieces > 0x40000000 || s.piece_bytes > ((int64_t)1 << 40) / s.pieces) VQ_FAIL(VQHIP_EDIM, "vqhip_beam_reorder_bwd: state %lld: %lld pieces of %lld bytes", (long long)i, (long long)s.pieces, (long long)s.piece_bytes);
+        const int64_t row = s.pieces * s.piece_bytes / eb;
+        const int unit = row < 16 / eb ? 1 : 16 / eb;
+        const int64_t per_row = (row + unit - 1) / unit;
+        ReorderBwdState &d = a.s[a.n];
+        d = ReorderBwdState{s.src, s.dst, row, (unsigned)per_row, (unsigned)unit, 0, (int)dtypes[i]};
+        rc = reorder_blocks(B * J, per_row, &d.first, &total, "vqhip_beam_reorder_bwd");
+        if (rc) return rc;
+        ++a.n;
     }
-    if (m == 0) return 0;
+    if (a.n == 0) return 0;
     a.parents = parents; a.B = B; a.J = (int)J; a.K = (int)K;
-    const int64_t blocks = (most + 256 * 4 - 1) / (256 * 4);
-    vq_beam_reorder_bwd_kernel<<<dim3((unsigned)(blocks > 65536 ? 65536 : blocks), (unsigned)m), 256, 0, (hipStream_t)stream>>>(a);
+    vq_beam_reorder_bwd_kernel<<<dim3(total), 256, 0, (hipStream_t)stream>>>(a);
     return vq_launch_status("vqhip_beam_reorder_bwd");
 }
