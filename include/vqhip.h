@@ -615,7 +615,7 @@ int vqhip_group_norm_bwd(const vqhip_group_norm_t *norm, const void *grad, void 
  * norm[0] = sqrt(sum of squares over all `count` tensors), squares and sums in 64 bits; dst = src * min(1, max_norm / (norm + eps)) for
  * every tensor with a dst (src itself, or memory that overlaps no tensor of the call).  A norm that is not finite goes through: the
  * factor is 0 for an infinite one, NaN for NaN.  `grads` is host memory, read during the call; src and dst are device pointers to n
- * contiguous elements of dtype F32 / BF16 / F16.  No tensor occurs twice.  workspace: vqhip_clip_grads_workspace_bytes bytes, 16-byte
+ * contiguous elements of dtype F32 / BF16 / F16.  No tensor occurs twice (VQHIP_EINVAL, as for overlaps).  workspace: vqhip_clip_grads_workspace_bytes bytes, 16-byte
  * aligned.  No host read: capturable. */
 typedef struct { const void *src; void *dst; int64_t n; int64_t dtype; } vqhip_grad_t;
 size_t vqhip_clip_grads_workspace_bytes(const vqhip_grad_t *grads, int64_t count);

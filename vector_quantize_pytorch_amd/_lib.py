@@ -204,7 +204,8 @@ def _check(rc, what):
 
 def _stream():
     # always called inside an @_on_device wrapper: the current device is the tensors' device
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the raw handle: torch.cuda.current_stream() builds a Stream object, 2 us a call)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _on_device(fn):
@@ -213,14 +214,15 @@ def _on_device(fn):
     different GPUs are an error; CPU tensors are rejected by _need_gpu inside `fn`."""
     @functools.wraps(fn)
     def wrapped(*args, **kwargs):
-        dev = None
+        dev = -1
         for t in (*args, *kwargs.values()):
-            if torch.is_tensor(t) and t.is_cuda:
-                if dev is None:
-                    dev = t.device
-                elif t.device != dev:
-                    raise VQHipError(f"{fn.__name__}: tensors on different devices ({dev} and {t.device})")
-        if dev is None or dev.index == torch.cuda.current_device():
+            if isinstance(t, torch.Tensor):
+                at = t.get_device()                          # -1: not on a GPU
+                if at >= 0 and at != dev:
+                    if dev >= 0:
+                        raise VQHipError(f"{fn.__name__}: tensors on different devices (cuda:{dev} and cuda:{at})")
+                    dev = at
+        if dev < 0 or dev == torch.cuda.current_device():
             return fn(*args, **kwargs)
         with torch.cuda.device(dev):
             return fn(*args, **kwargs)
@@ -255,9 +257,7 @@ def _need_gpu(*ts):
 
 def _written(tensors):
     """tells autograd that the library wrote into tensors of the caller (a graph that saved one then refuses its backward)"""
-    for t in tensors:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _ptr(t):

@@ -54,23 +54,23 @@ def _table(t: torch.Tensor, b: int, j: int, v: int) -> torch.Tensor:
 def _select(logits, scores, mask, finished, beam_size, end_token, normalize, want_lse):
     b, j, v = logits.shape
     dev = logits.device
-    out = torch.empty(b, beam_size, dtype=torch.float32, device=dev)
-    parents, tokens = torch.empty(2, b, beam_size, dtype=torch.int64, device=dev).unbind(0)
-    lse = torch.empty(b, j, dtype=torch.float64, device=dev) if want_lse else None
-    nws = L.lib().vqhip_beam_select_workspace_bytes(b, j, v, beam_size)
+    lib = L.lib()
+    out = torch.empty((b, beam_size), dtype=torch.float32, device=dev)
+    parents, tokens = torch.empty((2, b, beam_size), dtype=torch.int64, device=dev).unbind(0)
+    lse = torch.empty((b, j), dtype=torch.float64, device=dev) if want_lse else None
+    nws = lib.vqhip_beam_select_workspace_bytes(b, j, v, beam_size)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    s = _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse)
-    s.workspace, s.workspace_bytes = _addr(ws), nws
-    L._check(L.lib().vqhip_beam_select(ctypes.byref(s), L._stream()), "vqhip_beam_select")
+    s = _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse, ws, nws)
+    L._check(lib.vqhip_beam_select(ctypes.byref(s), L._stream()), "vqhip_beam_select")
     return out, parents, tokens, lse
 
 
-def _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse):
+def _struct(logits, scores, mask, finished, end_token, normalize, out, parents, tokens, lse, ws=None, nws=0):
     b, j, v = logits.shape
-    return _Select(logits=_addr(logits), dtype=L._ELEM_CODES[logits.dtype], B=b, J=j, V=v, stride_b=logits.stride(0), stride_j=logits.stride(1),
-                   scores=_addr(scores), mask=_addr(mask), mask_stride_b=0 if mask is None else mask.stride(0),
-                   mask_stride_j=0 if mask is None else mask.stride(1), finished=_addr(finished), end_token=end_token,
-                   normalize=int(normalize), K=out.shape[1], out_scores=_addr(out), parents=_addr(parents), tokens=_addr(tokens), lse=_addr(lse))
+    sb, sj, _ = logits.stride()
+    mb, mj, _ = (0, 0, 0) if mask is None else mask.stride()
+    return _Select(logits.data_ptr(), L._ELEM_CODES[logits.dtype], b, j, v, sb, sj, _addr(scores), _addr(mask), mb, mj, _addr(finished), end_token,
+                   normalize, out.shape[1], out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _addr(lse), _addr(ws), nws)
 
 
 @L._on_device

@@ -1,7 +1,9 @@
 // vq_grads.hip -- the global norm of many gradients, and their clipping.
 #include "vq_elem.h"
 
+#include <algorithm>
 #include <math.h>
+#include <stdlib.h>
 
 // norm = sqrt(sum of all squares): squares and sums in 64 bits, so that neither 1e30 nor 1e-30 leaves the range.  The tensors travel as
 // kernel arguments, TENSORS of a launch; a tensor is cut into chunks, one workgroup and one partial sum each.
@@ -74,6 +76,32 @@ __global__ void __launch_bounds__(256) vq_grad_scale_kernel(const GradArgs a, co
     else grad_scale<_Float16>(t, at, end, coef);
 }
 
+// every dst is its own src or shares no byte with a tensor of the call, and no src occurs twice: 1, or 0 with an overlap, -1 without memory
+static int grad_apart(const vqhip_grad_t *g, int64_t count)
+{
+    struct Span { uintptr_t first, behind; bool written; };
+    Span *s = (Span *)malloc(sizeof(Span) * 2 * (size_t)count);
+    if (!s) return -1;
+    size_t n = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (g[i].n <= 0) continue;
+        const uintptr_t bytes = (uintptr_t)g[i].n * vq_elem_bytes(g[i].dtype), src = (uintptr_t)g[i].src, dst = (uintptr_t)g[i].dst;
+        s[n++] = Span{src, src + bytes, src == dst};
+        if (dst && dst != src) s[n++] = Span{dst, dst + bytes, true};
+    }
+    std::sort(s, s + n, [](const Span &a, const Span &b) { return a.first < b.first; });
+    uintptr_t any = 0, written = 0, last = 0;                 // behind the last byte of any span, of a written one; the last first byte
+    int ok = 1;
+    for (size_t i = 0; i < n && ok; ++i) {
+        if (s[i].first < (s[i].written ? any : written) || (i && s[i].first == last)) ok = 0;
+        last = s[i].first;
+        any = std::max(any, s[i].behind);
+        if (s[i].written) written = std::max(written, s[i].behind);
+    }
+    free(s);
+    return ok;
+}
+
 static int64_t grad_blocks(const vqhip_grad_t *g, int64_t count)
 {
     int64_t n = 0;
@@ -100,6 +128,9 @@ extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double
     const int64_t blocks = grad_blocks(grads, count);
     if (blocks > 0x7fffffff) VQ_FAIL(VQHIP_EDIM, "vqhip_clip_grads: too many elements");
     if (workspace_bytes < (size_t)blocks * 8 + 16) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: workspace of %zu bytes", workspace_bytes);
+    const int apart = count > 0 ? grad_apart(grads, count) : 1;
+    if (apart < 0) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: no host memory");
+    if (!apart) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: a tensor occurs twice, or a result shares memory with another tensor");
     hipStream_t st = (hipStream_t)stream;
     float *coef = (float *)workspace;
     double *partial = (double *)((char *)workspace + 16);

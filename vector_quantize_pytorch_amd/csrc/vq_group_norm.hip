@@ -1,18 +1,27 @@
 // vq_group_norm.hip -- group norm with an activation on channels-last rows, forward and backward: the normalisation ahead of a quantizer
 // that reads rows [b, n, c].
+//
+// y = act((x - mean) rstd w + bias), mean and variance over the live rows and the C / G channels of a group; rows that `lens` or `mask`
+// leave out are neither read into the statistics nor normalised: their output is zero, whatever they hold.
+//
+// Two launches each way, both over (batch entry, chunk of rows): the first leaves each chunk's statistics (backward: its sums), the
+// second joins them -- in every workgroup, S * G pairs from cache -- and writes the rows.  Bound by HBM, with the second read of x from
+// the memory-side cache where it fits.  A thread keeps VEC channels of every row it visits (16 bytes where C divides so), so parameters and
+// statistics stay in registers and rows of any stride are read in whole lines.  All sums have one order: no atomics.
 #include "vq_elem.h"
 
 #include <math.h>
 
-// y = act((x - mean) rstd w + bias), mean and variance over the live rows and the C / G channels of a group; rows that `lens` or `mask`
-// leave out are neither read into the statistics nor normalised: their output is zero, whatever they hold.
+#define GN_FLUSH 32                // rows that a thread sums about one pivot
+
 struct GnArgs {
     const void *x; int64_t xb, xn;                      // element strides of batch and row
     const void *weight, *bias;
     const int64_t *lens; const uint8_t *mask;           // either or none
     void *y; float *mean, *rstd;
-    const void *grad; void *dx; float *dws, *dbs;       // backward: grad and dx contiguous; [B, C] sums each
-    int64_t N; int C, G, act, wdtype;
+    const void *grad; void *dx, *dweight, *dbias;       // backward: grad and dx contiguous
+    float2 *pair; float *chan, *live;                   // per chunk: [B * S, G] pairs, (backward) [B * S, 2, C] sums, [B * S] live rows
+    int64_t N, B, rows; int C, G, act, wdtype, S;       // S chunks of `rows` rows
     double eps;
 };
 
@@ -22,116 +31,436 @@ __device__ __forceinline__ float gn_param(const void *p, int dtype, int c, float
     return dtype == VQHIP_F32 ? ((const float *)p)[c] : dtype == VQHIP_BF16 ? (float)((const __bf16 *)p)[c] : (float)((const _Float16 *)p)[c];
 }
 
-__device__ __forceinline__ bool gn_live(const GnArgs &a, int64_t b, int64_t n)
+__device__ __forceinline__ void gn_store_param(void *p, int dtype, int c, float v)
 {
-    return a.lens ? n < a.lens[b] : a.mask ? a.mask[b * a.N + n] != 0 : true;
+    if (dtype == VQHIP_F32) ((float *)p)[c] = v;
+    else if (dtype == VQHIP_BF16) ((__bf16 *)p)[c] = (__bf16)v;
+    else ((_Float16 *)p)[c] = (_Float16)v;
 }
 
-__device__ double gn_block_sum(double v, double *red)
+// rows [0, len) of an entry may be live, with a mask those that it names
+struct GnLive {
+    int64_t len; const uint8_t *mask;
+    __device__ GnLive(const GnArgs &a, int64_t b) : len(a.lens ? a.lens[b] : a.N), mask(a.mask ? a.mask + b * a.N : nullptr) {}
+    __device__ __forceinline__ bool operator()(int64_t n) const { return n < len && (!mask || mask[n]); }
+};
+
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+
+// what a thread visits: rows first + lane, + step, ...; VEC channels from vector column col0 + (t % width), pass after pass of `width` columns
+struct GnShape { int cols, width, lanes; };
+template <int VEC> __device__ __forceinline__ GnShape gn_shape(int C)
 {
-    red[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    const int cols = C / VEC, width = cols < 256 ? cols : 256;
+    return GnShape{cols, width, 256 / width};
+}
+
+// sums over the channels of each group that lies in [c0, c1): f(lane entry) -> v[NV] doubles, entries = lanes x channels.  A group that
+// goes on in the next pass is carried there (two places, since one pass may read and write it).  done(g, v) by one thread a group.
+template <int NV, typename F, typename D> __device__ __forceinline__ void gn_groups(int c0, int c1, int cg, int lanes, const double *carry_in, double *carry_out, F &&entry, D &&done)
+{
+    const int g0 = c0 / cg, g1 = (c1 - 1) / cg, ng = g1 - g0 + 1;
+    int tg = 64;                                        // threads a group: a power of two within a wave
+    while (tg > 1 && tg * ng > 256) tg >>= 1;
+    const int per = 256 / tg;
+    const bool from_before = c0 % cg != 0, goes_on = c1 % cg != 0;
+    for (int base = 0; base < ng; base += per) {
+        const int g = g0 + base + (int)threadIdx.x / tg, q = threadIdx.x % tg;
+        double v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = 0.0;
+        if (g <= g1) {
+            const int lo = g * cg < c0 ? c0 : g * cg, hi = (g + 1) * cg > c1 ? c1 : (g + 1) * cg, wide = hi - lo;
+            for (int e = q; e < wide * lanes; e += tg) entry(e / wide, lo + e % wide, v);
+        }
+        for (int o = tg >> 1; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
+        if (g <= g1 && q == 0) {
+            if (g == g0 && from_before)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) v[i] += carry_in[i];
+            if (g == g1 && goes_on) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) carry_out[i] = v[i];
+            } else
+                done(g, v);
+        }
+    }
+}
+
+// ---- forward, first launch: each chunk's (mean, variance) of every group ------------------------------------------
+// A thread sums x - p and (x - p)^2 of a channel over up to GN_FLUSH rows, p the first of them: p is one of the values, so what cancels is
+// at most the number of rows -- an outlier or a far mean costs nothing.  Blocks, threads and channels join by counts, means and squared
+// deviations, the last in 64 bits.
+template <typename T, int VEC> __global__ void __launch_bounds__(256) vq_gn_stats_kernel(const GnArgs a)
+{
+    __shared__ float em[256 * VEC], ed[256 * VEC], en[256];
+    __shared__ double carry[2][3];
+    const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
+    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const GnShape sh = gn_shape<VEC>(a.C);
+    const int lane = t / sh.width, cg = a.C / a.G;
+    const GnLive lives(a, b);
+    const T *x = (const T *)a.x + b * a.xb;
+    float2 *out = a.pair + (int64_t)blockIdx.x * a.G;
+    for (int col0 = 0, pass = 0; col0 < sh.cols; col0 += sh.width, ++pass) {
+        const int col = col0 + t % sh.width;
+        float n = 0.f, mean[VEC], dev[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) mean[i] = dev[i] = 0.f;
+        if (lane < sh.lanes && col < sh.cols) {
+            const T *xc = x + (int64_t)col * VEC;
+            for (int64_t r = r0 + lane; r < r1; r += (int64_t)GN_FLUSH * sh.lanes) {
+                float p[VEC], s[VEC], q[VEC], m = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) p[i] = s[i] = q[i] = 0.f;
+                for (int k = 0; k < GN_FLUSH; k += 4) {
+                    VqVec<T, VEC> v[4];
+                    bool live[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int64_t at = r + (int64_t)(k + u) * sh.lanes;
+                        live[u] = at < r1 && lives(at);
+                        if (live[u]) v[u] = vq_ldv<T, VEC>(xc + at * a.xn);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (live[u]) {
+                            if (m == 0.f)
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i) p[i] = (float)v[u].v[i];
+                            m += 1.f;
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) {
+                                const float d = (float)v[u].v[i] - p[i];
+                                s[i] += d;
+                                q[i] = fmaf(d, d, q[i]);
+                            }
+                        }
+                    if (r + (int64_t)(k + 4) * sh.lanes >= r1) break;
+                }
+                if (m > 0.f) {
+                    const float all = n + m, inv = 1.f / m, part = m / all, cross = n * part;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float mb = s[i] * inv, db = fmaxf(fmaf(-s[i], mb, q[i]), 0.f), d = p[i] + mb - mean[i];
+                        dev[i] += fmaf(d * d, cross, db);
+                        mean[i] = n > 0.f ? fmaf(d, part, mean[i]) : p[i] + mb;
+                    }
+                    n = all;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { em[t * VEC + i] = mean[i]; ed[t * VEC + i] = dev[i]; }
+        en[t] = n;
+        __syncthreads();
+        const int c0 = col0 * VEC, c1 = (col0 + sh.width < sh.cols ? col0 + sh.width : sh.cols) * VEC;
+        if (t == 0 && col0 == 0) {
+            float rows = 0.f;
+            for (int l = 0; l < sh.lanes; ++l) rows += en[l * sh.width];
+            a.live[blockIdx.x] = rows;
+        }
+        // 64-bit sums about zero: count, count * mean, squared deviations + count * mean^2
+        gn_groups<3>(c0, c1, cg, sh.lanes, carry[pass & 1], carry[~pass & 1],
+            [&](int l, int c, double *v) {
+                const int e = l * sh.width * VEC + (c - c0);
+                const double k = en[l * sh.width + (c - c0) / VEC], m = em[e];
+                v[0] += k;
+                v[1] = fma(k, m, v[1]);
+                v[2] += fma(k * m, m, (double)ed[e]);
+            },
+            [&](int g, const double *v) {
+                const double m = v[0] > 0.0 ? v[1] / v[0] : 0.0, d = v[0] > 0.0 ? (v[2] - v[1] * m) / v[0] : 0.0;
+                out[g] = make_float2((float)m, (float)(d > 0.0 ? d : 0.0));
+            });
         __syncthreads();
     }
-    v = red[0];
+}
+
+// joins the chunks of a batch entry: f(chunk, group) -> v[NV], done(group, v); 64-bit sums in the order of the chunks' lanes
+template <int NV, typename F, typename D> __device__ __forceinline__ void gn_join(int S, int G, F &&entry, D &&done)
+{
+    int tg = 64;
+    while (tg > 1 && tg * G > 256) tg >>= 1;
+    for (int g = (int)threadIdx.x / tg; g < (G + 256 / tg - 1) / (256 / tg) * (256 / tg); g += 256 / tg) {
+        const int q = threadIdx.x % tg;
+        double v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = 0.0;
+        if (g < G)
+            for (int s = q; s < S; s += tg) entry(s, g, v);
+        for (int o = tg >> 1; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
+        if (g < G && q == 0) done(g, v);
+    }
+}
+
+// ---- forward, second launch --------------------------------------------------------------------------------------------------------
+template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_apply_kernel(const GnArgs a)
+{
+    extern __shared__ float stat[];                     // mean [G], rstd [G]
+    const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
+    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const int G = a.G, cg = a.C / G;
+    const float *rows = a.live + b * a.S;
+    const float2 *pair = a.pair + b * a.S * G;
+    gn_join<3>(a.S, G,
+        [&](int s, int g, double *v) {
+            const float2 p = pair[(int64_t)s * G + g];
+            const double k = rows[s], m = p.x;
+            v[0] += k;
+            v[1] = fma(k, m, v[1]);
+            v[2] += k * fma(m, m, (double)p.y);
+        },
+        [&](int g, const double *v) {
+            const double m = v[0] > 0.0 ? v[1] / v[0] : 0.0, d = v[0] > 0.0 ? (v[2] - v[1] * m) / v[0] : 0.0;
+            const float mf = (float)m, rf = (float)(1.0 / sqrt((d > 0.0 ? d : d == d ? 0.0 : d) + a.eps));
+            stat[g] = mf;
+            stat[G + g] = rf;
+            if (chunk == 0) { a.mean[b * G + g] = mf; a.rstd[b * G + g] = rf; }
+        });
     __syncthreads();
-    return v;
-}
-
-template <typename T> __global__ void __launch_bounds__(256) vq_group_norm_kernel(const GnArgs a)
-{
-    __shared__ double red[256];
-    const int64_t b = blockIdx.x / a.G;
-    const int g = blockIdx.x % a.G, cg = a.C / a.G;
-    const T *x = (const T *)a.x + b * a.xb + g * cg;
-    const int64_t total = a.N * cg;
-    double s = 0.0, n = 0.0;
-    for (int64_t i = threadIdx.x; i < total; i += 256)
-        if (gn_live(a, b, i / cg)) { s += (double)(float)x[(i / cg) * a.xn + i % cg]; n += 1.0; }
-    n = gn_block_sum(n, red);
-    const double mean = n > 0.0 ? gn_block_sum(s, red) / n : 0.0;
-    s = 0.0;
-    for (int64_t i = threadIdx.x; i < total; i += 256)
-        if (gn_live(a, b, i / cg)) { const double d = (double)(float)x[(i / cg) * a.xn + i % cg] - mean; s += d * d; }
-    const double rstd = n > 0.0 ? 1.0 / sqrt(gn_block_sum(s, red) / n + a.eps) : 0.0;
-    if (threadIdx.x == 0) {
-        a.mean[blockIdx.x] = (float)mean;
-        a.rstd[blockIdx.x] = (float)rstd;
-    }
-    for (int64_t i = threadIdx.x; i < total; i += 256) {
-        const int64_t r = i / cg;
-        const int c = g * cg + (int)(i % cg);
-        float y = 0.f;
-        if (gn_live(a, b, r)) {
-            const float xh = (float)(((double)(float)x[r * a.xn + i % cg] - mean) * rstd);
-            y = fmaf(xh, gn_param(a.weight, a.wdtype, c, 1.f), gn_param(a.bias, a.wdtype, c, 0.f));
-            if (a.act == VQHIP_ACT_SILU) y = y / (1.f + expf(-y));
-        }
-        ((T *)a.y)[(b * a.N + r) * a.C + c] = (T)y;
-    }
-}
-
-// dz = grad act'(z); db = sum dz, dw = sum dz xh over the live rows; dx = rstd (dz w - mean(dz w) - xh mean(dz w xh)), 0 in padding rows
-template <typename T> __global__ void __launch_bounds__(256) vq_group_norm_bwd_kernel(const GnArgs a)
-{
-    __shared__ double red[256];
-    const int64_t b = blockIdx.x / a.G;
-    const int g = blockIdx.x % a.G, cg = a.C / a.G;
+    const GnShape sh = gn_shape<VEC>(a.C);
+    const int lane = t / sh.width;
+    if (lane >= sh.lanes) return;
+    const GnLive lives(a, b);
     const T *x = (const T *)a.x + b * a.xb;
-    const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
-    double s1 = 0.0, s2 = 0.0, n = 0.0;
-    for (int c = g * cg; c < (g + 1) * cg; ++c) {
-        const float w = gn_param(a.weight, a.wdtype, c, 1.f), bias = gn_param(a.bias, a.wdtype, c, 0.f);
-        double db = 0.0, dw = 0.0;
-        n = 0.0;
-        for (int64_t r = threadIdx.x; r < a.N; r += 256)
-            if (gn_live(a, b, r)) {
-                const float xh = ((float)x[r * a.xn + c] - mean) * rstd, z = fmaf(xh, w, bias);
-                float dz = (float)((const T *)a.grad)[(b * a.N + r) * a.C + c];
-                if (a.act == VQHIP_ACT_SILU) { const float q = 1.f / (1.f + expf(-z)); dz *= q * (1.f + z * (1.f - q)); }
-                db += dz; dw += (double)dz * xh; n += 1.0;
-            }
-        db = gn_block_sum(db, red);
-        dw = gn_block_sum(dw, red);
-        n = gn_block_sum(n, red);
-        s1 += db * w; s2 += dw * w;
-        if (threadIdx.x == 0) { a.dbs[b * a.C + c] = (float)db; a.dws[b * a.C + c] = (float)dw; }
-    }
-    if (!a.dx) return;
-    n *= cg;
-    const float m1 = n > 0.0 ? (float)(s1 / n) : 0.f, m2 = n > 0.0 ? (float)(s2 / n) : 0.f;
-    for (int64_t i = threadIdx.x; i < a.N * cg; i += 256) {
-        const int64_t r = i / cg;
-        const int c = g * cg + (int)(i % cg);
-        float d = 0.f;
-        if (gn_live(a, b, r)) {
-            const float w = gn_param(a.weight, a.wdtype, c, 1.f);
-            const float xh = ((float)x[r * a.xn + c] - mean) * rstd, z = fmaf(xh, w, gn_param(a.bias, a.wdtype, c, 0.f));
-            float dz = (float)((const T *)a.grad)[(b * a.N + r) * a.C + c];
-            if (a.act == VQHIP_ACT_SILU) { const float q = 1.f / (1.f + expf(-z)); dz *= q * (1.f + z * (1.f - q)); }
-            d = rstd * (dz * w - m1 - xh * m2);
+    T *y = (T *)a.y + b * a.N * a.C;
+    for (int col = t % sh.width; col < sh.cols; col += sh.width) {
+        float mean[VEC], scale[VEC], shift[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = col * VEC + i, g = c / cg;
+            mean[i] = stat[g];
+            scale[i] = stat[G + g] * gn_param(a.weight, a.wdtype, c, 1.f);
+            shift[i] = gn_param(a.bias, a.wdtype, c, 0.f);
         }
-        ((T *)a.dx)[(b * a.N + r) * a.C + c] = (T)d;
+        for (int64_t r = r0 + lane; r < r1; r += 4 * sh.lanes) {
+            VqVec<T, VEC> v[4];
+            bool live[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = r + (int64_t)u * sh.lanes;
+                live[u] = at < r1 && lives(at);
+                if (live[u]) v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = r + (int64_t)u * sh.lanes;
+                if (at >= r1) break;
+                VqVec<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    float z = fmaf((float)v[u].v[i] - mean[i], scale[i], shift[i]);
+                    if (SILU) z *= gn_sigmoid(z);
+                    o.v[i] = live[u] ? (T)z : (T)0.f;
+                }
+                vq_stv<T, VEC>(y + at * a.C + (int64_t)col * VEC, o);
+            }
+        }
     }
 }
 
-// dweight[c] = sum_b dws[b, c], dbias likewise, in 64 bits and in the order of b
-__global__ void __launch_bounds__(256) vq_group_norm_params_kernel(const float *dws, const float *dbs, int64_t B, int C, void *dweight, void *dbias, int dtype)
+// ---- backward --------------------------------------------------------------------------------------------------------------------------
+// dz = grad act'(z); db = sum dz, dw = sum dz xh over the live rows; dx = rstd (dz w - mean(dz w) - xh mean(dz w xh)), 0 in padding rows
+template <bool SILU> __device__ __forceinline__ float gn_dz(float g, float xh, float w, float bias)
+{
+    if (!SILU) return g;
+    const float z = fmaf(xh, w, bias), q = gn_sigmoid(z);
+    return g * q * fmaf(z, 1.f - q, 1.f);
+}
+
+// first launch: each chunk's sums of dz and dz xh of every channel, and of w times them of every group
+template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_bwd_sums_kernel(const GnArgs a)
+{
+    __shared__ float e0[256 * VEC], e1[256 * VEC], en[256];
+    __shared__ double carry[2][2];
+    const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x, G = a.G, cg = a.C / G;
+    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const GnShape sh = gn_shape<VEC>(a.C);
+    const int lane = t / sh.width;
+    const GnLive lives(a, b);
+    const T *x = (const T *)a.x + b * a.xb, *gr = (const T *)a.grad + b * a.N * a.C;
+    float2 *pair = a.pair + (int64_t)blockIdx.x * G;
+    float *chan = a.chan + (int64_t)blockIdx.x * a.C * 2;
+    for (int col0 = 0, pass = 0; col0 < sh.cols; col0 += sh.width, ++pass) {
+        const int col = col0 + t % sh.width;
+        float s0[VEC], s1[VEC], n = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.f;
+        if (lane < sh.lanes && col < sh.cols) {
+            float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int c = col * VEC + i, g = c / cg;
+                mean[i] = a.mean[b * G + g];
+                rstd[i] = a.rstd[b * G + g];
+                w[i] = gn_param(a.weight, a.wdtype, c, 1.f);
+                bias[i] = gn_param(a.bias, a.wdtype, c, 0.f);
+            }
+            for (int64_t r = r0 + lane; r < r1; r += 4 * sh.lanes) {
+                VqVec<T, VEC> v[4], d[4];
+                bool live[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t at = r + (int64_t)u * sh.lanes;
+                    live[u] = at < r1 && lives(at);
+                    if (live[u]) {
+                        v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
+                        d[u] = vq_ldv<T, VEC>(gr + at * a.C + (int64_t)col * VEC);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (live[u]) {
+                        n += 1.f;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            const float xh = ((float)v[u].v[i] - mean[i]) * rstd[i], dz = gn_dz<SILU>((float)d[u].v[i], xh, w[i], bias[i]);
+                            s0[i] += dz;
+                            s1[i] = fmaf(dz, xh, s1[i]);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { e0[t * VEC + i] = s0[i]; e1[t * VEC + i] = s1[i]; }
+        en[t] = n;
+        __syncthreads();
+        const int c0 = col0 * VEC, c1 = (col0 + sh.width < sh.cols ? col0 + sh.width : sh.cols) * VEC, wide = sh.width * VEC;
+        if (t == 0 && col0 == 0) {
+            float rows = 0.f;
+            for (int l = 0; l < sh.lanes; ++l) rows += en[l * sh.width];
+            a.live[blockIdx.x] = rows;
+        }
+        for (int c = c0 + t; c < c1; c += 256) {
+            float q0 = 0.f, q1 = 0.f;
+            for (int l = 0; l < sh.lanes; ++l) { q0 += e0[l * wide + c - c0]; q1 += e1[l * wide + c - c0]; }
+            chan[c] = q0;
+            chan[a.C + c] = q1;
+            e0[c - c0] = q0;                            // (row 0 of the entries, read here alone: the groups sum from it)
+            e1[c - c0] = q1;
+        }
+        __syncthreads();
+        gn_groups<2>(c0, c1, cg, 1, carry[pass & 1], carry[~pass & 1],
+            [&](int, int c, double *v) {
+                const double w = gn_param(a.weight, a.wdtype, c, 1.f);
+                v[0] = fma(w, (double)e0[c - c0], v[0]);
+                v[1] = fma(w, (double)e1[c - c0], v[1]);
+            },
+            [&](int g, const double *v) { pair[g] = make_float2((float)v[0], (float)v[1]); });
+        __syncthreads();
+    }
+}
+
+// second launch: the first workgroups sum dweight and dbias over chunks and batch (GN_PARAM channels each), the others write dx
+#define GN_PARAM 32
+template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
+{
+    extern __shared__ float stat[];                     // mean(dz w) [G], mean(dz w xh) [G]
+    const int t = threadIdx.x, G = a.G, cg = a.C / G;
+    if (blockIdx.x < param_blocks) {
+        __shared__ double red[2][8][GN_PARAM];
+        const int c = blockIdx.x * GN_PARAM + t % GN_PARAM, q = t / GN_PARAM;
+        double v0 = 0.0, v1 = 0.0;
+        if (c < a.C)
+            for (int64_t s = q; s < a.B * a.S; s += 8) { v0 += a.chan[s * a.C * 2 + c]; v1 += a.chan[s * a.C * 2 + a.C + c]; }
+        red[0][q][t % GN_PARAM] = v0;
+        red[1][q][t % GN_PARAM] = v1;
+        __syncthreads();
+        if (q == 0 && c < a.C) {
+            for (int k = 1; k < 8; ++k) { v0 += red[0][k][t]; v1 += red[1][k][t]; }
+            if (a.dbias) gn_store_param(a.dbias, a.wdtype, c, (float)v0);
+            if (a.dweight) gn_store_param(a.dweight, a.wdtype, c, (float)v1);
+        }
+        return;
+    }
+    const unsigned block = blockIdx.x - param_blocks;
+    const int chunk = block % (unsigned)a.S;
+    const int64_t b = block / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const float *rows = a.live + b * a.S;
+    const float2 *pair = a.pair + b * a.S * G;
+    gn_join<3>(a.S, G,
+        [&](int s, int g, double *v) {
+            const float2 p = pair[(int64_t)s * G + g];
+            v[0] += rows[s];
+            v[1] += p.x;
+            v[2] += p.y;
+        },
+        [&](int g, const double *v) {
+            const double inv = v[0] > 0.0 ? 1.0 / (v[0] * cg) : 0.0;
+            stat[g] = (float)(v[1] * inv);
+            stat[G + g] = (float)(v[2] * inv);
+        });
+    __syncthreads();
+    const GnShape sh = gn_shape<VEC>(a.C);
+    const int lane = t / sh.width;
+    if (lane >= sh.lanes) return;
+    const GnLive lives(a, b);
+    const T *x = (const T *)a.x + b * a.xb, *gr = (const T *)a.grad + b * a.N * a.C;
+    T *dx = (T *)a.dx + b * a.N * a.C;
+    for (int col = t % sh.width; col < sh.cols; col += sh.width) {
+        float mean[VEC], rstd[VEC], w[VEC], bias[VEC], m1[VEC], m2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = col * VEC + i, g = c / cg;
+            mean[i] = a.mean[b * G + g];
+            rstd[i] = a.rstd[b * G + g];
+            w[i] = gn_param(a.weight, a.wdtype, c, 1.f);
+            bias[i] = gn_param(a.bias, a.wdtype, c, 0.f);
+            m1[i] = stat[g];
+            m2[i] = stat[G + g];
+        }
+        for (int64_t r = r0 + lane; r < r1; r += 2 * sh.lanes) {
+            VqVec<T, VEC> v[2], d[2];
+            bool live[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int64_t at = r + (int64_t)u * sh.lanes;
+                live[u] = at < r1 && lives(at);
+                if (live[u]) {
+                    v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
+                    d[u] = vq_ldv<T, VEC>(gr + at * a.C + (int64_t)col * VEC);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int64_t at = r + (int64_t)u * sh.lanes;
+                if (at >= r1) break;
+                VqVec<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float xh = ((float)v[u].v[i] - mean[i]) * rstd[i], dz = gn_dz<SILU>((float)d[u].v[i], xh, w[i], bias[i]);
+                    o.v[i] = live[u] ? (T)(rstd[i] * (fmaf(dz, w[i], -m1[i]) - xh * m2[i])) : (T)0.f;
+                }
+                vq_stv<T, VEC>(dx + at * a.C + (int64_t)col * VEC, o);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) vq_gn_zero_params_kernel(void *dweight, void *dbias, int dtype, int C)
 {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= C) return;
-    double w = 0.0, q = 0.0;
-    for (int64_t b = 0; b < B; ++b) { w += dws[b * C + c]; q += dbs[b * C + c]; }
-    for (int k = 0; k < 2; ++k) {
-        void *out = k ? dbias : dweight;
-        const float v = (float)(k ? q : w);
-        if (!out) continue;
-        if (dtype == VQHIP_F32) ((float *)out)[c] = v;
-        else if (dtype == VQHIP_BF16) ((__bf16 *)out)[c] = (__bf16)v;
-        else ((_Float16 *)out)[c] = (_Float16)v;
-    }
+    if (dweight) gn_store_param(dweight, dtype, c, 0.f);
+    if (dbias) gn_store_param(dbias, dtype, c, 0.f);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+// Four workgroups a CU in all, at most 256 chunks of an entry (every workgroup of the second launch reads them), at least 4096 elements each
+static void gn_plan(int64_t B, int64_t N, int64_t C, int64_t *S, int64_t *rows)
+{
+    int64_t s = B >= 1024 ? 1 : 1024 / B;
+    if (s > 256) s = 256;
+    const int64_t least = C >= 4096 ? 1 : 4096 / C;
+    int64_t r = (N + s - 1) / s;
+    if (r < least) r = least;
+    *rows = r;
+    *S = (N + r - 1) / r;
 }
 
 static int gn_check(const vqhip_group_norm_t *p, const char *what)
@@ -140,33 +469,47 @@ static int gn_check(const vqhip_group_norm_t *p, const char *what)
     if (!vq_elem_bytes(p->dtype) || !vq_elem_bytes(p->param_dtype)) VQ_FAIL(VQHIP_EINVAL, "%s: dtype %lld, parameters of %lld", what, (long long)p->dtype, (long long)p->param_dtype);
     if (p->B < 0 || p->N < 0 || p->C < 1 || p->groups < 1 || p->C % p->groups || !(p->eps >= 0.0)) VQ_FAIL(VQHIP_EINVAL, "%s: B %lld, N %lld, C %lld in %lld groups, eps %g", what, (long long)p->B, (long long)p->N, (long long)p->C, (long long)p->groups, p->eps);
     if (p->activation != VQHIP_ACT_NONE && p->activation != VQHIP_ACT_SILU) VQ_FAIL(VQHIP_EINVAL, "%s: activation %lld", what, (long long)p->activation);
-    if (p->C > VQHIP_NORM_MAX_C || p->B > 0x7fffffff / p->C || p->N > ((int64_t)1 << 40) / p->C) VQ_FAIL(VQHIP_EDIM, "%s: %lld x %lld rows of %lld channels (at most %d)", what, (long long)p->B, (long long)p->N, (long long)p->C, VQHIP_NORM_MAX_C);
+    if (p->C > VQHIP_NORM_MAX_C || p->B > (1 << 22) || p->N > ((int64_t)1 << 31) / p->C * 256) VQ_FAIL(VQHIP_EDIM, "%s: %lld x %lld rows of %lld channels (at most 2^22 entries, 2^39 elements each, %d channels)", what, (long long)p->B, (long long)p->N, (long long)p->C, VQHIP_NORM_MAX_C);
     if (p->lens && p->mask) VQ_FAIL(VQHIP_EINVAL, "%s: lens and mask", what);
     if (p->B > 0 && p->N > 0 && (!p->x || !p->mean || !p->rstd)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
-    if (p->workspace_bytes < vqhip_group_norm_workspace_bytes(p->B, p->N, p->C, p->groups) || (!p->workspace && p->workspace_bytes)) VQ_FAIL(VQHIP_EINVAL, "%s: workspace of %zu bytes", what, p->workspace_bytes);
+    const size_t need = vqhip_group_norm_workspace_bytes(p->B, p->N, p->C, p->groups);
+    if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "%s: workspace of %zu bytes, needs %zu", what, p->workspace_bytes, need);
     return 0;
 }
 
 static GnArgs gn_args(const vqhip_group_norm_t *p)
 {
     GnArgs a;
+    int64_t S, rows;
+    gn_plan(p->B, p->N, p->C, &S, &rows);
     a.x = p->x; a.xb = p->stride_b; a.xn = p->stride_n; a.weight = p->weight; a.bias = p->bias; a.lens = p->lens; a.mask = p->mask;
-    a.y = nullptr; a.mean = p->mean; a.rstd = p->rstd; a.grad = nullptr; a.dx = nullptr; a.dws = a.dbs = nullptr;
-    a.N = p->N; a.C = (int)p->C; a.G = (int)p->groups; a.act = (int)p->activation; a.wdtype = (int)p->param_dtype; a.eps = p->eps;
+    a.y = nullptr; a.mean = p->mean; a.rstd = p->rstd; a.grad = nullptr; a.dx = a.dweight = a.dbias = nullptr;
+    a.N = p->N; a.B = p->B; a.C = (int)p->C; a.G = (int)p->groups; a.act = (int)p->activation; a.wdtype = (int)p->param_dtype;
+    a.S = (int)S; a.rows = rows; a.eps = p->eps;
+    a.pair = (float2 *)p->workspace; a.chan = (float *)(a.pair + p->B * S * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
     return a;
 }
 
 extern "C" size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t C, int64_t groups)
 {
-    (void)N; (void)groups;
-    return B > 0 && C > 0 ? (size_t)B * C * 8 : 0;
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0) return 0;
+    int64_t S, rows;
+    gn_plan(B, N, C, &S, &rows);
+    return (size_t)(B * S) * (size_t)(1 + 2 * groups + 2 * C) * 4;
 }
 
-#define GN_BY_TYPE(dtype, kernel, ...)                                        \
-    do {                                                                      \
-        if ((dtype) == VQHIP_F32) kernel<float> __VA_ARGS__;                  \
-        else if ((dtype) == VQHIP_BF16) kernel<__bf16> __VA_ARGS__;           \
-        else kernel<_Float16> __VA_ARGS__;                                    \
+// channels of a thread: 16 bytes where C divides so, fewer where not
+#define GN_BY_VEC(T, MOST, C, call)                                                                       \
+    do {                                                                                                  \
+        if ((C) % (MOST) == 0) { constexpr int VEC = MOST; call; }                                        \
+        else if ((C) % 2 == 0) { constexpr int VEC = 2; call; }                                           \
+        else { constexpr int VEC = 1; call; }                                                             \
+    } while (0)
+#define GN_BY_TYPE(dtype, C, call)                                                                        \
+    do {                                                                                                  \
+        if ((dtype) == VQHIP_F32) { using T = float; GN_BY_VEC(T, 4, C, call); }                          \
+        else if ((dtype) == VQHIP_BF16) { using T = __bf16; GN_BY_VEC(T, 8, C, call); }                   \
+        else { using T = _Float16; GN_BY_VEC(T, 8, C, call); }                                            \
     } while (0)
 
 extern "C" int vqhip_group_norm(const vqhip_group_norm_t *p, void *y, void *stream)
@@ -177,7 +520,12 @@ extern "C" int vqhip_group_norm(const vqhip_group_norm_t *p, void *y, void *stre
     if (!y) VQ_FAIL(VQHIP_EINVAL, "vqhip_group_norm: null pointer");
     GnArgs a = gn_args(p);
     a.y = y;
-    GN_BY_TYPE(p->dtype, vq_group_norm_kernel, <<<dim3((unsigned)(p->B * p->groups)), 256, 0, (hipStream_t)stream>>>(a));
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)(a.B * a.S));
+    const size_t sm = (size_t)a.G * 8;
+    GN_BY_TYPE(p->dtype, a.C, (vq_gn_stats_kernel<T, VEC><<<grid, 256, 0, st>>>(a)));
+    if (a.act == VQHIP_ACT_SILU) GN_BY_TYPE(p->dtype, a.C, (vq_gn_apply_kernel<T, VEC, true><<<grid, 256, sm, st>>>(a)));
+    else GN_BY_TYPE(p->dtype, a.C, (vq_gn_apply_kernel<T, VEC, false><<<grid, 256, sm, st>>>(a)));
     return vq_launch_status("vqhip_group_norm");
 }
 
@@ -186,12 +534,24 @@ extern "C" int vqhip_group_norm_bwd(const vqhip_group_norm_t *p, const void *gra
     int rc = gn_check(p, "vqhip_group_norm_bwd");
     if (rc) return rc;
     if (!dx && !dweight && !dbias) return 0;
-    const bool some = p->B > 0 && p->N > 0;
-    if (some && !grad) VQ_FAIL(VQHIP_EINVAL, "vqhip_group_norm_bwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    if (p->B == 0 || p->N == 0) {
+        if (dweight || dbias) vq_gn_zero_params_kernel<<<dim3((unsigned)((p->C + 255) / 256)), 256, 0, st>>>(dweight, dbias, (int)p->param_dtype, (int)p->C);
+        return vq_launch_status("vqhip_group_norm_bwd");
+    }
+    if (!grad) VQ_FAIL(VQHIP_EINVAL, "vqhip_group_norm_bwd: null pointer");
     GnArgs a = gn_args(p);
-    a.grad = grad; a.dx = dx; a.dws = (float *)p->workspace; a.dbs = a.dws + p->B * p->C;
-    if (some) GN_BY_TYPE(p->dtype, vq_group_norm_bwd_kernel, <<<dim3((unsigned)(p->B * p->groups)), 256, 0, (hipStream_t)stream>>>(a));
-    if (dweight || dbias)
-        vq_group_norm_params_kernel<<<dim3((unsigned)((p->C + 255) / 256)), 256, 0, (hipStream_t)stream>>>(a.dws, a.dbs, some ? p->B : 0, a.C, dweight, dbias, a.wdtype);
+    a.grad = grad; a.dx = dx; a.dweight = dweight; a.dbias = dbias;
+    const dim3 grid((unsigned)(a.B * a.S));
+    const unsigned params = dweight || dbias ? (unsigned)((a.C + GN_PARAM - 1) / GN_PARAM) : 0;
+    const dim3 both(params + (dx ? (unsigned)(a.B * a.S) : 0));
+    const size_t sm = (size_t)a.G * 8;
+    if (a.act == VQHIP_ACT_SILU) {
+        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_sums_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a)));
+        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_apply_kernel<T, VEC, true><<<both, 256, sm, st>>>(a, params)));
+    } else {
+        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_sums_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a)));
+        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_apply_kernel<T, VEC, false><<<both, 256, sm, st>>>(a, params)));
+    }
     return vq_launch_status("vqhip_group_norm_bwd");
 }

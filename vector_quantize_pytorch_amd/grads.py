@@ -2,6 +2,7 @@
 `VectorQuantize(in_place_codebook_max_grad_norm=)` clips the gradients of its in-place optimizer with it."""
 from __future__ import annotations
 
+import array
 import ctypes
 from typing import Iterable, Optional, Sequence
 
@@ -18,13 +19,16 @@ class _Grad(ctypes.Structure):                            # vqhip_grad_t
 
 @L._on_device
 def _clip(first, grads, outs, max_norm):
-    codes = L._ELEM_CODES
-    dst = [None] * len(grads) if outs is None else [o.data_ptr() for o in outs]              # None: the norm alone
-    table = (_Grad * len(grads))(*[(g.data_ptr(), d, g.numel(), codes[g.dtype]) for g, d in zip(grads, dst)])
+    lib, count = L.lib(), len(grads)
+    src = [g.data_ptr() for g in grads]
+    dst = [0] * count if outs is None else [o.data_ptr() for o in outs]                      # 0: the norm alone
+    rows = zip(src, dst, [g.numel() for g in grads], [L._ELEM_CODES[g.dtype] for g in grads])
+    table = array.array("q", [v for row in rows for v in row])                               # vqhip_grad_t [count]
+    at = table.buffer_info()[0]
     norm = torch.empty((), dtype=torch.float32, device=first.device)
-    nws = L.lib().vqhip_clip_grads_workspace_bytes(table, len(grads))
+    nws = lib.vqhip_clip_grads_workspace_bytes(at, count)
     ws = torch.empty(nws, dtype=torch.uint8, device=first.device)
-    L._check(L.lib().vqhip_clip_grads(table, len(grads), max_norm, _EPS, norm.data_ptr(), ws.data_ptr(), nws, L._stream()), "vqhip_clip_grads")
+    L._check(lib.vqhip_clip_grads(at, count, max_norm, _EPS, norm.data_ptr(), ws.data_ptr(), nws, L._stream()), "vqhip_clip_grads")
     return norm
 
 
@@ -32,56 +36,35 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     """-> (clipped, norm): norm = the 2-norm over all elements of all tensors (a 0-dim float32 tensor, summed in 64 bits), clipped =
     every tensor times min(1, max_norm / (norm + 1e-6)), rounded once to its type.
 
-    grads: contiguous float32 / bfloat16 / float16 tensors of one device, none twice; out: contiguous tensors that take the result, of
-    the same shapes and types -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that is
-    not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  No gradient passes through."""
+    grads: contiguous float32 / bfloat16 / float16 tensors of one device; out: contiguous tensors of the same types and numbers of
+    elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that
+    is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  No gradient passes through."""
     grads = list(grads)
     if not max_norm >= 0.0:
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")
     if not grads:
         return [], torch.zeros((), dtype=torch.float32)
-    dev = grads[0].device
+    dev = grads[0].get_device()
     for g in grads:
         if g.dtype not in L._ELEM_CODES:
             L._elem_code(g, "clip_grads")
         if not g.is_contiguous():
             raise L.VQHipError(f"clip_grads: tensor {tuple(g.shape)} with strides {g.stride()}, expected a contiguous one")
-        if g.device != dev:
-            raise L.VQHipError(f"clip_grads: tensors on different devices ({dev} and {g.device})")
-    if len({g.data_ptr() for g in grads if g.numel()}) != sum(1 for g in grads if g.numel()):
-        raise L.VQHipError("clip_grads: a tensor occurs twice")
-    if out is None:
-        L._need_gpu(*grads[:1])
-        out = [torch.empty_like(g) for g in grads]
-    else:
+        if g.get_device() != dev:
+            raise L.VQHipError(f"clip_grads: tensors on different devices ({grads[0].device} and {g.device})")
+    if out is not None:
         out = list(out)
         if len(out) != len(grads):
             raise L.VQHipError(f"clip_grads: {len(out)} results for {len(grads)} tensors")
         for g, o in zip(grads, out):
-            if o.shape != g.shape or o.dtype != g.dtype or o.device != dev or not o.is_contiguous():
-                raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected contiguous {tuple(g.shape)} {g.dtype} on {dev}")
-        _check_memory(grads, out)
-        L._need_gpu(*grads[:1])
+            if o is not g and (o.numel() != g.numel() or o.dtype != g.dtype or o.get_device() != dev or not o.is_contiguous()):
+                raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {g.numel()} contiguous elements of {g.dtype} on {g.device}")
+    L._need_gpu(grads[0])
+    if out is None:
+        out = [torch.empty_like(g) for g in grads]
     norm = _clip(grads[0], grads, out, float(max_norm))
     L._written(out)
     return out, norm
-
-
-def _check_memory(grads, outs):
-    """every result is its own gradient's memory, or shares none with any tensor of the call"""
-    spans = [(g.data_ptr(), g.data_ptr() + g.numel() * g.element_size(), 0) for g in grads if g.numel()]
-    spans += [(o.data_ptr(), o.data_ptr() + o.numel() * o.element_size(), 1) for g, o in zip(grads, outs)
-              if o.numel() and o.data_ptr() != g.data_ptr()]
-    inside = {g.data_ptr() for g, o in zip(grads, outs) if o.data_ptr() == g.data_ptr()}       # gradients that are written themselves
-    spans.sort()
-    end = end_out = -1
-    for first, behind, is_out in spans:
-        written = is_out or first in inside
-        if first < (end if written else end_out):
-            raise L.VQHipError("clip_grads: a result shares memory with another tensor")
-        end = max(end, behind)
-        if written:
-            end_out = max(end_out, behind)
 
 
 def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:

@@ -28,13 +28,13 @@ def _addr(t):
 
 def _struct(x, weight, bias, lens, mask, groups, eps, act, stats):
     b, n, c = x.shape
+    sb, sn, _ = x.stride()
     nws = L.lib().vqhip_group_norm_workspace_bytes(b, n, c, groups)
     ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
     param = weight if weight is not None else bias
-    return ws, _Norm(x=_addr(x), dtype=L._ELEM_CODES[x.dtype], B=b, N=n, C=c, stride_b=x.stride(0), stride_n=x.stride(1), groups=groups,
-                     weight=_addr(weight), bias=_addr(bias), param_dtype=L.F32 if param is None else L._ELEM_CODES[param.dtype], eps=eps,
-                     activation=act, lens=_addr(lens), mask=_addr(mask), mean=stats[0].data_ptr(), rstd=stats[1].data_ptr(),
-                     workspace=_addr(ws), workspace_bytes=nws)
+    mean = stats.data_ptr()
+    return ws, _Norm(x.data_ptr(), L._ELEM_CODES[x.dtype], b, n, c, sb, sn, groups, _addr(weight), _addr(bias),
+                     L.F32 if param is None else L._ELEM_CODES[param.dtype], eps, act, _addr(lens), _addr(mask), mean, mean + 4 * b * groups, _addr(ws), nws)
 
 
 @L._on_device
