@@ -290,6 +290,12 @@ def test_clip_extremes(dev):
         t = torch.ones(8, device="cuda")
         A.clip_grads([t], 1.0, out=[t])
         assert abs(t.norm().item() - 1) < 1e-5
+    from vector_quantize_pytorch_amd._lib import VQHipError               # overlaps are refused before anything is launched
+    t = torch.ones(32, device="cuda")
+    for gs, out in (([t, t], None), ([t[:8]], [t[4:12]]), ([t[:16], t[20:24]], [t[:16], t[:4]]), ([t[:8], t[4:12]], [t[:8], t[4:12]])):
+        with pytest.raises(VQHipError, match="twice|shares memory"):
+            A.clip_grads(gs, 1.0, out=out)
+    assert (t == 1).all()
     odd = torch.ones(4099, device="cuda", dtype=torch.bfloat16)            # addresses off every vector's alignment
     parts = [odd[1:8], odd[9:1000], odd[1001:4098]]
     A.clip_grads(parts, 1.0, out=parts)

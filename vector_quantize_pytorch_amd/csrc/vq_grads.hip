@@ -6,11 +6,12 @@
 #include <stdlib.h>
 
 // norm = sqrt(sum of all squares): squares and sums in 64 bits, so that neither 1e30 nor 1e-30 leaves the range.  The tensors travel as
-// kernel arguments, TENSORS of a launch; a tensor is cut into chunks, one workgroup and one partial sum each.
+// kernel arguments, GRAD_TENSORS to a launch (4 KB of arguments); a tensor is cut into chunks, a workgroup and a partial sum each.
+// Bound by HBM: one read for the norm, one read and one write to clip.  Clipping goes through the tensors from the last to the first, since
+// the last ones read are the ones still in the memory-side cache.
 #define GRAD_TENSORS 100
-#define GRAD_CHUNK 16384
 struct GradTensor { const void *src; void *dst; int64_t n; unsigned first; int dtype; };        // first: its first workgroup in the launch
-struct GradArgs { GradTensor t[GRAD_TENSORS]; int count; };
+struct GradArgs { GradTensor t[GRAD_TENSORS]; int count, chunk; };
 
 __device__ __forceinline__ const GradTensor &grad_tensor(const GradArgs &a, unsigned block)
 {
@@ -24,34 +25,58 @@ __device__ __forceinline__ const GradTensor &grad_tensor(const GradArgs &a, unsi
 
 __device__ double grad_block_sum(double v)
 {
-    __shared__ double red[4];
+    __shared__ double red[16];
     v = vq_wave_sum(v);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    v = 0.0;
+    for (unsigned w = 0; w < blockDim.x / 64; ++w) v += red[w];
+    return v;
 }
 
-template <typename T> __device__ double grad_sumsq(const GradTensor &t, int64_t at, int64_t end)
+// 16-byte loads, four in flight a thread; what is left of a tensor's end one by one
+template <typename T> __device__ double grad_sumsq(const T *src, int64_t n)
 {
+    constexpr int N = 16 / sizeof(T);
     double s = 0.0;
-    for (int64_t i = at + threadIdx.x; i < end; i += 256) { const double v = (double)(float)((const T *)t.src)[i]; s = fma(v, v, s); }
+    const int64_t whole = n / N;
+    for (int64_t i = threadIdx.x; i < whole; i += 4 * 256) {
+        VqVec<T, N> v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * 256 < whole) v[u] = vq_ldv<T, N>(src + (i + u * 256) * N);
+            else
+                for (int k = 0; k < N; ++k) v[u].v[k] = (T)0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int k = 0; k < N; ++k) { const double f = (double)(float)v[u].v[k]; s = fma(f, f, s); }
+    }
+    const int64_t i = whole * N + threadIdx.x;
+    if (i < n) { const double f = (double)(float)src[i]; s = fma(f, f, s); }
     return s;
 }
 
 __global__ void __launch_bounds__(256) vq_grad_norm_kernel(const GradArgs a, double *partial)
 {
     const GradTensor &t = grad_tensor(a, blockIdx.x);
-    const int64_t at = (int64_t)(blockIdx.x - t.first) * GRAD_CHUNK, end = at + GRAD_CHUNK < t.n ? at + GRAD_CHUNK : t.n;
-    double s = t.dtype == VQHIP_F32 ? grad_sumsq<float>(t, at, end) : t.dtype == VQHIP_BF16 ? grad_sumsq<__bf16>(t, at, end) : grad_sumsq<_Float16>(t, at, end);
+    const int64_t at = (int64_t)(blockIdx.x - t.first) * a.chunk, n = t.n - at < a.chunk ? t.n - at : a.chunk;
+    double s = t.dtype == VQHIP_F32 ? grad_sumsq((const float *)t.src + at, n) : t.dtype == VQHIP_BF16 ? grad_sumsq((const __bf16 *)t.src + at, n) : grad_sumsq((const _Float16 *)t.src + at, n);
     s = grad_block_sum(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-// norm and coef = min(1, max_norm / (norm + eps)): (float) each behind the partial sums
-__global__ void __launch_bounds__(256) vq_grad_coef_kernel(const double *partial, int64_t n, double max_norm, double eps, float *norm, float *coef)
+// norm, and coef = min(1, max_norm / (norm + eps)): one workgroup, 8 partial sums in flight a thread
+__global__ void __launch_bounds__(1024) vq_grad_coef_kernel(const double *partial, int64_t n, double max_norm, double eps, float *norm, float *coef)
 {
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) s += partial[i];
+    for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+        double v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i + u * 1024 < n ? partial[i + u * 1024] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
+    }
     s = sqrt(grad_block_sum(s));
     if (threadIdx.x == 0) {
         const double c = max_norm / (s + eps);
@@ -60,9 +85,25 @@ __global__ void __launch_bounds__(256) vq_grad_coef_kernel(const double *partial
     }
 }
 
-template <typename T> __device__ void grad_scale(const GradTensor &t, int64_t at, int64_t end, float coef)
+template <typename T> __device__ void grad_scale(const T *src, T *dst, int64_t n, float coef)
 {
-    for (int64_t i = at + threadIdx.x; i < end; i += 256) ((T *)t.dst)[i] = (T)((float)((const T *)t.src)[i] * coef);
+    constexpr int N = 16 / sizeof(T);
+    const int64_t whole = n / N;
+    for (int64_t i = threadIdx.x; i < whole; i += 4 * 256) {
+        VqVec<T, N> v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * 256 < whole) v[u] = vq_ldv<T, N>(src + (i + u * 256) * N);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * 256 < whole) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) v[u].v[k] = (T)((float)v[u].v[k] * coef);
+                vq_stv<T, N>(dst + (i + u * 256) * N, v[u]);
+            }
+    }
+    const int64_t i = whole * N + threadIdx.x;
+    if (i < n) dst[i] = (T)((float)src[i] * coef);
 }
 
 __global__ void __launch_bounds__(256) vq_grad_scale_kernel(const GradArgs a, const float *coef_p)
@@ -70,10 +111,10 @@ __global__ void __launch_bounds__(256) vq_grad_scale_kernel(const GradArgs a, co
     const GradTensor &t = grad_tensor(a, blockIdx.x);
     const float coef = *coef_p;
     if (coef == 1.f && t.src == t.dst) return;          // in place and nothing to clip: g * 1 is g
-    const int64_t at = (int64_t)(blockIdx.x - t.first) * GRAD_CHUNK, end = at + GRAD_CHUNK < t.n ? at + GRAD_CHUNK : t.n;
-    if (t.dtype == VQHIP_F32) grad_scale<float>(t, at, end, coef);
-    else if (t.dtype == VQHIP_BF16) grad_scale<__bf16>(t, at, end, coef);
-    else grad_scale<_Float16>(t, at, end, coef);
+    const int64_t at = (int64_t)(blockIdx.x - t.first) * a.chunk, n = t.n - at < a.chunk ? t.n - at : a.chunk;
+    if (t.dtype == VQHIP_F32) grad_scale((const float *)t.src + at, (float *)t.dst + at, n, coef);
+    else if (t.dtype == VQHIP_BF16) grad_scale((const __bf16 *)t.src + at, (__bf16 *)t.dst + at, n, coef);
+    else grad_scale((const _Float16 *)t.src + at, (_Float16 *)t.dst + at, n, coef);
 }
 
 // every dst is its own src or shares no byte with a tensor of the call, and no src occurs twice: 1, or 0 with an overlap, -1 without memory
@@ -102,16 +143,21 @@ static int grad_apart(const vqhip_grad_t *g, int64_t count)
     return ok;
 }
 
-static int64_t grad_blocks(const vqhip_grad_t *g, int64_t count)
+// 16384 elements a workgroup where that makes 4 for each CU, else 4096
+static int64_t grad_blocks(const vqhip_grad_t *g, int64_t count, int *chunk)
 {
     int64_t n = 0;
-    for (int64_t i = 0; i < count; ++i) n += g[i].n > 0 ? (g[i].n + GRAD_CHUNK - 1) / GRAD_CHUNK : 0;
-    return n;
+    for (*chunk = 16384;; *chunk = 4096) {
+        n = 0;
+        for (int64_t i = 0; i < count; ++i) n += g[i].n > 0 ? (g[i].n + *chunk - 1) / *chunk : 0;
+        if (n >= 1024 || *chunk == 4096) return n;
+    }
 }
 
 extern "C" size_t vqhip_clip_grads_workspace_bytes(const vqhip_grad_t *grads, int64_t count)
 {
-    return grads && count > 0 ? (size_t)grad_blocks(grads, count) * 8 + 16 : 16;
+    int chunk;
+    return grads && count > 0 ? (size_t)grad_blocks(grads, count, &chunk) * 8 + 16 : 16;
 }
 
 extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double max_norm, double eps, float *norm, void *workspace,
@@ -125,7 +171,8 @@ extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double
         if (grads[i].n > 0 && !grads[i].src) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: tensor %lld: null pointer", (long long)i);
         write |= grads[i].n > 0 && grads[i].dst;
     }
-    const int64_t blocks = grad_blocks(grads, count);
+    int chunk;
+    const int64_t blocks = grad_blocks(grads, count, &chunk);
     if (blocks > 0x7fffffff) VQ_FAIL(VQHIP_EDIM, "vqhip_clip_grads: too many elements");
     if (workspace_bytes < (size_t)blocks * 8 + 16) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: workspace of %zu bytes", workspace_bytes);
     const int apart = count > 0 ? grad_apart(grads, count) : 1;
@@ -139,18 +186,20 @@ extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double
         for (int64_t i = 0; i < count;) {
             GradArgs a;
             a.count = 0;
+            a.chunk = chunk;
             unsigned nb = 0;
-            for (; i < count && a.count < GRAD_TENSORS; ++i)
-                if (grads[i].n > 0 && (pass == 0 || grads[i].dst)) {
-                    a.t[a.count++] = GradTensor{grads[i].src, grads[i].dst, grads[i].n, nb, (int)grads[i].dtype};
-                    nb += (unsigned)((grads[i].n + GRAD_CHUNK - 1) / GRAD_CHUNK);
-                }
+            for (; i < count && a.count < GRAD_TENSORS; ++i) {
+                const vqhip_grad_t &g = grads[pass == 0 ? i : count - 1 - i];
+                if (g.n <= 0 || (pass == 1 && !g.dst)) continue;
+                a.t[a.count++] = GradTensor{g.src, g.dst, g.n, nb, (int)g.dtype};
+                nb += (unsigned)((g.n + chunk - 1) / chunk);
+            }
             if (!nb) continue;
             if (pass == 0) vq_grad_norm_kernel<<<dim3(nb), 256, 0, st>>>(a, partial + done);
             else vq_grad_scale_kernel<<<dim3(nb), 256, 0, st>>>(a, coef);
             done += nb;
         }
-        if (pass == 0) vq_grad_coef_kernel<<<1, 256, 0, st>>>(partial, done, max_norm, eps, norm, coef);
+        if (pass == 0) vq_grad_coef_kernel<<<1, 1024, 0, st>>>(partial, done, max_norm, eps, norm, coef);
     }
     return vq_launch_status("vqhip_clip_grads");
 }

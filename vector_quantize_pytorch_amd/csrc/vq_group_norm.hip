@@ -190,6 +190,7 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_joi
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = 0.0;
         if (g < G)
+#pragma unroll 8
             for (int s = q; s < S; s += tg) entry(s, g, v);
         for (int o = tg >> 1; o; o >>= 1)
 #pragma unroll
@@ -357,22 +358,23 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
 }
 
 // second launch: the first workgroups sum dweight and dbias over chunks and batch (GN_PARAM channels each), the others write dx
-#define GN_PARAM 32
+#define GN_PARAM 16
 template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
 {
     extern __shared__ float stat[];                     // mean(dz w) [G], mean(dz w xh) [G]
     const int t = threadIdx.x, G = a.G, cg = a.C / G;
     if (blockIdx.x < param_blocks) {
-        __shared__ double red[2][8][GN_PARAM];
+        __shared__ double red[2][256 / GN_PARAM][GN_PARAM];
         const int c = blockIdx.x * GN_PARAM + t % GN_PARAM, q = t / GN_PARAM;
         double v0 = 0.0, v1 = 0.0;
         if (c < a.C)
-            for (int64_t s = q; s < a.B * a.S; s += 8) { v0 += a.chan[s * a.C * 2 + c]; v1 += a.chan[s * a.C * 2 + a.C + c]; }
+#pragma unroll 8
+            for (int64_t s = q; s < a.B * a.S; s += 256 / GN_PARAM) { v0 += a.chan[s * a.C * 2 + c]; v1 += a.chan[s * a.C * 2 + a.C + c]; }
         red[0][q][t % GN_PARAM] = v0;
         red[1][q][t % GN_PARAM] = v1;
         __syncthreads();
         if (q == 0 && c < a.C) {
-            for (int k = 1; k < 8; ++k) { v0 += red[0][k][t]; v1 += red[1][k][t]; }
+            for (int k = 1; k < 256 / GN_PARAM; ++k) { v0 += red[0][k][t]; v1 += red[1][k][t]; }
             if (a.dbias) gn_store_param(a.dbias, a.wdtype, c, (float)v0);
             if (a.dweight) gn_store_param(a.dweight, a.wdtype, c, (float)v1);
         }
