@@ -650,27 +650,30 @@ template <int BYTES> __device__ __forceinline__ void reo_move(const ReorderArgs 
     const int64_t rows = a.B * a.K;
     const int64_t id0 = (int64_t)(blockIdx.x - s.first) * REO_UNITS, row0 = id0 / s.per_row;
     const unsigned off0 = (unsigned)(id0 - row0 * s.per_row);
+    const unsigned here = row0 + (off0 + REO_UNITS - 1) / s.per_row < rows ? REO_UNITS : (unsigned)(rows * s.per_row - id0);
     U v[REO_PER_THREAD];
-    char *dst[REO_PER_THREAD];
+    int64_t dst[REO_PER_THREAD];
+    bool some[REO_PER_THREAD];
 #pragma unroll
-    for (int u = 0; u < REO_PER_THREAD; ++u) {
-        const unsigned off = off0 + u * 256 + threadIdx.x, skip = off / s.per_row, in_row = off - skip * s.per_row;
+    for (int u = 0; u < REO_PER_THREAD; ++u) {                // loads without conditions, so that all are in flight: the workgroup's last unit again
+        const unsigned want = u * 256 + threadIdx.x, off = off0 + (want < here ? want : here - 1), skip = off / s.per_row, in_row = off - skip * s.per_row;
         const int64_t row = row0 + skip;
-        dst[u] = nullptr;
-        if (row < rows) {
-            const unsigned piece = s.n1 == 1 ? 0 : in_row / s.per_piece;
-            int64_t at = (int64_t)(in_row - piece * s.per_piece) * BYTES;
-            at = at + BYTES <= s.run ? at : s.run - BYTES;
-            const int64_t b = (int64_t)((unsigned)row / (unsigned)a.K), p = a.parents[row];
-            dst[u] = s.dst + (row * s.n1 + piece) * s.run + at;
-            if (p >= 0 && p < a.J) v[u] = *(const U *)(s.src + b * s.sb + p * s.sj + piece * s.s1 + at);
-            else
-                for (int i = 0; i < BYTES; ++i) v[u].v[i] = 0;
-        }
+        const unsigned piece = s.n1 == 1 ? 0 : in_row / s.per_piece;
+        int64_t at = (int64_t)(in_row - piece * s.per_piece) * BYTES;
+        at = at + BYTES <= s.run ? at : s.run - BYTES;
+        const int64_t b = (int64_t)((unsigned)row / (unsigned)a.K), p = a.parents[row];
+        some[u] = p >= 0 && p < a.J;
+        dst[u] = (row * s.n1 + piece) * s.run + at;
+        v[u] = *(const U *)(s.src + b * s.sb + (some[u] ? p : 0) * s.sj + piece * s.s1 + at);
     }
 #pragma unroll
     for (int u = 0; u < REO_PER_THREAD; ++u)
-        if (dst[u]) *(U *)dst[u] = v[u];
+        if (u * 256 + threadIdx.x < here) {
+            if (!some[u])
+#pragma unroll
+                for (int i = 0; i < BYTES; ++i) v[u].v[i] = 0;
+            *(U *)(s.dst + dst[u]) = v[u];
+        }
 }
 
 __global__ void __launch_bounds__(256) vq_beam_reorder_kernel(const ReorderArgs a)

@@ -44,13 +44,12 @@ template <typename T> __device__ double grad_sumsq(const T *src, int64_t n)
         VqVec<T, N> v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (i + u * 256 < whole) v[u] = vq_ldv<T, N>(src + (i + u * 256) * N);
-            else
-                for (int k = 0; k < N; ++k) v[u].v[k] = (T)0.f;
+            v[u] = vq_ldv<T, N>(src + (i + u * 256 < whole ? i + u * 256 : i) * N);           // (unconditional: four in flight)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
+            if (i + u * 256 < whole)
 #pragma unroll
-            for (int k = 0; k < N; ++k) { const double f = (double)(float)v[u].v[k]; s = fma(f, f, s); }
+                for (int k = 0; k < N; ++k) { const double f = (double)(float)v[u].v[k]; s = fma(f, f, s); }
     }
     const int64_t i = whole * N + threadIdx.x;
     if (i < n) { const double f = (double)(float)src[i]; s = fma(f, f, s); }
@@ -92,8 +91,7 @@ template <typename T> __device__ void grad_scale(const T *src, T *dst, int64_t n
     for (int64_t i = threadIdx.x; i < whole; i += 4 * 256) {
         VqVec<T, N> v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u * 256 < whole) v[u] = vq_ldv<T, N>(src + (i + u * 256) * N);
+        for (int u = 0; u < 4; ++u) v[u] = vq_ldv<T, N>(src + (i + u * 256 < whole ? i + u * 256 : i) * N);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (i + u * 256 < whole) {

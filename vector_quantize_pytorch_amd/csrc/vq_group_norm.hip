@@ -22,6 +22,7 @@ struct GnArgs {
     const void *grad; void *dx, *dweight, *dbias;       // backward: grad and dx contiguous
     float2 *pair; float *chan, *live;                   // per chunk: [B * S, G] pairs, (backward) [B * S, 2, C] sums, [B * S] live rows
     int64_t N, B, rows; int C, G, act, wdtype, S;       // S chunks of `rows` rows
+    int stream;                                         // results past the caches
     double eps;
 };
 
@@ -31,6 +32,23 @@ __device__ __forceinline__ float gn_param(const void *p, int dtype, int c, float
     return dtype == VQHIP_F32 ? ((const float *)p)[c] : dtype == VQHIP_BF16 ? (float)((const __bf16 *)p)[c] : (float)((const _Float16 *)p)[c];
 }
 
+// VEC parameters from channel c on, in one load (one by one, each waits for the one before it)
+template <int VEC> __device__ __forceinline__ void gn_params(const void *p, int dtype, int c, float none, float *out)
+{
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = none;
+    } else if (dtype == VQHIP_F32) {
+        const VqVec<float, VEC> v = vq_ldv<float, VEC>((const float *)p + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = v.v[i];
+    } else {
+        const VqVec<uint16_t, VEC> v = vq_ldv<uint16_t, VEC>((const uint16_t *)p + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = dtype == VQHIP_BF16 ? (float)__builtin_bit_cast(__bf16, v.v[i]) : (float)__builtin_bit_cast(_Float16, v.v[i]);
+    }
+}
+
 __device__ __forceinline__ void gn_store_param(void *p, int dtype, int c, float v)
 {
     if (dtype == VQHIP_F32) ((float *)p)[c] = v;
@@ -38,14 +56,19 @@ __device__ __forceinline__ void gn_store_param(void *p, int dtype, int c, float 
     else ((_Float16 *)p)[c] = (_Float16)v;
 }
 
-// rows [0, len) of an entry may be live, with a mask those that it names
-struct GnLive {
-    int64_t len; const uint8_t *mask;
-    __device__ GnLive(const GnArgs &a, int64_t b) : len(a.lens ? a.lens[b] : a.N), mask(a.mask ? a.mask + b * a.N : nullptr) {}
-    __device__ __forceinline__ bool operator()(int64_t n) const { return n < len && (!mask || mask[n]); }
-};
+// rows [0, gn_len) of an entry may be live, with a mask (template parameter MASKED) those that it names
+__device__ __forceinline__ int64_t gn_len(const GnArgs &a, int64_t b)
+{
+    const int64_t len = a.lens ? a.lens[b] : a.N;
+    return len < 0 ? 0 : len < a.N ? len : a.N;
+}
 
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+
+template <typename T, int N> __device__ __forceinline__ void gn_store(T *p, const VqVec<T, N> &v, int stream)
+{
+    if (stream) vq_stv_nt<T, N>(p, v); else vq_stv<T, N>(p, v);
+}
 
 // what a thread visits: rows first + lane, + step, ...; VEC channels from vector column col0 + (t % width), pass after pass of `width` columns
 struct GnShape { int cols, width, lanes; };
@@ -93,16 +116,16 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_gro
 // A thread sums x - p and (x - p)^2 of a channel over up to GN_FLUSH rows, p the first of them: p is one of the values, so what cancels is
 // at most the number of rows -- an outlier or a far mean costs nothing.  Blocks, threads and channels join by counts, means and squared
 // deviations, the last in 64 bits.
-template <typename T, int VEC> __global__ void __launch_bounds__(256) vq_gn_stats_kernel(const GnArgs a)
+template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_stats_kernel(const GnArgs a)
 {
     __shared__ float em[256 * VEC], ed[256 * VEC], en[256];
     __shared__ double carry[2][3];
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
-    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < len ? r0 + a.rows : len;
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width, cg = a.C / a.G;
-    const GnLive lives(a, b);
     const T *x = (const T *)a.x + b * a.xb;
+    const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     float2 *out = a.pair + (int64_t)blockIdx.x * a.G;
     for (int col0 = 0, pass = 0; col0 < sh.cols; col0 += sh.width, ++pass) {
         const int col = col0 + t % sh.width;
@@ -118,18 +141,23 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) vq_gn_stat
                 for (int k = 0; k < GN_FLUSH; k += 4) {
                     VqVec<T, VEC> v[4];
                     bool live[4];
+                    const int64_t at = r + (int64_t)k * sh.lanes;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int64_t at = r + (int64_t)(k + u) * sh.lanes;
-                        live[u] = at < r1 && lives(at);
-                        if (live[u]) v[u] = vq_ldv<T, VEC>(xc + at * a.xn);
+                        const int64_t row = at + u * sh.lanes, in = row < r1 ? row : r1 - 1;
+                        live[u] = row < r1 && (!MASKED || mask[in]);
+                        v[u] = vq_ldv<T, VEC>(xc + in * a.xn);                     // (loads without conditions: four in flight)
+                    }
+                    if (m == 0.f) {                           // the first live one of these is the pivot
+#pragma unroll
+                        for (int u = MASKED ? 3 : 0; u >= 0; --u)
+                            if (live[u])
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i) p[i] = (float)v[u].v[i];
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         if (live[u]) {
-                            if (m == 0.f)
-#pragma unroll
-                                for (int i = 0; i < VEC; ++i) p[i] = (float)v[u].v[i];
                             m += 1.f;
 #pragma unroll
                             for (int i = 0; i < VEC; ++i) {
@@ -138,7 +166,7 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) vq_gn_stat
                                 q[i] = fmaf(d, d, q[i]);
                             }
                         }
-                    if (r + (int64_t)(k + 4) * sh.lanes >= r1) break;
+                    if (at + 4 * sh.lanes >= r1) break;
                 }
                 if (m > 0.f) {
                     const float all = n + m, inv = 1.f / m, part = m / all, cross = n * part;
@@ -200,11 +228,20 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_joi
 }
 
 // ---- forward, second launch --------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_apply_kernel(const GnArgs a)
+// rows [from, to) x VEC channels of zeros, what padding gives
+template <typename T, int VEC> __device__ __forceinline__ void gn_zero_rows(T *p, int64_t from, int64_t to, int step, int64_t stride)
+{
+    VqVec<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = (T)0.f;
+    for (int64_t r = from; r < to; r += step) vq_stv<T, VEC>(p + r * stride, o);
+}
+
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_apply_kernel(const GnArgs a)
 {
     extern __shared__ float stat[];                     // mean [G], rstd [G]
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
-    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, end = r0 + a.rows < a.N ? r0 + a.rows : a.N, r1 = end < len ? end : len;
     const int G = a.G, cg = a.C / G;
     const float *rows = a.live + b * a.S;
     const float2 *pair = a.pair + b * a.S * G;
@@ -227,26 +264,33 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width;
     if (lane >= sh.lanes) return;
-    const GnLive lives(a, b);
     const T *x = (const T *)a.x + b * a.xb;
+    const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     T *y = (T *)a.y + b * a.N * a.C;
+    // 16-bit rows: x scale + (bias - mean scale) in one step, its rounding is far below theirs.  32-bit rows subtract the mean first: a mean
+    // far from zero then costs nothing.
+    constexpr bool FOLD = sizeof(T) == 2;
     for (int col = t % sh.width; col < sh.cols; col += sh.width) {
         float mean[VEC], scale[VEC], shift[VEC];
+        gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, scale);
+        gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, shift);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const int c = col * VEC + i, g = c / cg;
-            mean[i] = stat[g];
-            scale[i] = stat[G + g] * gn_param(a.weight, a.wdtype, c, 1.f);
-            shift[i] = gn_param(a.bias, a.wdtype, c, 0.f);
+            const int g = (col * VEC + i) / cg;
+            mean[i] = FOLD ? 0.f : stat[g];
+            scale[i] *= stat[G + g];
+            if (FOLD) shift[i] = fmaf(-stat[g], scale[i], shift[i]);
         }
+        const T *xc = x + (int64_t)col * VEC;
+        T *yc = y + (int64_t)col * VEC;
         for (int64_t r = r0 + lane; r < r1; r += 4 * sh.lanes) {
             VqVec<T, VEC> v[4];
             bool live[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int64_t at = r + (int64_t)u * sh.lanes;
-                live[u] = at < r1 && lives(at);
-                if (live[u]) v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
+                const int64_t at = r + (int64_t)u * sh.lanes, in = at < r1 ? at : r1 - 1;
+                live[u] = at < r1 && (!MASKED || mask[in]);
+                v[u] = vq_ldv<T, VEC>(xc + in * a.xn);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -255,13 +299,14 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
                 VqVec<T, VEC> o;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    float z = fmaf((float)v[u].v[i] - mean[i], scale[i], shift[i]);
+                    float z = fmaf(FOLD ? (float)v[u].v[i] : (float)v[u].v[i] - mean[i], scale[i], shift[i]);
                     if (SILU) z *= gn_sigmoid(z);
-                    o.v[i] = live[u] ? (T)z : (T)0.f;
+                    o.v[i] = !MASKED || live[u] ? (T)z : (T)0.f;
                 }
-                vq_stv<T, VEC>(y + at * a.C + (int64_t)col * VEC, o);
+                gn_store<T, VEC>(yc + at * a.C, o, a.stream);
             }
         }
+        gn_zero_rows<T, VEC>(yc, (r0 > len ? r0 : len) + lane, end, sh.lanes, a.C);
     }
 }
 
@@ -275,16 +320,16 @@ template <bool SILU> __device__ __forceinline__ float gn_dz(float g, float xh, f
 }
 
 // first launch: each chunk's sums of dz and dz xh of every channel, and of w times them of every group
-template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_bwd_sums_kernel(const GnArgs a)
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_bwd_sums_kernel(const GnArgs a)
 {
     __shared__ float e0[256 * VEC], e1[256 * VEC], en[256];
     __shared__ double carry[2][2];
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x, G = a.G, cg = a.C / G;
-    const int64_t b = blockIdx.x / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < len ? r0 + a.rows : len;
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width;
-    const GnLive lives(a, b);
     const T *x = (const T *)a.x + b * a.xb, *gr = (const T *)a.grad + b * a.N * a.C;
+    const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     float2 *pair = a.pair + (int64_t)blockIdx.x * G;
     float *chan = a.chan + (int64_t)blockIdx.x * a.C * 2;
     for (int col0 = 0, pass = 0; col0 < sh.cols; col0 += sh.width, ++pass) {
@@ -294,25 +339,23 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
         for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.f;
         if (lane < sh.lanes && col < sh.cols) {
             float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
+            gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, w);
+            gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, bias);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const int c = col * VEC + i, g = c / cg;
+                const int g = (col * VEC + i) / cg;
                 mean[i] = a.mean[b * G + g];
                 rstd[i] = a.rstd[b * G + g];
-                w[i] = gn_param(a.weight, a.wdtype, c, 1.f);
-                bias[i] = gn_param(a.bias, a.wdtype, c, 0.f);
             }
             for (int64_t r = r0 + lane; r < r1; r += 4 * sh.lanes) {
                 VqVec<T, VEC> v[4], d[4];
                 bool live[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int64_t at = r + (int64_t)u * sh.lanes;
-                    live[u] = at < r1 && lives(at);
-                    if (live[u]) {
-                        v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
-                        d[u] = vq_ldv<T, VEC>(gr + at * a.C + (int64_t)col * VEC);
-                    }
+                    const int64_t at = r + (int64_t)u * sh.lanes, in = at < r1 ? at : r1 - 1;
+                    live[u] = at < r1 && (!MASKED || mask[in]);
+                    v[u] = vq_ldv<T, VEC>(x + in * a.xn + (int64_t)col * VEC);
+                    d[u] = vq_ldv<T, VEC>(gr + in * a.C + (int64_t)col * VEC);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
@@ -359,7 +402,7 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
 
 // second launch: the first workgroups sum dweight and dbias over chunks and batch (GN_PARAM channels each), the others write dx
 #define GN_PARAM 16
-template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
 {
     extern __shared__ float stat[];                     // mean(dz w) [G], mean(dz w xh) [G]
     const int t = threadIdx.x, G = a.G, cg = a.C / G;
@@ -382,7 +425,7 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
     }
     const unsigned block = blockIdx.x - param_blocks;
     const int chunk = block % (unsigned)a.S;
-    const int64_t b = block / (unsigned)a.S, r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < a.N ? r0 + a.rows : a.N;
+    const int64_t b = block / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, end = r0 + a.rows < a.N ? r0 + a.rows : a.N, r1 = end < len ? end : len;
     const float *rows = a.live + b * a.S;
     const float2 *pair = a.pair + b * a.S * G;
     gn_join<3>(a.S, G,
@@ -401,18 +444,18 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width;
     if (lane >= sh.lanes) return;
-    const GnLive lives(a, b);
     const T *x = (const T *)a.x + b * a.xb, *gr = (const T *)a.grad + b * a.N * a.C;
     T *dx = (T *)a.dx + b * a.N * a.C;
+    const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     for (int col = t % sh.width; col < sh.cols; col += sh.width) {
         float mean[VEC], rstd[VEC], w[VEC], bias[VEC], m1[VEC], m2[VEC];
+        gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, w);
+        gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, bias);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const int c = col * VEC + i, g = c / cg;
+            const int g = (col * VEC + i) / cg;
             mean[i] = a.mean[b * G + g];
             rstd[i] = a.rstd[b * G + g];
-            w[i] = gn_param(a.weight, a.wdtype, c, 1.f);
-            bias[i] = gn_param(a.bias, a.wdtype, c, 0.f);
             m1[i] = stat[g];
             m2[i] = stat[G + g];
         }
@@ -421,12 +464,10 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
             bool live[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int64_t at = r + (int64_t)u * sh.lanes;
-                live[u] = at < r1 && lives(at);
-                if (live[u]) {
-                    v[u] = vq_ldv<T, VEC>(x + at * a.xn + (int64_t)col * VEC);
-                    d[u] = vq_ldv<T, VEC>(gr + at * a.C + (int64_t)col * VEC);
-                }
+                const int64_t at = r + (int64_t)u * sh.lanes, in = at < r1 ? at : r1 - 1;
+                live[u] = at < r1 && (!MASKED || mask[in]);
+                v[u] = vq_ldv<T, VEC>(x + in * a.xn + (int64_t)col * VEC);
+                d[u] = vq_ldv<T, VEC>(gr + in * a.C + (int64_t)col * VEC);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -436,11 +477,12 @@ template <typename T, int VEC, bool SILU> __global__ void __launch_bounds__(256)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float xh = ((float)v[u].v[i] - mean[i]) * rstd[i], dz = gn_dz<SILU>((float)d[u].v[i], xh, w[i], bias[i]);
-                    o.v[i] = live[u] ? (T)(rstd[i] * (fmaf(dz, w[i], -m1[i]) - xh * m2[i])) : (T)0.f;
+                    o.v[i] = !MASKED || live[u] ? (T)(rstd[i] * (fmaf(dz, w[i], -m1[i]) - xh * m2[i])) : (T)0.f;
                 }
-                vq_stv<T, VEC>(dx + at * a.C + (int64_t)col * VEC, o);
+                gn_store<T, VEC>(dx + at * a.C + (int64_t)col * VEC, o, a.stream);
             }
         }
+        gn_zero_rows<T, VEC>(dx + (int64_t)col * VEC, (r0 > len ? r0 : len) + lane, end, sh.lanes, a.C);
     }
 }
 
@@ -487,6 +529,8 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     a.x = p->x; a.xb = p->stride_b; a.xn = p->stride_n; a.weight = p->weight; a.bias = p->bias; a.lens = p->lens; a.mask = p->mask;
     a.y = nullptr; a.mean = p->mean; a.rstd = p->rstd; a.grad = nullptr; a.dx = a.dweight = a.dbias = nullptr;
     a.N = p->N; a.B = p->B; a.C = (int)p->C; a.G = (int)p->groups; a.act = (int)p->activation; a.wdtype = (int)p->param_dtype;
+    // results of more than a quarter of the 256 MB memory-side cache go past it: 6 x 65536 x 128 bf16 90 -> 80 us with x still in it
+    a.stream = p->B * p->N * p->C * vq_elem_bytes(p->dtype) > (64 << 20);
     a.S = (int)S; a.rows = rows; a.eps = p->eps;
     a.pair = (float2 *)p->workspace; a.chan = (float *)(a.pair + p->B * S * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
     return a;
@@ -507,6 +551,10 @@ extern "C" size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t
         else if ((C) % 2 == 0) { constexpr int VEC = 2; call; }                                           \
         else { constexpr int VEC = 1; call; }                                                             \
     } while (0)
+#define GN_BY_MASK(mask, call)                                                                            \
+    do {                                                                                                  \
+        if (mask) { constexpr bool MASKED = true; call; } else { constexpr bool MASKED = false; call; }   \
+    } while (0)
 #define GN_BY_TYPE(dtype, C, call)                                                                        \
     do {                                                                                                  \
         if ((dtype) == VQHIP_F32) { using T = float; GN_BY_VEC(T, 4, C, call); }                          \
@@ -525,9 +573,9 @@ extern "C" int vqhip_group_norm(const vqhip_group_norm_t *p, void *y, void *stre
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(a.B * a.S));
     const size_t sm = (size_t)a.G * 8;
-    GN_BY_TYPE(p->dtype, a.C, (vq_gn_stats_kernel<T, VEC><<<grid, 256, 0, st>>>(a)));
-    if (a.act == VQHIP_ACT_SILU) GN_BY_TYPE(p->dtype, a.C, (vq_gn_apply_kernel<T, VEC, true><<<grid, 256, sm, st>>>(a)));
-    else GN_BY_TYPE(p->dtype, a.C, (vq_gn_apply_kernel<T, VEC, false><<<grid, 256, sm, st>>>(a)));
+    GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_stats_kernel<T, VEC, MASKED><<<grid, 256, 0, st>>>(a))));
+    if (a.act == VQHIP_ACT_SILU) GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, true, MASKED><<<grid, 256, sm, st>>>(a))));
+    else GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, false, MASKED><<<grid, 256, sm, st>>>(a))));
     return vq_launch_status("vqhip_group_norm");
 }
 
@@ -549,11 +597,11 @@ extern "C" int vqhip_group_norm_bwd(const vqhip_group_norm_t *p, const void *gra
     const dim3 both(params + (dx ? (unsigned)(a.B * a.S) : 0));
     const size_t sm = (size_t)a.G * 8;
     if (a.act == VQHIP_ACT_SILU) {
-        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_sums_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a)));
-        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_apply_kernel<T, VEC, true><<<both, 256, sm, st>>>(a, params)));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, true, MASKED><<<grid, 256, 0, st>>>(a))));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, true, MASKED><<<both, 256, sm, st>>>(a, params))));
     } else {
-        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_sums_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a)));
-        GN_BY_TYPE(p->dtype, a.C, (vq_gn_bwd_apply_kernel<T, VEC, false><<<both, 256, sm, st>>>(a, params)));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, false, MASKED><<<grid, 256, 0, st>>>(a))));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, false, MASKED><<<both, 256, sm, st>>>(a, params))));
     }
     return vq_launch_status("vqhip_group_norm_bwd");
 }
