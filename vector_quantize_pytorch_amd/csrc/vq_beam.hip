@@ -97,6 +97,20 @@ __device__ __forceinline__ unsigned sel_order(float f)       // ascending like f
 
 __device__ __forceinline__ float sel_value(unsigned u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
 
+// a value that at least K (<= 64) of the wave's 64 values are not below, the K-th largest cut to its upper 20 bits: bisection over the
+// ordered bits, a ballot each.  -inf where fewer than K are above it.
+__device__ __forceinline__ float sel_kth(float f, int K)
+{
+    const unsigned mine = sel_order(f);
+    unsigned kth = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 12; --bit) {
+        const unsigned want = kth | 1u << bit;
+        if (__popcll(__ballot(mine >= want)) >= K) kth = want;
+    }
+    return kth <= 0x007fffffu ? -INFINITY : sel_value(kth);
+}
+
 // exp(x) for x <= 0 (NaN stays NaN, -inf gives 0).  The product's rounding grows with |x|, but so falls the term: a term of weight e^-5
 // is off by 5 steps of fp32, e^-5 of one in the sum.  Measured on normal logits of deviation 1 to 4, 1000 to 131071 of them: log-sums off
 // by 2e-8 to 5e-8 rms, most of it the same for every row (the rounding of log2 e).
@@ -168,16 +182,10 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
     if (t == 0) found = 0;
     __syncthreads();
     gm = group_max[t & 63];
-    float mx = gm;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mx = vq_wave_max(gm);
     if (t >> 6 == NW - 1) {
-        // ranks by value with the lane in the low 6 bits, so that no two are equal; the bound is the value without them
-        const unsigned key = (sel_order(gm) & ~63u) | (unsigned)(t & 63);
-        int rank = 0;
-#pragma unroll
-        for (int k = 0; k < 64; ++k) rank += (unsigned)__builtin_amdgcn_readlane((int)key, k) > key ? 1 : 0;
-        if (rank == K - 1) bound_s = gm > -INFINITY ? sel_value(key & ~63u) : -INFINITY;
+        const float k = sel_kth(gm, K);
+        if ((t & 63) == 0) bound_s = k;
     }
     // the log-sum: 8 terms in 32 bits, the rest in 64; a logit of +inf or NaN makes it NaN
     if (a.normalize) {
@@ -269,6 +277,7 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
         const int2 me = list[i];
         const float f = __int_as_float(me.x);
         int rank = 0;
+#pragma unroll 8
         for (int k = 0; k < n; ++k) {
             const int2 o = list[k];
             const float g = __int_as_float(o.x);
@@ -293,7 +302,8 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
 #define SEL_HELD 4
 __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
 {
-    __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], group_max[64], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
+    __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
+    __shared__ float group_max[64];
     __shared__ int ps[SEL_CAP], found;
     __shared__ uint8_t fin[VQHIP_BEAM_MAX];
     __shared__ double rc[4];
@@ -311,17 +321,14 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
         const bool f = a.finished && a.finished[row], live = !f && s > -INFINITY;
         double lse = 0.0;
         if (a.normalize) {
-            float m = -INFINITY;
-            double sum = 0.0;
-            for (int q = t & 15; q < S; q += 16) {            // running maximum and sum
-                const float pm = a.part_max[row * S + q];
-                const double p = a.part_sum[row * S + q];
-                if (pm > m) { sum = sum == 0.0 ? 0.0 : sum * exp((double)m - (double)pm); m = pm; }
-                sum += p == 0.0 ? 0.0 : p * exp((double)pm - (double)m);
-            }
-            float top = m;
+            float top = -INFINITY;
+            for (int q = t & 15; q < S; q += 16) top = fmaxf(top, a.part_max[row * S + q]);
             for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-            sum = sum == 0.0 ? 0.0 : sum * exp((double)m - (double)top);
+            double sum = 0.0;
+            for (int q = t & 15; q < S; q += 16) {
+                const double p = a.part_sum[row * S + q];
+                sum += p == 0.0 ? 0.0 : p * exp((double)a.part_max[row * S + q] - (double)top);
+            }
             for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
             lse = (double)top + log(sum);                      // (no logit admitted: not finite)
         }
@@ -354,18 +361,13 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
         best = fmax(best, c_held[h]);
     }
     for (int i = SEL_HELD * 256 + t; i < total; i += 256) best = fmax(best, value(i, lists[i], place));
-    best = fmax(best, __shfl_xor(best, 1, 64));
-    best = fmax(best, __shfl_xor(best, 2, 64));
-    if ((t & 3) == 0) group_max[t >> 2] = best;
+    // (32 bits, rounded down: a bound need not be exact)
+    float low = __double2float_rd(best);
+    low = fmaxf(low, __shfl_xor(low, 1, 64));
+    low = fmaxf(low, __shfl_xor(low, 2, 64));
+    if ((t & 3) == 0) group_max[t >> 2] = low;
     __syncthreads();
-    best = group_max[t & 63];
-    int order = 0;
-#pragma unroll 16
-    for (int k = 0; k < 64; ++k) {
-        const double o = group_max[k];
-        order += o > best || (o == best && k < (t & 63)) ? 1 : 0;
-    }
-    const double bound = __shfl(best, __builtin_ctzll(__ballot(order == K - 1)), 64);
+    const double bound = (double)sel_kth(group_max[t & 63], K);
     auto offer = [&](double c, int p) {
         if (c >= bound && c > -INFINITY) {
             const int k = atomicAdd(&found, 1);
@@ -385,6 +387,7 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
             const double c = cs[i];
             const int p = ps[i];
             int rank = 0;
+#pragma unroll 8
             for (int k = 0; k < n; ++k) rank += sel_before(cs[k], ps[k], c, p) ? 1 : 0;
             if (rank < K) {
                 a.scores_out[b * K + rank] = (float)c;
