@@ -5,14 +5,16 @@
 // leave out are neither read into the statistics nor normalised: their output is zero, whatever they hold.
 //
 // Two launches each way, both over (batch entry, chunk of rows): the first leaves each chunk's statistics (backward: its sums), the
-// second joins them -- in every workgroup, S * G pairs from cache -- and writes the rows.  Bound by HBM, with the second read of x from
+// second joins them -- in every workgroup, S * G pairs from cache; beyond GN_JOIN chunks in a small launch between -- and writes the rows.  Bound by HBM, with the second read of x from
 // the memory-side cache where it fits.  A thread keeps VEC channels of every row it visits (16 bytes where C divides so), so parameters and
 // statistics stay in registers and rows of any stride are read in whole lines.  All sums have one order: no atomics.
 #include "vq_elem.h"
 
 #include <math.h>
 
+#define GN_T 512                   // threads of a workgroup
 #define GN_FLUSH 32                // rows that a thread sums about one pivot
+#define GN_JOIN 48                 // chunks that every workgroup of the second launch joins for itself; more are joined in a launch between
 
 struct GnArgs {
     const void *x; int64_t xb, xn;                      // element strides of batch and row
@@ -20,7 +22,7 @@ struct GnArgs {
     const int64_t *lens; const uint8_t *mask;           // either or none
     void *y; float *mean, *rstd;
     const void *grad; void *dx, *dweight, *dbias;       // backward: grad and dx contiguous
-    float2 *pair; float *chan, *live;                   // per chunk: [B * S, G] pairs, (backward) [B * S, 2, C] sums, [B * S] live rows
+    float2 *pair, *joined; float *chan, *live;          // per chunk: [B * S, G] pairs, (backward) [B * S, 2, C] sums, [B * S] live rows; joined [B, G] or null
     int64_t N, B, rows; int C, G, act, wdtype, S;       // S chunks of `rows` rows
     int stream;                                         // results past the caches
     double eps;
@@ -74,8 +76,8 @@ template <typename T, int N> __device__ __forceinline__ void gn_store(T *p, cons
 struct GnShape { int cols, width, lanes; };
 template <int VEC> __device__ __forceinline__ GnShape gn_shape(int C)
 {
-    const int cols = C / VEC, width = cols < 256 ? cols : 256;
-    return GnShape{cols, width, 256 / width};
+    const int cols = C / VEC, width = cols < GN_T ? cols : GN_T;
+    return GnShape{cols, width, GN_T / width};
 }
 
 // sums over the channels of each group that lies in [c0, c1): f(lane entry) -> v[NV] doubles, entries = lanes x channels.  A group that
@@ -84,8 +86,8 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_gro
 {
     const int g0 = c0 / cg, g1 = (c1 - 1) / cg, ng = g1 - g0 + 1;
     int tg = 64;                                        // threads a group: a power of two within a wave
-    while (tg > 1 && tg * ng > 256) tg >>= 1;
-    const int per = 256 / tg;
+    while (tg > 1 && tg * ng > GN_T) tg >>= 1;
+    const int per = GN_T / tg;
     const bool from_before = c0 % cg != 0, goes_on = c1 % cg != 0;
     for (int base = 0; base < ng; base += per) {
         const int g = g0 + base + (int)threadIdx.x / tg, q = threadIdx.x % tg;
@@ -116,9 +118,9 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_gro
 // A thread sums x - p and (x - p)^2 of a channel over up to GN_FLUSH rows, p the first of them: p is one of the values, so what cancels is
 // at most the number of rows -- an outlier or a far mean costs nothing.  Blocks, threads and channels join by counts, means and squared
 // deviations, the last in 64 bits.
-template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_stats_kernel(const GnArgs a)
+template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_stats_kernel(const GnArgs a)
 {
-    __shared__ float em[256 * VEC], ed[256 * VEC], en[256];
+    __shared__ float em[GN_T * VEC], ed[GN_T * VEC], en[GN_T];
     __shared__ double carry[2][3];
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
     const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < len ? r0 + a.rows : len;
@@ -207,23 +209,64 @@ template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(25
     }
 }
 
-// joins the chunks of a batch entry: f(chunk, group) -> v[NV], done(group, v); 64-bit sums in the order of the chunks' lanes
-template <int NV, typename F, typename D> __device__ __forceinline__ void gn_join(int S, int G, F &&entry, D &&done)
+// ---- the chunks of a batch entry joined, 64-bit sums: forward to (mean, rstd), backward to (mean(dz w), mean(dz w xh)) of a group --------
+template <bool BWD> __device__ __forceinline__ void gn_add(const GnArgs &a, int64_t chunk, int g, double *v)
 {
-    int tg = 64;
-    while (tg > 1 && tg * G > 256) tg >>= 1;
-    for (int g = (int)threadIdx.x / tg; g < (G + 256 / tg - 1) / (256 / tg) * (256 / tg); g += 256 / tg) {
-        const int q = threadIdx.x % tg;
-        double v[NV];
+    const float2 p = a.pair[chunk * a.G + g];
+    const double k = a.live[chunk];
+    v[0] += k;
+    if (BWD) {
+        v[1] += p.x;
+        v[2] += p.y;
+    } else {
+        v[1] = fma(k, (double)p.x, v[1]);
+        v[2] += k * fma((double)p.x, (double)p.x, (double)p.y);
+    }
+}
+template <bool BWD> __device__ __forceinline__ float2 gn_joined(const GnArgs &a, const double *v)
+{
+    if (BWD) {
+        const double inv = v[0] > 0.0 ? 1.0 / (v[0] * (a.C / a.G)) : 0.0;
+        return make_float2((float)(v[1] * inv), (float)(v[2] * inv));
+    }
+    const double m = v[0] > 0.0 ? v[1] / v[0] : 0.0, d = v[0] > 0.0 ? (v[2] - v[1] * m) / v[0] : 0.0;
+    return make_float2((float)m, (float)(1.0 / sqrt((d > 0.0 ? d : d == d ? 0.0 : d) + a.eps)));
+}
+
+// many chunks: a launch of its own, a wave each (batch entry, group)
+template <bool BWD> __global__ void __launch_bounds__(256) vq_gn_join_kernel(const GnArgs a)
+{
+    const int64_t bg = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    if (bg >= a.B * a.G) return;
+    const int64_t b = bg / a.G;
+    const int g = (int)(bg - b * a.G);
+    double v[3] = {0.0, 0.0, 0.0};
+#pragma unroll 4
+    for (int s = threadIdx.x & 63; s < a.S; s += 64) gn_add<BWD>(a, b * a.S + s, g, v);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = 0.0;
+    for (int i = 0; i < 3; ++i) v[i] = vq_wave_sum(v[i]);
+    if ((threadIdx.x & 63) == 0) a.joined[bg] = gn_joined<BWD>(a, v);
+}
+
+// few: every workgroup for itself, into LDS
+template <bool BWD> __device__ __forceinline__ void gn_join(const GnArgs &a, int64_t b, float2 *stat)
+{
+    const int S = a.S, G = a.G;
+    if (a.joined) {
+        for (int g = threadIdx.x; g < G; g += GN_T) stat[g] = a.joined[b * G + g];
+        return;
+    }
+    int tg = 64;
+    while (tg > 1 && (tg * G > GN_T || tg / 2 >= S)) tg >>= 1;
+    for (int g = (int)threadIdx.x / tg; g < (G + GN_T / tg - 1) / (GN_T / tg) * (GN_T / tg); g += GN_T / tg) {
+        double v[3] = {0.0, 0.0, 0.0};
         if (g < G)
 #pragma unroll 8
-            for (int s = q; s < S; s += tg) entry(s, g, v);
+            for (int s = threadIdx.x % tg; s < S; s += tg) gn_add<BWD>(a, b * S + s, g, v);
         for (int o = tg >> 1; o; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
-        if (g < G && q == 0) done(g, v);
+            for (int i = 0; i < 3; ++i) v[i] += __shfl_xor(v[i], o, 64);
+        if (g < G && threadIdx.x % tg == 0) stat[g] = gn_joined<BWD>(a, v);
     }
 }
 
@@ -237,30 +280,16 @@ template <typename T, int VEC> __device__ __forceinline__ void gn_zero_rows(T *p
     for (int64_t r = from; r < to; r += step) vq_stv<T, VEC>(p + r * stride, o);
 }
 
-template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_apply_kernel(const GnArgs a)
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_apply_kernel(const GnArgs a)
 {
-    extern __shared__ float stat[];                     // mean [G], rstd [G]
+    extern __shared__ float2 stat[];                    // (mean, rstd) [G]
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
     const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, end = r0 + a.rows < a.N ? r0 + a.rows : a.N, r1 = end < len ? end : len;
     const int G = a.G, cg = a.C / G;
-    const float *rows = a.live + b * a.S;
-    const float2 *pair = a.pair + b * a.S * G;
-    gn_join<3>(a.S, G,
-        [&](int s, int g, double *v) {
-            const float2 p = pair[(int64_t)s * G + g];
-            const double k = rows[s], m = p.x;
-            v[0] += k;
-            v[1] = fma(k, m, v[1]);
-            v[2] += k * fma(m, m, (double)p.y);
-        },
-        [&](int g, const double *v) {
-            const double m = v[0] > 0.0 ? v[1] / v[0] : 0.0, d = v[0] > 0.0 ? (v[2] - v[1] * m) / v[0] : 0.0;
-            const float mf = (float)m, rf = (float)(1.0 / sqrt((d > 0.0 ? d : d == d ? 0.0 : d) + a.eps));
-            stat[g] = mf;
-            stat[G + g] = rf;
-            if (chunk == 0) { a.mean[b * G + g] = mf; a.rstd[b * G + g] = rf; }
-        });
+    gn_join<false>(a, b, stat);
     __syncthreads();
+    if (chunk == 0)
+        for (int g = t; g < G; g += GN_T) { a.mean[b * G + g] = stat[g].x; a.rstd[b * G + g] = stat[g].y; }
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width;
     if (lane >= sh.lanes) return;
@@ -277,9 +306,9 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const int g = (col * VEC + i) / cg;
-            mean[i] = FOLD ? 0.f : stat[g];
-            scale[i] *= stat[G + g];
-            if (FOLD) shift[i] = fmaf(-stat[g], scale[i], shift[i]);
+            mean[i] = FOLD ? 0.f : stat[g].x;
+            scale[i] *= stat[g].y;
+            if (FOLD) shift[i] = fmaf(-stat[g].x, scale[i], shift[i]);
         }
         const T *xc = x + (int64_t)col * VEC;
         T *yc = y + (int64_t)col * VEC;
@@ -320,9 +349,9 @@ template <bool SILU> __device__ __forceinline__ float gn_dz(float g, float xh, f
 }
 
 // first launch: each chunk's sums of dz and dz xh of every channel, and of w times them of every group
-template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_bwd_sums_kernel(const GnArgs a)
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_bwd_sums_kernel(const GnArgs a)
 {
-    __shared__ float e0[256 * VEC], e1[256 * VEC], en[256];
+    __shared__ float e0[GN_T * VEC], e1[GN_T * VEC], en[GN_T];
     __shared__ double carry[2][2];
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x, G = a.G, cg = a.C / G;
     const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < len ? r0 + a.rows : len;
@@ -380,7 +409,7 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
             for (int l = 0; l < sh.lanes; ++l) rows += en[l * sh.width];
             a.live[blockIdx.x] = rows;
         }
-        for (int c = c0 + t; c < c1; c += 256) {
+        for (int c = c0 + t; c < c1; c += GN_T) {
             float q0 = 0.f, q1 = 0.f;
             for (int l = 0; l < sh.lanes; ++l) { q0 += e0[l * wide + c - c0]; q1 += e1[l * wide + c - c0]; }
             chan[c] = q0;
@@ -402,22 +431,22 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
 
 // second launch: the first workgroups sum dweight and dbias over chunks and batch (GN_PARAM channels each), the others write dx
 #define GN_PARAM 16
-template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(256) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
+template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
 {
-    extern __shared__ float stat[];                     // mean(dz w) [G], mean(dz w xh) [G]
+    extern __shared__ float2 stat[];                    // (mean(dz w), mean(dz w xh)) [G]
     const int t = threadIdx.x, G = a.G, cg = a.C / G;
     if (blockIdx.x < param_blocks) {
-        __shared__ double red[2][256 / GN_PARAM][GN_PARAM];
+        __shared__ double red[2][GN_T / GN_PARAM][GN_PARAM];
         const int c = blockIdx.x * GN_PARAM + t % GN_PARAM, q = t / GN_PARAM;
         double v0 = 0.0, v1 = 0.0;
         if (c < a.C)
 #pragma unroll 8
-            for (int64_t s = q; s < a.B * a.S; s += 256 / GN_PARAM) { v0 += a.chan[s * a.C * 2 + c]; v1 += a.chan[s * a.C * 2 + a.C + c]; }
+            for (int64_t s = q; s < a.B * a.S; s += GN_T / GN_PARAM) { v0 += a.chan[s * a.C * 2 + c]; v1 += a.chan[s * a.C * 2 + a.C + c]; }
         red[0][q][t % GN_PARAM] = v0;
         red[1][q][t % GN_PARAM] = v1;
         __syncthreads();
         if (q == 0 && c < a.C) {
-            for (int k = 1; k < 256 / GN_PARAM; ++k) { v0 += red[0][k][t]; v1 += red[1][k][t]; }
+            for (int k = 1; k < GN_T / GN_PARAM; ++k) { v0 += red[0][k][t]; v1 += red[1][k][t]; }
             if (a.dbias) gn_store_param(a.dbias, a.wdtype, c, (float)v0);
             if (a.dweight) gn_store_param(a.dweight, a.wdtype, c, (float)v1);
         }
@@ -426,20 +455,7 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
     const unsigned block = blockIdx.x - param_blocks;
     const int chunk = block % (unsigned)a.S;
     const int64_t b = block / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, end = r0 + a.rows < a.N ? r0 + a.rows : a.N, r1 = end < len ? end : len;
-    const float *rows = a.live + b * a.S;
-    const float2 *pair = a.pair + b * a.S * G;
-    gn_join<3>(a.S, G,
-        [&](int s, int g, double *v) {
-            const float2 p = pair[(int64_t)s * G + g];
-            v[0] += rows[s];
-            v[1] += p.x;
-            v[2] += p.y;
-        },
-        [&](int g, const double *v) {
-            const double inv = v[0] > 0.0 ? 1.0 / (v[0] * cg) : 0.0;
-            stat[g] = (float)(v[1] * inv);
-            stat[G + g] = (float)(v[2] * inv);
-        });
+    gn_join<true>(a, b, stat);
     __syncthreads();
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width;
@@ -456,8 +472,8 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
             const int g = (col * VEC + i) / cg;
             mean[i] = a.mean[b * G + g];
             rstd[i] = a.rstd[b * G + g];
-            m1[i] = stat[g];
-            m2[i] = stat[G + g];
+            m1[i] = stat[g].x;
+            m2[i] = stat[g].y;
         }
         for (int64_t r = r0 + lane; r < r1; r += 2 * sh.lanes) {
             VqVec<T, VEC> v[2], d[2];
@@ -495,12 +511,13 @@ __global__ void __launch_bounds__(256) vq_gn_zero_params_kernel(void *dweight, v
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
-// Four workgroups a CU in all, at most 256 chunks of an entry (every workgroup of the second launch reads them), at least 4096 elements each
+// Two workgroups a CU in all, at most 256 chunks of an entry, at least 8192 elements each.  (6 x 65536 x 128 bf16, second launch: 45 us with
+// 1020 workgroups of 256 threads that each join 170 chunks, 38 us with half as many.)
 static void gn_plan(int64_t B, int64_t N, int64_t C, int64_t *S, int64_t *rows)
 {
-    int64_t s = B >= 1024 ? 1 : 1024 / B;
+    int64_t s = B >= 512 ? 1 : 512 / B;
     if (s > 256) s = 256;
-    const int64_t least = C >= 4096 ? 1 : 4096 / C;
+    const int64_t least = C >= 8192 ? 1 : 8192 / C;
     int64_t r = (N + s - 1) / s;
     if (r < least) r = least;
     *rows = r;
@@ -532,7 +549,8 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     // results of more than a quarter of the 256 MB memory-side cache go past it: 6 x 65536 x 128 bf16 90 -> 80 us with x still in it
     a.stream = p->B * p->N * p->C * vq_elem_bytes(p->dtype) > (64 << 20);
     a.S = (int)S; a.rows = rows; a.eps = p->eps;
-    a.pair = (float2 *)p->workspace; a.chan = (float *)(a.pair + p->B * S * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
+    a.pair = (float2 *)p->workspace; a.joined = a.pair + p->B * S * p->groups; a.chan = (float *)(a.joined + p->B * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
+    if (S <= GN_JOIN) a.joined = nullptr;
     return a;
 }
 
@@ -541,7 +559,7 @@ extern "C" size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t
     if (B <= 0 || N <= 0 || C <= 0 || groups <= 0) return 0;
     int64_t S, rows;
     gn_plan(B, N, C, &S, &rows);
-    return (size_t)(B * S) * (size_t)(1 + 2 * groups + 2 * C) * 4;
+    return ((size_t)(B * S) * (size_t)(1 + 2 * groups + 2 * C) + (size_t)(B * groups) * 2) * 4;
 }
 
 // channels of a thread: 16 bytes where C divides so, fewer where not
@@ -573,9 +591,10 @@ extern "C" int vqhip_group_norm(const vqhip_group_norm_t *p, void *y, void *stre
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(a.B * a.S));
     const size_t sm = (size_t)a.G * 8;
-    GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_stats_kernel<T, VEC, MASKED><<<grid, 256, 0, st>>>(a))));
-    if (a.act == VQHIP_ACT_SILU) GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, true, MASKED><<<grid, 256, sm, st>>>(a))));
-    else GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, false, MASKED><<<grid, 256, sm, st>>>(a))));
+    GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_stats_kernel<T, VEC, MASKED><<<grid, GN_T, 0, st>>>(a))));
+    if (a.joined) vq_gn_join_kernel<false><<<dim3((unsigned)((a.B * a.G + 3) / 4)), 256, 0, st>>>(a);
+    if (a.act == VQHIP_ACT_SILU) GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, true, MASKED><<<grid, GN_T, sm, st>>>(a))));
+    else GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_apply_kernel<T, VEC, false, MASKED><<<grid, GN_T, sm, st>>>(a))));
     return vq_launch_status("vqhip_group_norm");
 }
 
@@ -597,11 +616,13 @@ extern "C" int vqhip_group_norm_bwd(const vqhip_group_norm_t *p, const void *gra
     const dim3 both(params + (dx ? (unsigned)(a.B * a.S) : 0));
     const size_t sm = (size_t)a.G * 8;
     if (a.act == VQHIP_ACT_SILU) {
-        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, true, MASKED><<<grid, 256, 0, st>>>(a))));
-        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, true, MASKED><<<both, 256, sm, st>>>(a, params))));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, true, MASKED><<<grid, GN_T, 0, st>>>(a))));
+        if (a.joined && dx) vq_gn_join_kernel<true><<<dim3((unsigned)((a.B * a.G + 3) / 4)), 256, 0, st>>>(a);
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, true, MASKED><<<both, GN_T, sm, st>>>(a, params))));
     } else {
-        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, false, MASKED><<<grid, 256, 0, st>>>(a))));
-        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, false, MASKED><<<both, 256, sm, st>>>(a, params))));
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, false, MASKED><<<grid, GN_T, 0, st>>>(a))));
+        if (a.joined && dx) vq_gn_join_kernel<true><<<dim3((unsigned)((a.B * a.G + 3) / 4)), 256, 0, st>>>(a);
+        GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_apply_kernel<T, VEC, false, MASKED><<<both, GN_T, sm, st>>>(a, params))));
     }
     return vq_launch_status("vqhip_group_norm_bwd");
 }
