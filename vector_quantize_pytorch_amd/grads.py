@@ -18,18 +18,31 @@ class _Grad(ctypes.Structure):                            # vqhip_grad_t
 
 
 @L._on_device
-def _clip(first, grads, outs, max_norm):
-    lib, count = L.lib(), len(grads)
-    src = [g.data_ptr() for g in grads]
-    dst = [0] * count if outs is None else [o.data_ptr() for o in outs]                      # 0: the norm alone
-    rows = zip(src, dst, [g.numel() for g in grads], [L._ELEM_CODES[g.dtype] for g in grads])
-    table = array.array("q", [v for row in rows for v in row])                               # vqhip_grad_t [count]
-    at = table.buffer_info()[0]
+def _clip(first, table, max_norm):
+    """table: array('q') of vqhip_grad_t rows"""
+    lib, (at, fields) = L.lib(), table.buffer_info()
     norm = torch.empty((), dtype=torch.float32, device=first.device)
-    nws = lib.vqhip_clip_grads_workspace_bytes(at, count)
+    nws = lib.vqhip_clip_grads_workspace_bytes(at, fields // 4)
     ws = torch.empty(nws, dtype=torch.uint8, device=first.device)
-    L._check(lib.vqhip_clip_grads(at, count, max_norm, _EPS, norm.data_ptr(), ws.data_ptr(), nws, L._stream()), "vqhip_clip_grads")
+    L._check(lib.vqhip_clip_grads(at, fields // 4, max_norm, _EPS, norm.data_ptr(), ws.data_ptr(), nws, L._stream()), "vqhip_clip_grads")
     return norm
+
+
+def _table(grads, out):
+    """the checked rows of vqhip_grad_t; out None: the norm alone"""
+    codes, dev, flat = L._ELEM_CODES, grads[0].get_device(), []
+    for g, o in zip(grads, out if out is not None else grads):          # (one pass: a model has hundreds)
+        dt, n = g.dtype, g.numel()
+        if dt not in codes:
+            L._elem_code(g, "clip_grads")
+        if not g.is_contiguous():
+            raise L.VQHipError(f"clip_grads: tensor {tuple(g.shape)} with strides {g.stride()}, expected a contiguous one")
+        if g.get_device() != dev:
+            raise L.VQHipError(f"clip_grads: tensors on different devices ({grads[0].device} and {g.device})")
+        if o is not g and (o.numel() != n or o.dtype != dt or not o.is_contiguous() or o.get_device() != dev):
+            raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {n} contiguous elements of {dt} on {g.device}")
+        flat += (g.data_ptr(), o.data_ptr() if out is not None else 0, n, codes[dt])
+    return array.array("q", flat)
 
 
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[Sequence[torch.Tensor]] = None):
@@ -44,25 +57,18 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")
     if not grads:
         return [], torch.zeros((), dtype=torch.float32)
-    dev = grads[0].get_device()
-    for g in grads:
-        if g.dtype not in L._ELEM_CODES:
-            L._elem_code(g, "clip_grads")
-        if not g.is_contiguous():
-            raise L.VQHipError(f"clip_grads: tensor {tuple(g.shape)} with strides {g.stride()}, expected a contiguous one")
-        if g.get_device() != dev:
-            raise L.VQHipError(f"clip_grads: tensors on different devices ({grads[0].device} and {g.device})")
-    if out is not None:
+    if out is None:
+        table = _table(grads, None)
+        L._need_gpu(grads[0])
+        out = [torch.empty_like(g) for g in grads]
+        table[1::4] = array.array("q", [o.data_ptr() for o in out])
+    else:
         out = list(out)
         if len(out) != len(grads):
             raise L.VQHipError(f"clip_grads: {len(out)} results for {len(grads)} tensors")
-        for g, o in zip(grads, out):
-            if o is not g and (o.numel() != g.numel() or o.dtype != g.dtype or o.get_device() != dev or not o.is_contiguous()):
-                raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {g.numel()} contiguous elements of {g.dtype} on {g.device}")
-    L._need_gpu(grads[0])
-    if out is None:
-        out = [torch.empty_like(g) for g in grads]
-    norm = _clip(grads[0], grads, out, float(max_norm))
+        table = _table(grads, out)
+        L._need_gpu(grads[0])
+    norm = _clip(grads[0], table, float(max_norm))
     L._written(out)
     return out, norm
 
@@ -76,8 +82,9 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, error_i
     grads = list({id(p.grad): p.grad.detach() for p in parameters if p.grad is not None}.values())      # a shared one counts once
     work = [g if g.is_contiguous() else g.contiguous() for g in grads]
     if error_if_nonfinite and work:
-        L._need_gpu(*work[:1])
-        if not torch.isfinite(_clip(work[0], work, None, 0.0)).item():
+        table = _table(work, None)
+        L._need_gpu(work[0])
+        if not torch.isfinite(_clip(work[0], table, 0.0)).item():
             raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
     _, norm = clip_grads(work, max_norm, out=work)
     for g, w in zip(grads, work):
