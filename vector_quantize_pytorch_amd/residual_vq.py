@@ -564,17 +564,17 @@ class ResidualVQ(nn.Module):
                 raise RuntimeError("ResidualVQ: beam search scores codes by their commitment loss, which exists in training and with "
                                    "commitment_weight > 0 only")
             J, K = ind.shape[-2:]
-            gain = -(loss.detach().float() * self.beam_score_weights[qi])                    # [b, n, J, K]
+            total = scores[..., None] - loss.detach().float() * self.beam_score_weights[qi]  # [b, n, J, K], rounded to fp32 as rvq.py's are
             keep = beam_size if qi != last else 1
             if J * K <= keep:                                       # everything survives, in place
-                scores = (scores[..., None] + gain).flatten(-2)
+                scores = total.flatten(-2)
                 at = torch.arange(J * K, device=x.device).expand(*lead, J * K)
                 parents = at // K
             elif max(J, keep) <= BEAM_MAX:
-                scores, parents, tokens = beam_select(gain, scores, keep, normalize=False)
+                scores, parents, tokens = beam_select(total, None, keep, normalize=False)
                 at = parents * K + tokens
             else:
-                scores, at = (scores[..., None] + gain).flatten(-2).topk(keep, dim=-1)
+                scores, at = total.flatten(-2).topk(keep, dim=-1)
                 parents = at // K
             if want_inputs:
                 inputs.append(residual)
