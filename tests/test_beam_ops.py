@@ -403,6 +403,11 @@ def test_c_entry_refusals():
         s = _Select(**{**ok, **change})
         assert L.vqhip_beam_select(ctypes.byref(s), None) == rc, change
     assert L.vqhip_beam_select(None, None) == -1
+    big = dict(ok, V=5000, stride_j=5000)
+    nws = L.vqhip_beam_select_workspace_bytes(1, 2, 5000, 3)
+    for rc, ws, size in [(-1, None, 0), (-1, 16, nws - 1), (-3, 24, nws)]:
+        s = _Select(**big, workspace=ws, workspace_bytes=size)
+        assert L.vqhip_beam_select(ctypes.byref(s), None) == rc
     s = _Select(**ok)
     assert L.vqhip_beam_select_bwd(ctypes.byref(s), None, 8, 8, None) == -1              # no gradient
     assert L.vqhip_beam_select_bwd(ctypes.byref(s), 8, 8, 8, None) == -1                 # normalized, no log-sums

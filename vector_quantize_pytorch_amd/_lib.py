@@ -257,7 +257,10 @@ def _need_gpu(*ts):
 
 def _written(tensors):
     """tells autograd that the library wrote into tensors of the caller (a graph that saved one then refuses its backward)"""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                                     # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _ptr(t):

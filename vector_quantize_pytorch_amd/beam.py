@@ -46,7 +46,8 @@ def _addr(t):
 
 def _table(t: torch.Tensor, b: int, j: int, v: int) -> torch.Tensor:
     """t [..., j, v] as [b, j, v] with contiguous continuations, without a copy where the layout allows it"""
-    t = t.reshape(b, j, v)
+    if t.ndim != 3:
+        t = t.reshape(b, j, v)
     return t if t.stride(-1) == 1 or v == 1 else t.contiguous()
 
 
@@ -140,11 +141,12 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
         raise L.VQHipError(f"beam_select: {beam_size} survivors of {j} x {v} continuations: takes 1 to {BEAM_MAX} beams and survivors, "
                            "no more survivors than continuations")
     L._need_gpu(logits, scores, mask, finished)
+    beam_size = int(beam_size)
     n = 1
     for d in lead:
         n *= d
     lg = _table(logits, n, j, v)
-    sc = None if scores is None else scores.reshape(n, j).contiguous()
+    sc = scores if scores is None or (len(lead) == 1 and scores.is_contiguous()) else scores.reshape(n, j).contiguous()
     mk = None if mask is None else _table(mask, n, j, v).view(torch.uint8)
     fin = None if finished is None else finished.reshape(n, j).contiguous().view(torch.uint8)
     end = 0 if finished is None else int(end_token)

@@ -477,6 +477,7 @@ extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
     if (p->B == 0) return 0;
     const size_t need = vqhip_beam_select_workspace_bytes(p->B, p->J, p->V, p->K);
     if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select: workspace of %zu bytes, needs %zu", p->workspace_bytes, need);
+    if ((uintptr_t)p->workspace & 15) VQ_FAIL(VQHIP_EALIGN, "vqhip_beam_select: workspace not 16-byte aligned");
     SelArgs a;
     a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.scores = p->scores;
     a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j; a.finished = p->finished;

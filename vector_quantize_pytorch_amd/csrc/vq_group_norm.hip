@@ -282,7 +282,7 @@ template <typename T, int VEC> __device__ __forceinline__ void gn_zero_rows(T *p
 
 template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_apply_kernel(const GnArgs a)
 {
-    extern __shared__ float2 stat[];                    // (mean, rstd) [G]
+    extern __shared__ __align__(16) float2 stat[];      // (mean, rstd) [G]
     const int chunk = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
     const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, end = r0 + a.rows < a.N ? r0 + a.rows : a.N, r1 = end < len ? end : len;
     const int G = a.G, cg = a.C / G;
@@ -433,10 +433,10 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
 #define GN_PARAM 16
 template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_bwd_apply_kernel(const GnArgs a, unsigned param_blocks)
 {
-    extern __shared__ float2 stat[];                    // (mean(dz w), mean(dz w xh)) [G]
+    extern __shared__ __align__(16) float2 stat[];      // (mean(dz w), mean(dz w xh)) [G]; the first workgroups' partial sums
     const int t = threadIdx.x, G = a.G, cg = a.C / G;
     if (blockIdx.x < param_blocks) {
-        __shared__ double red[2][GN_T / GN_PARAM][GN_PARAM];
+        double (*red)[GN_T / GN_PARAM][GN_PARAM] = (double (*)[GN_T / GN_PARAM][GN_PARAM])stat;          // (with it, 8192 groups would pass 64 KB)
         const int c = blockIdx.x * GN_PARAM + t % GN_PARAM, q = t / GN_PARAM;
         double v0 = 0.0, v1 = 0.0;
         if (c < a.C)
@@ -535,6 +535,7 @@ static int gn_check(const vqhip_group_norm_t *p, const char *what)
     if (p->B > 0 && p->N > 0 && (!p->x || !p->mean || !p->rstd)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
     const size_t need = vqhip_group_norm_workspace_bytes(p->B, p->N, p->C, p->groups);
     if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "%s: workspace of %zu bytes, needs %zu", what, p->workspace_bytes, need);
+    if ((uintptr_t)p->workspace & 15) VQ_FAIL(VQHIP_EALIGN, "%s: workspace not 16-byte aligned", what);
     return 0;
 }
 
@@ -614,7 +615,7 @@ extern "C" int vqhip_group_norm_bwd(const vqhip_group_norm_t *p, const void *gra
     const dim3 grid((unsigned)(a.B * a.S));
     const unsigned params = dweight || dbias ? (unsigned)((a.C + GN_PARAM - 1) / GN_PARAM) : 0;
     const dim3 both(params + (dx ? (unsigned)(a.B * a.S) : 0));
-    const size_t sm = (size_t)a.G * 8;
+    const size_t sums = (size_t)2 * GN_T * 8, sm = (size_t)a.G * 8 > sums ? (size_t)a.G * 8 : sums;
     if (a.act == VQHIP_ACT_SILU) {
         GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_bwd_sums_kernel<T, VEC, true, MASKED><<<grid, GN_T, 0, st>>>(a))));
         if (a.joined && dx) vq_gn_join_kernel<true><<<dim3((unsigned)((a.B * a.G + 3) / 4)), 256, 0, st>>>(a);

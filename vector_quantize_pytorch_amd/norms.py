@@ -26,24 +26,26 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _struct(x, weight, bias, lens, mask, groups, eps, act, stats):
+def _struct(x, weight, bias, lens, mask, groups, eps, act, mean, ws, nws):
     b, n, c = x.shape
     sb, sn, _ = x.stride()
-    nws = L.lib().vqhip_group_norm_workspace_bytes(b, n, c, groups)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
     param = weight if weight is not None else bias
-    mean = stats.data_ptr()
-    return ws, _Norm(x.data_ptr(), L._ELEM_CODES[x.dtype], b, n, c, sb, sn, groups, _addr(weight), _addr(bias),
-                     L.F32 if param is None else L._ELEM_CODES[param.dtype], eps, act, _addr(lens), _addr(mask), mean, mean + 4 * b * groups, _addr(ws), nws)
+    return _Norm(x.data_ptr(), L._ELEM_CODES[x.dtype], b, n, c, sb, sn, groups, _addr(weight), _addr(bias),
+                 L.F32 if param is None else L._ELEM_CODES[param.dtype], eps, act, _addr(lens), _addr(mask), mean, mean + 4 * b * groups, ws, nws)
 
 
 @L._on_device
-def _forward(x, weight, bias, lens, mask, groups, eps, act):
+def _forward(x, weight, bias, lens, mask, groups, eps, act, keep):
+    """keep: mean and rstd in memory of their own, for a backward; otherwise behind the workspace"""
     b, n, c = x.shape
-    y = torch.empty(b, n, c, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, b, groups, dtype=torch.float32, device=x.device)
-    ws, s = _struct(x, weight, bias, lens, mask, groups, eps, act, stats)
-    L._check(L.lib().vqhip_group_norm(ctypes.byref(s), _addr(y), L._stream()), "vqhip_group_norm")
+    lib, dev = L.lib(), x.device
+    y = torch.empty((b, n, c), dtype=x.dtype, device=dev)
+    nws = lib.vqhip_group_norm_workspace_bytes(b, n, c, groups)
+    stats = torch.empty((2, b, groups), dtype=torch.float32, device=dev) if keep else None
+    ws = torch.empty(nws + (0 if keep else 8 * b * groups), dtype=torch.uint8, device=dev)
+    at = ws.data_ptr()
+    s = _struct(x, weight, bias, lens, mask, groups, eps, act, stats.data_ptr() if keep else at + nws, at, nws)
+    L._check(lib.vqhip_group_norm(ctypes.byref(s), y.data_ptr(), L._stream()), "vqhip_group_norm")
     return y, stats
 
 
@@ -52,15 +54,18 @@ def _backward(grad, x, weight, bias, lens, mask, groups, eps, act, stats, want_x
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
     dw = torch.empty_like(weight) if want_w else None
     db = torch.empty_like(bias) if want_b else None
-    ws, s = _struct(x, weight, bias, lens, mask, groups, eps, act, stats)
-    L._check(L.lib().vqhip_group_norm_bwd(ctypes.byref(s), _addr(grad), _addr(dx), _addr(dw), _addr(db), L._stream()), "vqhip_group_norm_bwd")
+    lib = L.lib()
+    nws = lib.vqhip_group_norm_workspace_bytes(*x.shape, groups)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    s = _struct(x, weight, bias, lens, mask, groups, eps, act, stats.data_ptr(), ws.data_ptr(), nws)
+    L._check(lib.vqhip_group_norm_bwd(ctypes.byref(s), _addr(grad), _addr(dx), _addr(dw), _addr(db), L._stream()), "vqhip_group_norm_bwd")
     return dx, dw, db
 
 
 class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, lens, mask, groups, eps, act):
-        y, stats = _forward(x, weight, bias, lens, mask, groups, eps, act)
+        y, stats = _forward(x, weight, bias, lens, mask, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, lens, mask, stats)
         ctx.args = groups, eps, act
         return y
@@ -80,7 +85,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
 
     Mean and variance of each of the `num_groups` channel groups over all positions of a batch entry, in 32 bits or more, whatever x's
     type; activation None or 'silu'.  weight, bias [c]: both of one type, float32 or x's, either may be left out.
-    mask / lens: as in VectorQuantize.forward for x [b, n, c] -- bool [b, n], or the number of live rows [b] (int64; more than n counts as
+    mask / lens: as in VectorQuantize.forward for x [b, n, c] -- bool [b, n], or the number of live rows [b] (integers; more than n counts as
     n, less than 1 as none).  Padding rows take no part in the statistics, may hold anything, and give zeros, gradients as well."""
     L._elem_code(x, "group_norm")
     if x.ndim < 2:
@@ -101,21 +106,24 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         raise L.VQHipError("group_norm: mask and lens")
     if mask is not None and (x.ndim != 3 or mask.dtype != torch.bool or tuple(mask.shape) != tuple(x.shape[:2])):
         raise L.VQHipError(f"group_norm: mask {tuple(mask.shape)} {mask.dtype} for x {tuple(x.shape)}, expected bool [b, n] for [b, n, c]")
-    if lens is not None and (x.ndim != 3 or lens.dtype != torch.int64 or tuple(lens.shape) != (b,)):
-        raise L.VQHipError(f"group_norm: lens {tuple(lens.shape)} {lens.dtype} for x {tuple(x.shape)}, expected int64 [b] for [b, n, c]")
+    if lens is not None and (x.ndim != 3 or lens.dtype not in (torch.int64, torch.int32) or tuple(lens.shape) != (b,)):
+        raise L.VQHipError(f"group_norm: lens {tuple(lens.shape)} {lens.dtype} for x {tuple(x.shape)}, expected integers [b] for [b, n, c]")
     L._need_gpu(x, weight, bias, mask, lens)
-    rows = x.flatten(1, -2) if x.ndim > 2 else x[:, None]
+    rows = x if x.ndim == 3 else x.flatten(1, -2) if x.ndim > 3 else x[:, None]
     if rows.stride(-1) != 1 and c > 1:
         rows = rows.contiguous()
-    w, q = (None if p is None else p.contiguous() for p in (weight, bias))
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     mk = None if mask is None else mask.contiguous().view(torch.uint8)
-    ln = None if lens is None else lens.contiguous()
-    args = (rows, w, q, ln, mk, num_groups, float(eps), _ACTIVATIONS[activation])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    ln = None if lens is None else lens.to(torch.int64).contiguous()
+    args = (rows, weight, bias, ln, mk, num_groups, float(eps), _ACTIVATIONS[activation])
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _GroupNormFn.apply(*args)
     else:
-        y, _ = _forward(*args)
-    return y.view(x.shape)
+        y, _ = _forward(*args, False)
+    return y if x.ndim == 3 else y.view(x.shape)
 
 
 class GroupNorm(nn.Module):
