@@ -80,6 +80,13 @@ template <int VEC> __device__ __forceinline__ GnShape gn_shape(int C)
     return GnShape{cols, width, GN_T / width};
 }
 
+// the groups of channels that follow each other: one division, then steps
+struct GnGroup {
+    int g, r, cg;
+    __device__ GnGroup(int c, int cg_) : g(c / cg_), r(c - c / cg_ * cg_), cg(cg_) {}
+    __device__ __forceinline__ void next() { if (++r == cg) { r = 0; ++g; } }
+};
+
 // sums over the channels of each group that lies in [c0, c1): f(lane entry) -> v[NV] doubles, entries = lanes x channels.  A group that
 // goes on in the next pass is carried there (two places, since one pass may read and write it).  done(g, v) by one thread a group.
 template <int NV, typename F, typename D> __device__ __forceinline__ void gn_groups(int c0, int c1, int cg, int lanes, const double *carry_in, double *carry_out, F &&entry, D &&done)
@@ -96,7 +103,10 @@ template <int NV, typename F, typename D> __device__ __forceinline__ void gn_gro
         for (int i = 0; i < NV; ++i) v[i] = 0.0;
         if (g <= g1) {
             const int lo = g * cg < c0 ? c0 : g * cg, hi = (g + 1) * cg > c1 ? c1 : (g + 1) * cg, wide = hi - lo;
-            for (int e = q; e < wide * lanes; e += tg) entry(e / wide, lo + e % wide, v);
+            for (int l = q / wide, c = q - l * wide; l < lanes;) {             // entry l * wide + c, then tg further
+                entry(l, lo + c, v);
+                for (c += tg; c >= wide; c -= wide) ++l;
+            }
         }
         for (int o = tg >> 1; o; o >>= 1)
 #pragma unroll
@@ -126,6 +136,7 @@ template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(GN
     const int64_t b = blockIdx.x / (unsigned)a.S, len = gn_len(a, b), r0 = (int64_t)chunk * a.rows, r1 = r0 + a.rows < len ? r0 + a.rows : len;
     const GnShape sh = gn_shape<VEC>(a.C);
     const int lane = t / sh.width, cg = a.C / a.G;
+    const bool whole = cg % VEC == 0;
     const T *x = (const T *)a.x + b * a.xb;
     const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     float2 *out = a.pair + (int64_t)blockIdx.x * a.G;
@@ -182,24 +193,34 @@ template <typename T, int VEC, bool MASKED> __global__ void __launch_bounds__(GN
                 }
             }
         }
+        // a thread's channels in one group are joined here: an entry a thread instead of VEC
+        if (whole) {
+            float m = 0.f, d = 0.f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { em[t * VEC + i] = mean[i]; ed[t * VEC + i] = dev[i]; }
+            for (int i = 0; i < VEC; ++i) m += mean[i] * (1.f / VEC);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d += fmaf((mean[i] - m) * (mean[i] - m), n, dev[i]);
+            em[t] = m;
+            ed[t] = d;
+        } else
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) { em[t * VEC + i] = mean[i]; ed[t * VEC + i] = dev[i]; }
         en[t] = n;
         __syncthreads();
-        const int c0 = col0 * VEC, c1 = (col0 + sh.width < sh.cols ? col0 + sh.width : sh.cols) * VEC;
         if (t == 0 && col0 == 0) {
             float rows = 0.f;
             for (int l = 0; l < sh.lanes; ++l) rows += en[l * sh.width];
             a.live[blockIdx.x] = rows;
         }
         // 64-bit sums about zero: count, count * mean, squared deviations + count * mean^2
-        gn_groups<3>(c0, c1, cg, sh.lanes, carry[pass & 1], carry[~pass & 1],
+        const int per = whole ? 1 : VEC, last = col0 + sh.width < sh.cols ? col0 + sh.width : sh.cols;
+        gn_groups<3>(col0 * per, last * per, whole ? cg / VEC : cg, sh.lanes, carry[pass & 1], carry[~pass & 1],
             [&](int l, int c, double *v) {
-                const int e = l * sh.width * VEC + (c - c0);
-                const double k = en[l * sh.width + (c - c0) / VEC], m = em[e];
-                v[0] += k;
-                v[1] = fma(k, m, v[1]);
-                v[2] += fma(k * m, m, (double)ed[e]);
+                const int k = c - col0 * per, e = l * sh.width * per + k;
+                const double w = whole ? en[e] * VEC : en[l * sh.width + k / VEC], m = em[e];
+                v[0] += w;
+                v[1] = fma(w, m, v[1]);
+                v[2] += fma(w * m, m, (double)ed[e]);
             },
             [&](int g, const double *v) {
                 const double m = v[0] > 0.0 ? v[1] / v[0] : 0.0, d = v[0] > 0.0 ? (v[2] - v[1] * m) / v[0] : 0.0;
@@ -303,12 +324,13 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
         float mean[VEC], scale[VEC], shift[VEC];
         gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, scale);
         gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, shift);
+        GnGroup of(col * VEC, cg);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int g = (col * VEC + i) / cg;
-            mean[i] = FOLD ? 0.f : stat[g].x;
-            scale[i] *= stat[g].y;
-            if (FOLD) shift[i] = fmaf(-stat[g].x, scale[i], shift[i]);
+        for (int i = 0; i < VEC; ++i, of.next()) {
+            const float2 st = stat[of.g];
+            mean[i] = FOLD ? 0.f : st.x;
+            scale[i] *= st.y;
+            if (FOLD) shift[i] = fmaf(-st.x, scale[i], shift[i]);
         }
         const T *xc = x + (int64_t)col * VEC;
         T *yc = y + (int64_t)col * VEC;
@@ -336,6 +358,133 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
             }
         }
         gn_zero_rows<T, VEC>(yc, (r0 > len ? r0 : len) + lane, end, sh.lanes, a.C);
+    }
+}
+
+// ---- forward, small slabs in one launch -----------------------------------------------------------------------------------------------
+// A workgroup keeps all rows of a span of whole groups (128 bytes of a row or more, a power of two of columns) in registers, U rows a
+// thread: x is read once.  The mean first, then the deviations from it, whose own mean corrects it; 32 bits hold both.  A wave's rows
+// join by shuffles, the waves in LDS, and every thread sums its groups' channels for itself.  Bound by latency and by the instructions of a
+// wave: 1 x 256 x 512 bf16 12 us of kernels in two launches, 10 in one with 8 workgroups of 64 KB, 5.7 with 32 of 8 KB.
+template <typename T, int VEC, int U, bool SILU, bool MASKED> __global__ void __launch_bounds__(GN_T) vq_gn_one_kernel(const GnArgs a, int span)
+{
+    constexpr int WAVES = GN_T / 64;
+    __shared__ float part[2][WAVES][64 * VEC], chan[2][64 * VEC], count[WAVES];
+    const int t = threadIdx.x, cols = span / VEC, lanes = GN_T / cols, lane = t / cols, cg = a.C / a.G, spans = a.C / span, wave = t >> 6;
+    const int64_t b = blockIdx.x / (unsigned)spans;
+    const int c0 = (int)(blockIdx.x % (unsigned)spans) * span, own = t % cols * VEC, c = c0 + own;
+    const int N = (int)a.N, len = (int)gn_len(a, b);
+    const T *x = (const T *)a.x + b * a.xb + c;
+    const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
+    VqVec<T, VEC> v[U];
+    bool live[U];
+    float n = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = lane + u * lanes, at = r < N ? r : N - 1;
+        v[u] = vq_ldv<T, VEC>(x + (int64_t)at * a.xn);
+        live[u] = r < len && (!MASKED || mask[at]);
+        n += live[u] ? 1.f : 0.f;
+    }
+    float scale[VEC], shift[VEC], mean[VEC];
+    gn_params<VEC>(a.weight, a.wdtype, c, 1.f, scale);
+    gn_params<VEC>(a.bias, a.wdtype, c, 0.f, shift);
+    if (MASKED) {
+        for (int o = cols; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
+        if ((t & 63) == 0) count[wave] = n;
+    } else
+        n = (float)len;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mean[i] = 0.f;
+    float inv = 0.f, unit = 1.f, rstd[VEC];             // unit: 1 / sqrt(count), so that squares sum to the variance, in its range
+    const int parts = cg % VEC == 0 ? 1 : VEC;          // a thread's channels in one group: summed here, in the place of its first
+    if (parts == 1)
+        for (int k = t; k < 2 * span; k += GN_T) (&chan[0][0])[(k >= span) * 64 * VEC + (k >= span ? k - span : k)] = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {              // 0: sums; 1: sums of deviations and of their squares
+        float s[VEC], q[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            s[i] = q[i] = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (live[u]) {
+                    const float d = ((float)v[u].v[i] - mean[i]) * unit;
+                    s[i] += d;
+                    if (pass) q[i] = fmaf(d, d, q[i]);
+                }
+        }
+        if (parts == 1)
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) { s[0] += s[i]; q[0] += q[i]; }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < parts) {
+                for (int o = cols; o < 64; o <<= 1) {
+                    s[i] += __shfl_xor(s[i], o, 64);
+                    q[i] += __shfl_xor(q[i], o, 64);
+                }
+                if ((t & 63) < cols) { part[0][wave][own + i] = s[i]; part[1][wave][own + i] = q[i]; }
+            }
+        __syncthreads();
+        const int step = parts == 1 ? VEC : 1;
+        for (int k = t * step; k < 2 * span; k += GN_T * step) {
+            const int w = k >= span, e = k - w * span;
+            float r = 0.f;
+#pragma unroll
+            for (int l = 0; l < WAVES; ++l) r += part[w][l][e];
+            chan[w][e] = r;
+        }
+        if (!pass) {
+            if (MASKED) {
+                n = 0.f;
+#pragma unroll
+                for (int l = 0; l < WAVES; ++l) n += count[l];
+            }
+            inv = n > 0.f ? 1.f / (n * (float)cg) : 0.f;
+        }
+        __syncthreads();
+        const float back = pass ? unit : inv;
+        unit = sqrtf(inv);
+        GnGroup of(own, cg);
+        float m = 0.f, d = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i, of.next()) {
+            if (i == 0 || of.r == 0) {
+                float r = 0.f;
+                m = 0.f;
+                for (int k = 0; k < cg; k += step) { m += chan[0][of.g * cg + k]; r += chan[1][of.g * cg + k]; }
+                m *= back;
+                d = fmaf(-m, m, r);
+                if (pass) d = 1.f / sqrtf((d > 0.f ? d : d == d ? 0.f : d) + (float)a.eps);
+            }
+            mean[i] += m;
+            rstd[i] = d;
+        }
+    }
+    if (lane == 0) {                                    // the groups that begin among this thread's channels
+        GnGroup of(own, cg);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i, of.next())
+            if (of.r == 0) {
+                a.mean[b * a.G + c0 / cg + of.g] = mean[i];
+                a.rstd[b * a.G + c0 / cg + of.g] = rstd[i];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) scale[i] *= rstd[i];
+    T *y = (T *)a.y + b * a.N * a.C + c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = lane + u * lanes;
+        if (r >= N) break;
+        VqVec<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float z = fmaf((float)v[u].v[i] - mean[i], scale[i], shift[i]);
+            if (SILU) z *= gn_sigmoid(z);
+            o.v[i] = live[u] ? (T)z : (T)0.f;
+        }
+        vq_stv<T, VEC>(y + (int64_t)r * a.C, o);
     }
 }
 
@@ -370,11 +519,11 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
             float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
             gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, w);
             gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, bias);
+            GnGroup of(col * VEC, cg);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int g = (col * VEC + i) / cg;
-                mean[i] = a.mean[b * G + g];
-                rstd[i] = a.rstd[b * G + g];
+            for (int i = 0; i < VEC; ++i, of.next()) {
+                mean[i] = a.mean[b * G + of.g];
+                rstd[i] = a.rstd[b * G + of.g];
             }
             for (int64_t r = r0 + lane; r < r1; r += 4 * sh.lanes) {
                 VqVec<T, VEC> v[4], d[4];
@@ -467,13 +616,13 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
         float mean[VEC], rstd[VEC], w[VEC], bias[VEC], m1[VEC], m2[VEC];
         gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, w);
         gn_params<VEC>(a.bias, a.wdtype, col * VEC, 0.f, bias);
+        GnGroup of(col * VEC, cg);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int g = (col * VEC + i) / cg;
-            mean[i] = a.mean[b * G + g];
-            rstd[i] = a.rstd[b * G + g];
-            m1[i] = stat[g].x;
-            m2[i] = stat[g].y;
+        for (int i = 0; i < VEC; ++i, of.next()) {
+            mean[i] = a.mean[b * G + of.g];
+            rstd[i] = a.rstd[b * G + of.g];
+            m1[i] = stat[of.g].x;
+            m2[i] = stat[of.g].y;
         }
         for (int64_t r = r0 + lane; r < r1; r += 2 * sh.lanes) {
             VqVec<T, VEC> v[2], d[2];
@@ -555,6 +704,44 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     return a;
 }
 
+// the span of vq_gn_one_kernel and its rows a thread; U 0: the slab does not fit.  The widest of up to 128 bytes that leaves a workgroup to
+// every CU, else the narrowest: a small map wants its rows over as many CUs as there are.
+struct GnOne { int span, U; };
+static GnOne gn_one(int64_t B, int64_t N, int C, int G, int elem)
+{
+    const int cg = C / G, vec = 16 / elem;
+    GnOne best{0, 0};
+    if (C % vec || cg > 64 || N > GN_T * 16) return best;
+    for (int k = 1; k <= G; ++k) {
+        const int span = cg * k, cols = span / vec;
+        if (cols > 64 || (best.span && (span * elem > 128 || B * (C / span) < 256))) break;
+        if (G % k || span % vec || cols & (cols - 1)) continue;
+        const int lanes = GN_T / cols, rows = (int)((N + lanes - 1) / lanes);
+        if (rows > 16) break;
+        best = GnOne{span, rows <= 1 ? 1 : rows <= 4 ? 4 : 16};
+    }
+    return best;
+}
+
+template <typename T, int VEC, int U> static void gn_one_launch(const GnArgs &a, int span, hipStream_t st)
+{
+    const dim3 grid((unsigned)(a.B * (a.C / span)));
+    if (a.act == VQHIP_ACT_SILU) {
+        if (a.mask) vq_gn_one_kernel<T, VEC, U, true, true><<<grid, GN_T, 0, st>>>(a, span);
+        else vq_gn_one_kernel<T, VEC, U, true, false><<<grid, GN_T, 0, st>>>(a, span);
+    } else {
+        if (a.mask) vq_gn_one_kernel<T, VEC, U, false, true><<<grid, GN_T, 0, st>>>(a, span);
+        else vq_gn_one_kernel<T, VEC, U, false, false><<<grid, GN_T, 0, st>>>(a, span);
+    }
+}
+template <typename T> static void gn_one_rows(const GnArgs &a, const GnOne &o, hipStream_t st)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    if (o.U == 1) gn_one_launch<T, VEC, 1>(a, o.span, st);
+    else if (o.U == 4) gn_one_launch<T, VEC, 4>(a, o.span, st);
+    else gn_one_launch<T, VEC, 16>(a, o.span, st);
+}
+
 extern "C" size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t C, int64_t groups)
 {
     if (B <= 0 || N <= 0 || C <= 0 || groups <= 0) return 0;
@@ -590,6 +777,13 @@ extern "C" int vqhip_group_norm(const vqhip_group_norm_t *p, void *y, void *stre
     GnArgs a = gn_args(p);
     a.y = y;
     hipStream_t st = (hipStream_t)stream;
+    const GnOne one = gn_one(a.B, a.N, a.C, a.G, vq_elem_bytes(p->dtype));
+    if (one.U) {
+        if (p->dtype == VQHIP_F32) gn_one_rows<float>(a, one, st);
+        else if (p->dtype == VQHIP_BF16) gn_one_rows<__bf16>(a, one, st);
+        else gn_one_rows<_Float16>(a, one, st);
+        return vq_launch_status("vqhip_group_norm");
+    }
     const dim3 grid((unsigned)(a.B * a.S));
     const size_t sm = (size_t)a.G * 8;
     GN_BY_TYPE(p->dtype, a.C, GN_BY_MASK(a.mask, (vq_gn_stats_kernel<T, VEC, MASKED><<<grid, GN_T, 0, st>>>(a))));
