@@ -553,7 +553,8 @@ int vqhip_row_sumsq(const void *x, int x_dtype, int64_t N, int D, int64_t ldx, f
  *   scores   nullable (zeros) [B, J] fp32        mask      nullable [B, J, V] bytes at byte strides mask_stride_b / _j (0: shared)
  *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out: the log-sums, which the backward reads
  *   out_scores / parents / tokens  [B, K]        workspace vqhip_beam_select_workspace_bytes(B, J, V, K) bytes, 16-byte aligned
- * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B * J * ceil(V / 2048) < 2^31 (VQHIP_EDIM beyond).
+ * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B * J * ceil(V / 2048) < 2^24, or B < 2^26 where J * V <= 64
+ * (VQHIP_EDIM beyond).
  * vqhip_beam_select_bwd: the gradients of out_scores (grad [B, K]) with the fields of the forward call, its outputs among them:
  *   d_scores[b, j] (nullable [B, J] fp32) = sum of grad over the kept continuations of beam j,
  *   d_logits (nullable [B, J, V] contiguous, dtype) = sum of grad over those with token v - (normalize) d_scores softmax(logits).
@@ -575,7 +576,7 @@ int vqhip_beam_select_bwd(const vqhip_beam_select_t *step, const float *grad, vo
 /* ---- beam search: the states follow their beams ------------------------------------------------------
  * dst[b, i] = src[b, parents[b, i]] for n <= VQHIP_BEAM_STATES states in one launch (`pick`, the gathers of rvq.py:533-562).  A state's row is
  * `pieces` runs of piece_bytes contiguous bytes, piece_stride bytes apart; rows lie stride_j, batch entries stride_b bytes apart; dst is
- * contiguous [B, K, pieces * piece_bytes] and overlaps no src.  parents [B, K] int64; one outside [0, J) gives a row of zeros.
+ * contiguous [B, K, pieces * piece_bytes] and overlaps no src; less than 2^24 workgroups of 16 KB in all.  parents [B, K] int64; one outside [0, J) gives a row of zeros.
  * vqhip_beam_reorder_bwd: dst[b, j] = sum of src[b, i] over parents[b, i] == j, summed in fp32 by ascending i and rounded once; src
  * (the gradients [B, K, row]) and dst ([B, J, row]) contiguous, element types dtypes[n] F32 / BF16 / F16; the strides are not read. */
 #define VQHIP_BEAM_STATES 32
@@ -596,7 +597,7 @@ int vqhip_beam_reorder_bwd(const vqhip_beam_state_t *states, const int64_t *dtyp
  *   workspace     vqhip_group_norm_workspace_bytes bytes, 16-byte aligned, for either call
  * vqhip_group_norm_bwd: from grad (y's gradient, [B, N, C] contiguous) dx (contiguous, x's dtype), dweight and dbias (param_dtype), each
  * nullable; the sums over rows and batch in 32 bits or more, in an order that depends on the sizes alone.
- * C <= VQHIP_NORM_MAX_C. */
+ * C <= VQHIP_NORM_MAX_C, B <= 2^22, N * C <= 2^39. */
 #define VQHIP_ACT_NONE 0
 #define VQHIP_ACT_SILU 1
 #define VQHIP_NORM_MAX_C 8192

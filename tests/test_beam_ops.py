@@ -339,6 +339,78 @@ def test_reorder_many_states_in_a_graph(dev):
         assert all(torch.equal(o.cpu(), reorder_ref(s, par)) for s, o in zip(states, out))
 
 
+# ---- the residual quantizer's beam search on these operators ---------------------------------------------------------------------------
+def plain_beam_search(rvq, x, beam, mask=None, drop_at=None):
+    """every continuation formed, then the kept ones picked; equal totals by place (stable sort)"""
+    lead, last = x.shape[:-1], len(rvq.layers) - 1 if drop_at is None else drop_at
+    scores = torch.zeros(*lead, 1, device=x.device)
+    residual, out = x[..., None, :], torch.zeros_like(x)[..., None, :]
+    idxs, losses = torch.empty(*lead, 1, 0, dtype=torch.long, device=x.device), torch.empty(*lead, 1, 0, device=x.device)
+    for qi, vq in enumerate(rvq.layers):
+        if qi > last:
+            idxs, losses = torch.nn.functional.pad(idxs, (0, 1), value=-1), torch.nn.functional.pad(losses, (0, 1))
+            continue
+        q, ind, loss = vq(residual, mask=mask, topk=beam)
+        k = ind.shape[-1]
+        scores = (scores[..., None] - loss.detach() * rvq.beam_score_weights[qi]).flatten(-2)
+        step = q.detach() if rvq.quant_grad_frac <= 0 else rvq.quant_grad_frac * q + (1 - rvq.quant_grad_frac) * q.detach()
+        residual = (residual[..., None, :] - step).flatten(-3, -2)
+        out = (out[..., None, :] + q).flatten(-3, -2)
+        idxs = torch.cat((idxs[..., None, :].expand(*idxs.shape[:-1], k, -1), ind[..., None]), -1).flatten(-3, -2)
+        losses = torch.cat((losses[..., None, :].expand(*losses.shape[:-1], k, -1), loss[..., None].float()), -1).flatten(-3, -2)
+        keep = beam if qi != last else 1
+        if scores.shape[-1] > keep:
+            scores, order = scores.sort(dim=-1, descending=True, stable=True)
+            scores, order = scores[..., :keep], order[..., :keep]
+            residual, out = (t.gather(-2, order[..., None].expand(*order.shape, t.shape[-1])) for t in (residual, out))
+            idxs, losses = (t.gather(-2, order[..., None].expand(*order.shape, t.shape[-1])) for t in (idxs, losses))
+    out, idxs, losses = out[..., 0, :], idxs[..., 0, :], losses[..., 0, :]
+    if mask is not None:
+        losses = torch.where(mask[..., None], losses, 0.0).flatten(0, -2).sum(0) / mask.sum().clamp_min(1e-4)
+    else:
+        losses = losses.flatten(0, -2).mean(0)
+    return out, idxs, losses
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw,beam", [(dict(), 2), (dict(quant_grad_frac=0.25), 4), (dict(masked=True), 3), (dict(shared_codebook=True, threshold_ema_dead_code=2), 3),
+                                     (dict(quantize_dropout=True), 4), (dict(beam_score_quantizer_weights=[1.0, 0.5, 0.25, 2.0]), 5), (dict(bf16=True), 4), (dict(), 70)])
+def test_residual_beam_search_matches_plain(dev, kw, beam):
+    """the same values bit for bit; gradients add a beam's continuations in another order: 2^-20 of their size"""
+    import copy
+
+    import vector_quantize_pytorch_amd as A
+    torch.manual_seed(beam)
+    kw = dict(kw)
+    masked, half = kw.pop("masked", False), kw.pop("bf16", False)
+    a = A.ResidualVQ(dim=32, num_quantizers=4, codebook_size=96, beam_size=beam, **kw).cuda().train()
+    b = copy.deepcopy(a)
+    x = torch.randn(1, 90, 32, device="cuda").to(torch.bfloat16 if half else torch.float32)
+    mask = (torch.arange(90, device="cuda") < 61)[None] if masked else None
+    drop = None
+    fw = dict(mask=mask)
+    if kw.get("quantize_dropout"):
+        import random
+        fw["rand_quantize_dropout_fixed_seed"] = 5
+        drop = random.Random(5).randrange(0, 4)
+    xa, xb = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    got, want = a(xa, **fw), plain_beam_search(b, xb, beam, mask, drop)
+    assert got[0].shape == x.shape and got[1].shape == (1, 90, 4) and got[2].shape == (4,)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0], want[0]) and torch.allclose(got[2], want[2], rtol=2.0 ** -20, atol=0.0)
+    w = torch.randn(x.shape, device="cuda").to(x.dtype)
+    ga, = torch.autograd.grad((got[0] * w).float().sum() + got[2].sum(), xa)
+    gb, = torch.autograd.grad((want[0] * w).float().sum() + want[2].sum(), xb)
+    assert (ga - gb).abs().max().item() <= (2.0 ** -5 if half else 2.0 ** -18) * gb.abs().max().item()
+
+
+@pytest.mark.gpu
+def test_residual_beam_search_needs_losses(dev):
+    import vector_quantize_pytorch_amd as A
+    r = A.ResidualVQ(dim=32, num_quantizers=2, codebook_size=32, beam_size=2).cuda()
+    with pytest.raises(RuntimeError, match="commitment loss"):
+        r.eval()(torch.randn(1, 8, 32, device="cuda"))
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A

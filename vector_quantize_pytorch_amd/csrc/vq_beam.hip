@@ -429,6 +429,9 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
     if (t == 0 && n < K) sel_fill(a, b, n);
 }
 
+#define SEL_MOST_SMALL ((1 << 26) - 1)
+#define SEL_MOST_TILES ((1 << 24) - 1)
+
 // tiles of the rows: one wave for rows of up to 512 logits; 8192 logits a workgroup where that gives each CU two, else 2048
 struct SelPlan { int small, threads, per_thread, tiles; };
 static SelPlan sel_plan(int64_t B, int64_t J, int64_t V)
@@ -456,8 +459,10 @@ static int sel_check(const vqhip_beam_select_t *p, const char *what)
     if (!p) VQ_FAIL(VQHIP_EINVAL, "%s: null argument", what);
     if (!vq_elem_bytes(p->dtype)) VQ_FAIL(VQHIP_EINVAL, "%s: dtype %lld", what, (long long)p->dtype);
     if (p->B < 0 || p->J < 1 || p->V < 1 || p->K < 1) VQ_FAIL(VQHIP_EINVAL, "%s: B %lld, J %lld, V %lld, K %lld", what, (long long)p->B, (long long)p->J, (long long)p->V, (long long)p->K);
-    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->V > (1 << 30) / p->J || p->K > p->J * p->V || p->B > 0x7fffffff / p->J / ((p->V + 2047) / 2048))
-        VQ_FAIL(VQHIP_EDIM, "%s: %lld entries, %lld kept of %lld x %lld continuations: at most %d beams, %d kept, 2^30 continuations an entry, 2^31 tiles in all",
+    // (a launch takes fewer than 2^32 threads: 256 a row of a tile, 64 an entry of up to 64 continuations)
+    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->V > (1 << 30) / p->J || p->K > p->J * p->V ||
+        p->B > (p->J * p->V <= 64 ? SEL_MOST_SMALL : SEL_MOST_TILES / p->J / ((p->V + 2047) / 2048)))
+        VQ_FAIL(VQHIP_EDIM, "%s: %lld entries, %lld kept of %lld x %lld continuations: at most %d beams, %d kept, 2^30 continuations an entry, 2^24 tiles in all",
                 what, (long long)p->B, (long long)p->K, (long long)p->J, (long long)p->V, VQHIP_BEAM_MAX, VQHIP_BEAM_MAX);
     if (p->finished && (p->end_token < 0 || p->end_token >= p->V)) VQ_FAIL(VQHIP_EINVAL, "%s: end token %lld outside [0, %lld)", what, (long long)p->end_token, (long long)p->V);
     if (p->B > 0 && (!p->logits || !p->parents || !p->tokens || !p->out_scores)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
@@ -538,7 +543,7 @@ template <typename T, bool MASKED> __global__ void __launch_bounds__(256) vq_bea
             g[at] = gk;
             tok[at] = tk;
         }
-        const float onto = vq_wave_sum(gk);
+        const float onto = (float)vq_wave_sum((double)gk);     // (64 bits: the gradients of a beam's survivors may cancel)
         const bool any = __ballot(mine) != 0;
         if (t == 0) {
             if (a.d_scores && tile == 0) a.d_scores[row] = onto;
@@ -610,6 +615,7 @@ extern "C" int vqhip_beam_select_bwd(const vqhip_beam_select_t *p, const float *
     a.d_logits = d_logits; a.d_scores = d_scores;
     a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.normalize = p->normalize != 0;
     a.tiles = d_logits ? (a.V + SEL_BWD - 1) / SEL_BWD : 1;
+    if (a.B > SEL_MOST_TILES / a.J / a.tiles) VQ_FAIL(VQHIP_EDIM, "vqhip_beam_select_bwd: %lld x %d rows", (long long)a.B, a.J);
     hipStream_t st = (hipStream_t)stream;
     if (p->dtype == VQHIP_F32) sel_bwd<float>(a, st);
     else if (p->dtype == VQHIP_BF16) sel_bwd<__bf16>(a, st);
@@ -760,12 +766,12 @@ static int reorder_check(int64_t n, const void *states, const int64_t *parents, 
     return 0;
 }
 
-// workgroups of `rows` rows of per_row units; a launch takes fewer than 2^31
+// workgroups of `rows` rows of per_row units; a launch takes fewer than 2^32 threads
 static int reorder_blocks(int64_t rows, int64_t per_row, unsigned *first, unsigned *total, const char *what)
 {
     if (per_row > 0x40000000 || rows > (((int64_t)1 << 62) / per_row)) VQ_FAIL(VQHIP_EDIM, "%s: rows of %lld units", what, (long long)per_row);
     const int64_t blocks = (rows * per_row + REO_UNITS - 1) / REO_UNITS;
-    if (blocks > 0x7fffffff - (int64_t)*total) VQ_FAIL(VQHIP_EDIM, "%s: too many bytes", what);
+    if (blocks > ((1 << 24) - 1) - (int64_t)*total) VQ_FAIL(VQHIP_EDIM, "%s: too many bytes", what);
     *first = *total;
     *total += (unsigned)blocks;
     return 0;

@@ -171,7 +171,7 @@ extern "C" int vqhip_clip_grads(const vqhip_grad_t *grads, int64_t count, double
     }
     int chunk;
     const int64_t blocks = grad_blocks(grads, count, &chunk);
-    if (blocks > 0x7fffffff) VQ_FAIL(VQHIP_EDIM, "vqhip_clip_grads: too many elements");
+    if (blocks >= 1 << 24) VQ_FAIL(VQHIP_EDIM, "vqhip_clip_grads: too many elements");              // (2^32 threads)
     if (workspace_bytes < (size_t)blocks * 8 + 16) VQ_FAIL(VQHIP_EINVAL, "vqhip_clip_grads: workspace of %zu bytes", workspace_bytes);
     if ((uintptr_t)workspace & 15) VQ_FAIL(VQHIP_EALIGN, "vqhip_clip_grads: workspace not 16-byte aligned");
     const int apart = count > 0 ? grad_apart(grads, count) : 1;

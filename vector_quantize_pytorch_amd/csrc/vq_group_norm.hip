@@ -711,7 +711,7 @@ static GnOne gn_one(int64_t B, int64_t N, int C, int G, int elem)
 {
     const int cg = C / G, vec = 16 / elem;
     GnOne best{0, 0};
-    if (C % vec || cg > 64 || N > GN_T * 16) return best;
+    if (C % vec || cg > 64 || N > GN_T * 16 || B > (1 << 22) / G) return best;          // (a launch takes fewer than 2^32 threads)
     for (int k = 1; k <= G; ++k) {
         const int span = cg * k, cols = span / vec;
         if (cols > 64 || (best.span && (span * elem > 128 || B * (C / span) < 256))) break;
