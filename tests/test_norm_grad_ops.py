@@ -61,7 +61,7 @@ def check_forward(y, want, dtype, xmax, rmax):
 
 
 NORMS = [(1, 1, 1, 1), (2, 1, 64, 2), (1, 7, 6, 3), (3, 16, 32, 32), (2, 49, 96, 8), (2, 256, 512, 32), (1, 1000, 128, 32), (5, 33, 40, 1),
-         (2, 4099, 24, 4), (1, 20000, 64, 16), (3, 301, 1025, 5), (1, 5, 8192, 64), (2, 300, 8192, 8192), (1, 70000, 8, 2), (70, 9, 16, 4), (2, 2048, 257, 257)]
+         (2, 4099, 24, 4), (1, 20000, 64, 16), (3, 301, 1025, 5), (1, 5, 8192, 64), (2, 300, 8192, 8192), (1, 70000, 8, 2), (70, 9, 16, 4), (2, 2048, 257, 257), (2, 16384, 128, 32)]
 
 
 @pytest.mark.gpu
@@ -80,7 +80,7 @@ def test_norm(dev, b, n, c, groups, act, dtype, wtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("act", [None, "silu"])
-@pytest.mark.parametrize("b,n,c,groups", [(1, 16, 8, 2), (3, 49, 96, 8), (2, 256, 512, 32), (1, 4099, 24, 4), (2, 20000, 16, 4), (3, 301, 1025, 5), (40, 130, 64, 8), (1, 300, 8192, 8192), (600, 3, 32, 1)])
+@pytest.mark.parametrize("b,n,c,groups", [(1, 16, 8, 2), (3, 49, 96, 8), (2, 256, 512, 32), (1, 4099, 24, 4), (2, 20000, 16, 4), (3, 301, 1025, 5), (40, 130, 64, 8), (1, 300, 8192, 8192), (600, 3, 32, 1), (2, 16384, 128, 32)])
 def test_norm_gradient(dev, b, n, c, groups, act, dtype):
     """dx: rstd times three terms of at most |dz w| + mean + |xh| mean, each with 16 half steps of 2^-24 and the error of xh (2^-21 of
     1 + |x| rstd), rounded once; dw, db: n b terms, each with that error, summed in 32 bits or more (a pairwise or blocked sum: at most

@@ -5,7 +5,7 @@
 // leave out are neither read into the statistics nor normalised: their output is zero, whatever they hold.
 //
 // Two launches each way, both over (batch entry, chunk of rows): the first leaves each chunk's statistics (backward: its sums), the
-// second joins them -- in every workgroup, S * G pairs from cache; beyond GN_JOIN chunks in a small launch between -- and writes the rows.  Bound by HBM, with the second read of x from
+// second joins them -- in every workgroup, S * G pairs from cache; beyond GN_JOIN in a small launch between -- and writes the rows.  Bound by HBM, with the second read of x from
 // the memory-side cache where it fits.  A thread keeps VEC channels of every row it visits (16 bytes where C divides so), so parameters and
 // statistics stay in registers and rows of any stride are read in whole lines.  All sums have one order: no atomics.
 #include "vq_elem.h"
@@ -14,7 +14,10 @@
 
 #define GN_T 512                   // threads of a workgroup
 #define GN_FLUSH 32                // rows that a thread sums about one pivot
-#define GN_JOIN 48                 // chunks that every workgroup of the second launch joins for itself; more are joined in a launch between
+// pairs (chunks x groups) of a batch row that every workgroup of the second launch joins for itself; more are joined in a launch between.
+// Apply kernel against join and apply: 64 x 8 9.5 and 3.9 + 8.2 us, 128 x 32 26.9 and 4.0 + 22.5, 170 x 32 36.2 and 4.6 + 32.4, 256 x 32 19.7 and
+// 3.8 + 11.4; a launch more costs its 3 us of host besides.
+#define GN_JOIN 6144
 
 struct GnArgs {
     const void *x; int64_t xb, xn;                      // element strides of batch and row
@@ -700,12 +703,12 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     a.stream = p->B * p->N * p->C * vq_elem_bytes(p->dtype) > (64 << 20);
     a.S = (int)S; a.rows = rows; a.eps = p->eps;
     a.pair = (float2 *)p->workspace; a.joined = a.pair + p->B * S * p->groups; a.chan = (float *)(a.joined + p->B * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
-    if (S <= GN_JOIN) a.joined = nullptr;
+    if (S * p->groups <= GN_JOIN) a.joined = nullptr;
     return a;
 }
 
 // the span of vq_gn_one_kernel and its rows a thread; U 0: the slab does not fit.  The widest of up to 128 bytes that leaves a workgroup to
-// every CU, else the narrowest: a small map wants its rows over as many CUs as there are.
+// every CU, else the narrowest: a small map wants its rows over as many CUs as there are.  16 x 1024 x 256 fp32: 14.5 us, 7.0 + 8.8 in two launches.
 struct GnOne { int span, U; };
 static GnOne gn_one(int64_t B, int64_t N, int C, int G, int elem)
 {
