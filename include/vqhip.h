@@ -553,8 +553,8 @@ int vqhip_row_sumsq(const void *x, int x_dtype, int64_t N, int D, int64_t ldx, f
  *   scores   nullable (zeros) [B, J] fp32        mask      nullable [B, J, V] bytes at byte strides mask_stride_b / _j (0: shared)
  *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out: the log-sums, which the backward reads
  *   out_scores / parents / tokens  [B, K]        workspace vqhip_beam_select_workspace_bytes(B, J, V, K) bytes, 16-byte aligned
- * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B * J * ceil(V / 2048) < 2^24, or B < 2^26 where J * V <= 64
- * (VQHIP_EDIM beyond).
+ * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B * J * ceil(V / 2048) < 2^24, or B < 2^26 where J * V <= 64; the
+ * backward B * J * ceil(V / 4096) < 2^24 (VQHIP_EDIM beyond).
  * vqhip_beam_select_bwd: the gradients of out_scores (grad [B, K]) with the fields of the forward call, its outputs among them:
  *   d_scores[b, j] (nullable [B, J] fp32) = sum of grad over the kept continuations of beam j,
  *   d_logits (nullable [B, J, V] contiguous, dtype) = sum of grad over those with token v - (normalize) d_scores softmax(logits).
@@ -615,7 +615,7 @@ int vqhip_group_norm_bwd(const vqhip_group_norm_t *norm, const void *grad, void 
 /* ---- the global norm of many gradients, and clipping ---------------------------------------------------
  * norm[0] = sqrt(sum of squares over all `count` tensors), squares and sums in 64 bits; dst = src * min(1, max_norm / (norm + eps)) for
  * every tensor with a dst (src itself, or memory that overlaps no tensor of the call).  A norm that is not finite goes through: the
- * factor is 0 for an infinite one, NaN for NaN.  `grads` is host memory, read during the call; src and dst are device pointers to n
+ * factor is 0 for an infinite one (1 if max_norm is infinite too), NaN for NaN.  `grads` is host memory, read during the call; src and dst are device pointers to n
  * contiguous elements of dtype F32 / BF16 / F16.  No tensor occurs twice (VQHIP_EINVAL, as for overlaps).  workspace: vqhip_clip_grads_workspace_bytes bytes, 16-byte
  * aligned.  No host read: capturable. */
 typedef struct { const void *src; void *dst; int64_t n; int64_t dtype; } vqhip_grad_t;

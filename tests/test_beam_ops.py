@@ -63,6 +63,44 @@ def test_select(dev, b, j, v, k, normalize, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("b,j,v,k", [(4, 4, 5, 7), (3, 5, 40, 9), (2, 6, 1000, 6), (2, 3, 9000, 64), (1, 4, 70001, 5), (70, 8, 9000, 8)])
+@pytest.mark.parametrize("kind", ["lowest", "infinite", "one", "first", "finished", "masked"])
+def test_select_scores_that_hide_logits(dev, b, j, v, k, kind, dtype):
+    """scores beside which 64 bits do not see the logits: all continuations of such a beam are equal, and their places decide.  one: only
+    the last beam has such a score; first: the first beam has an ordinary one; finished: it has ended, one continuation is left to it"""
+    import vector_quantize_pytorch_amd as A
+    lg, sc = make(b, j, v, dtype, seed=3)
+    low = torch.finfo(torch.float32).min
+    finished = mask = None
+    if kind == "one":
+        sc[:, -1] = 1e30
+    else:
+        sc[:, 0 if kind in ("lowest", "infinite", "masked") else 1:] = float("inf") if kind == "infinite" else low
+    if kind == "finished":
+        finished = torch.zeros(b, j, dtype=torch.bool, device="cuda")
+        finished[:, 0] = True
+        finished[0, -1] = True
+    if kind == "masked":
+        mask = torch.rand(b, j, v, generator=torch.Generator().manual_seed(4)).cuda() < 0.1
+    for normalize in (True, False):
+        step = A.beam_select(lg, sc, k, mask=mask, finished=finished, end_token=None if finished is None else v // 2, normalize=normalize)
+        check_select(step, select_ref(lg, sc, k, mask=mask, finished=finished, end=v // 2, normalize=normalize))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,k", [(300, 5), (2500, 40), (40000, 8)])
+def test_select_logits_that_scores_hide(dev, v, k):
+    """logits around 0 that differ by 2^-80: beside a score of -1 they are equal, beside a score of 0 they are not"""
+    import vector_quantize_pytorch_amd as A
+    g = torch.Generator().manual_seed(v)
+    lg = (torch.randn(2, 3, v, generator=g) * 2.0 ** -80).cuda()
+    lg[0, 2, v - 3] = 1.0
+    for sc in (torch.full((2, 3), -1.0), torch.tensor([[0.0, -1.0, -1.0], [-1.0, 0.0, 0.0]]), torch.tensor([[0.0, -1.0, -2.0], [-1.0, 2.0 ** -81, 0.0]])):
+        check_select(A.beam_select(lg, sc.cuda(), k, normalize=False), select_ref(lg, sc, k, normalize=False))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("b,j,v,k", [(3, 4, 4, 5), (2, 5, 1000, 6), (2, 3, 40009, 9)])
 @pytest.mark.parametrize("kind", ["row", "shared", "each", "beam", "nothing"])
 def test_select_masked(dev, b, j, v, k, kind):
@@ -432,7 +470,8 @@ def test_select_refusals():
             ("survivors", lambda: A.beam_select(lg, sc, 31)),
             ("survivors", lambda: A.beam_select(torch.zeros(1, 1, 1000), None, 65)),
             ("survivors", lambda: A.beam_select(torch.zeros(1, 65, 10), None, 4)),
-            ("survivors", lambda: A.beam_select(torch.zeros(1, 2, 0), None, 1))]:
+            ("survivors", lambda: A.beam_select(torch.zeros(1, 2, 0), None, 1)),
+            ("its gradient takes", lambda: A.beam_select(torch.zeros(1).expand(1 << 22, 4, 4).requires_grad_(), None, 1))]:
         with pytest.raises(VQHipError, match=match):
             call()
 

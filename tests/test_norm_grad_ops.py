@@ -283,6 +283,10 @@ def test_clip_extremes(dev):
     assert norm.item() == float("inf") and out[1].item() == 0.0 and out[0].isnan()
     outs, norm = A.clip_grads([torch.tensor([float("nan")], device="cuda"), g], 1.0)
     assert norm.isnan() and outs[1].isnan().all()
+    (out,), norm = A.clip_grads([g], float("inf"))                         # max_norm inf: the norm alone
+    assert torch.equal(out, g) and abs(norm.item() - 10 ** 0.5) < 1e-6
+    (out,), norm = A.clip_grads([torch.tensor([float("inf"), 2.0], device="cuda")], float("inf"))
+    assert norm.item() == float("inf") and out.tolist() == [float("inf"), 2.0]
     assert A.clip_grads([], 1.0)[0] == []
     zero = [torch.zeros(5, device="cuda")]
     assert A.clip_grads(zero, 1.0)[1].item() == 0.0 and (A.clip_grads(zero, 1.0)[0][0] == 0).all()

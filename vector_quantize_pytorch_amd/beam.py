@@ -140,17 +140,20 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     if j < 1 or v < 1 or j > BEAM_MAX or not 1 <= beam_size <= min(BEAM_MAX, j * v):
         raise L.VQHipError(f"beam_select: {beam_size} survivors of {j} x {v} continuations: takes 1 to {BEAM_MAX} beams and survivors, "
                            "no more survivors than continuations")
-    L._need_gpu(logits, scores, mask, finished)
-    beam_size = int(beam_size)
     n = 1
     for d in lead:
         n *= d
+    grad = torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad))
+    if grad and n * j * (-(-v // 4096)) >= 1 << 24:
+        raise L.VQHipError(f"beam_select: {n} x {j} x {v} continuations are more than its gradient takes (2^24 tiles of 4096)")
+    L._need_gpu(logits, scores, mask, finished)
+    beam_size = int(beam_size)
     lg = _table(logits, n, j, v)
     sc = scores if scores is None or (len(lead) == 1 and scores.is_contiguous()) else scores.reshape(n, j).contiguous()
     mk = None if mask is None else _table(mask, n, j, v).view(torch.uint8)
     fin = None if finished is None else finished.reshape(n, j).contiguous().view(torch.uint8)
     end = 0 if finished is None else int(end_token)
-    if torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad)):
+    if grad:
         out, parents, tokens = _SelectFn.apply(lg, sc, mk, fin, beam_size, end, bool(normalize))
     else:
         out, parents, tokens, _ = _select(lg, sc, mk, fin, beam_size, end, bool(normalize), False)

@@ -9,11 +9,13 @@
 // the mask leaves out, and every sum that is not a number, is -inf.  Out: the K largest c of a batch entry, equal ones by ascending
 // j * V + v.  Sums and comparisons are 64-bit: two continuations of different beams may be closer than fp32 resolves.
 //
-// Within a row c grows with l, so the K best of a row are the K largest l.  Two launches: vq_beam_rows_kernel reads every logit once
-// (its tile stays in registers), and leaves of each tile the log-sum's maximum and sum and its K largest logits; vq_beam_merge_kernel
-// joins the tiles of a batch entry's rows.  Bound by the read of the logits.  vq_beam_small_kernel does small entries in one launch.
+// Within a row c grows with l, so the K best of a row are the K largest l (where 64 bits tell their c apart, see sel_places).  Two
+// launches: vq_beam_rows_kernel reads every logit once (its tile stays in registers), and leaves of each tile the log-sum's maximum and
+// sum and its K largest logits; vq_beam_merge_kernel joins the tiles of a batch entry's rows.  Bound by the read of the logits.
+// vq_beam_small_kernel does small entries in one launch.
 struct SelArgs {
     const void *logits; int64_t lb, lj;                 // element strides of batch and beam
+    int dtype;
     const float *scores;                                // [B, J] or null (zeros)
     const uint8_t *mask; int64_t mb, mj;                // byte strides; null: everything admitted
     const uint8_t *finished;                            // [B, J] or null
@@ -295,6 +297,43 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
     }
 }
 
+// The lists hold a tile's K largest logits, yet under a score of -1e30, or around a logit of 1e-20, different logits have one and the same c,
+// and the places decide.  Where the cut between the survivors and the rest goes through such a c (one step of a logit further down it is
+// still the same), the survivors at the cut are the first places that have it, found by going through the entry's logits again.  `at`: the
+// survivors above the cut.  The test for it costs a merge 0.7 us.
+__device__ void sel_places(const SelArgs &a, int64_t b, double cut, int at, const double *base, const double *log_sum, const uint8_t *fin, int *wave_cnt)
+{
+    const int t = threadIdx.x, V = a.V;
+    for (int j = 0; j < a.J && at < a.K; ++j) {
+        if (!(base[j] > -INFINITY)) continue;
+        for (int v0 = fin[j] ? a.end_token / 256 * 256 : 0; v0 < V && at < a.K; v0 += 256) {
+            const int v = v0 + t;
+            bool hit = false;
+            if (fin[j]) hit = v == a.end_token && sel_sum(base[j], 0.0) == cut;
+            else if (v < V && (!a.mask || a.mask[b * a.mb + j * a.mj + v])) {
+                const int64_t i = b * a.lb + j * a.lj + v;
+                const float l = a.dtype == VQHIP_F32 ? ((const float *)a.logits)[i] : a.dtype == VQHIP_BF16 ? (float)((const __bf16 *)a.logits)[i] : (float)((const _Float16 *)a.logits)[i];
+                hit = sel_sum(base[j], (double)l - log_sum[j]) == cut;
+            }
+            const unsigned long long hits = __ballot(hit);
+            __syncthreads();
+            if ((t & 63) == 0) wave_cnt[t >> 6] = __popcll(hits);
+            __syncthreads();
+            int rank = at + __popcll(hits & ((1ull << (t & 63)) - 1));
+            for (int w = 0; w < 4; ++w) {
+                if (w < t >> 6) rank += wave_cnt[w];
+                at += wave_cnt[w];
+            }
+            if (hit && rank < a.K) {
+                a.scores_out[b * a.K + rank] = (float)cut;
+                a.parents_out[b * a.K + rank] = j;
+                a.tokens_out[b * a.K + rank] = v;
+            }
+            if (fin[j]) break;
+        }
+    }
+}
+
 // ---- merge: one workgroup per batch entry -------------------------------------------------------------------------------------------
 // The rows' log-sums from their tiles (16 lanes a row), then the K best of J * tiles * K (and the finished beams') by the same bound and
 // ranks in 64 bits; where ties let more than SEL_CAP through, K rounds that each find the next one.  Bound by latency: the first
@@ -303,8 +342,9 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
 __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
 {
     __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
-    __shared__ float group_max[64];
+    __shared__ float group_max[64], ls[SEL_CAP];
     __shared__ int ps[SEL_CAP], found;
+    __shared__ double cut_s;
     __shared__ uint8_t fin[VQHIP_BEAM_MAX];
     __shared__ double rc[4];
     __shared__ int rp[4];
@@ -368,20 +408,24 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
     if ((t & 3) == 0) group_max[t >> 2] = low;
     __syncthreads();
     const double bound = (double)sel_kth(group_max[t & 63], K);
-    auto offer = [&](double c, int p) {
+    auto offer = [&](double c, int p, int logit) {
         if (c >= bound && c > -INFINITY) {
             const int k = atomicAdd(&found, 1);
-            if (k < SEL_CAP) { cs[k] = c; ps[k] = p; }
+            if (k < SEL_CAP) { cs[k] = c; ps[k] = p; ls[k] = __int_as_float(logit); }
         }
     };
 #pragma unroll
-    for (int h = 0; h < SEL_HELD; ++h) offer(c_held[h], p_held[h]);
+    for (int h = 0; h < SEL_HELD; ++h) offer(c_held[h], p_held[h], held[h].x);
     for (int i = SEL_HELD * 256 + t; i < total; i += 256) {
-        const double c = value(i, lists[i], place);
-        offer(c, place);
+        const int2 q = lists[i];
+        const double c = value(i, q, place);
+        offer(c, place, q.x);
     }
     __syncthreads();
-    int n = found;
+    // whether a logit below l, which no list may hold, has l's c (the cut's) too
+    auto more = [&](int j, float l) { return !fin[j] && sel_sum(base[j], (double)nextafterf(l, -INFINITY) - log_sum[j]) == cut_s; };
+    bool open = false;
+    int n = found, above = 0;
     if (n <= SEL_CAP) {
         for (int i = t; i < n; i += 256) {
             const double c = cs[i];
@@ -394,8 +438,16 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
                 a.parents_out[b * K + rank] = p / a.V;
                 a.tokens_out[b * K + rank] = p % a.V;
             }
+            if (rank == K - 1) cut_s = c;
         }
-        n = n < K ? n : K;
+        __syncthreads();
+        if (n >= K) {
+            for (int i = t; i < n; i += 256) open |= cs[i] == cut_s && more(ps[i] / a.V, ls[i]);
+            open = __syncthreads_or(open);
+            if (open)
+                for (int k = 0; k < n; ++k) above += cs[k] > cut_s ? 1 : 0;
+            n = K;
+        }
     } else {
         double last = INFINITY;
         int lastp = -1;
@@ -417,16 +469,26 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
                 if (sel_before(rc[w], rp[w], c, p)) { c = rc[w]; p = rp[w]; }
             __syncthreads();
             if (!(c > -INFINITY)) break;
+            if (c < last) above = n;
             last = c; lastp = p;
             if (t == 0) {
+                cut_s = c;
                 a.scores_out[b * K + n] = (float)c;
                 a.parents_out[b * K + n] = p / a.V;
                 a.tokens_out[b * K + n] = p % a.V;
             }
         }
+        __syncthreads();
+        if (n == K)
+            for (int i = t; i < total; i += 256) {
+                const int2 q = lists[i];
+                open |= value(i, q, place) == cut_s && more(i / per, __int_as_float(q.x));
+            }
+        open = __syncthreads_or(open);
     }
     __syncthreads();
-    if (t == 0 && n < K) sel_fill(a, b, n);
+    if (open) sel_places(a, b, cut_s, above, base, log_sum, fin, rp);
+    else if (t == 0 && n < K) sel_fill(a, b, n);
 }
 
 #define SEL_MOST_SMALL ((1 << 26) - 1)
@@ -485,7 +547,7 @@ extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
     if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select: workspace of %zu bytes, needs %zu", p->workspace_bytes, need);
     if ((uintptr_t)p->workspace & 15) VQ_FAIL(VQHIP_EALIGN, "vqhip_beam_select: workspace not 16-byte aligned");
     SelArgs a;
-    a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.scores = p->scores;
+    a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.dtype = (int)p->dtype; a.scores = p->scores;
     a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j; a.finished = p->finished;
     a.scores_out = p->out_scores; a.parents_out = p->parents; a.tokens_out = p->tokens; a.lse_out = p->lse;
     a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.end_token = (int)p->end_token; a.normalize = p->normalize != 0;

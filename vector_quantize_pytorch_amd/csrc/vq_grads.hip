@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(1024) vq_grad_coef_kernel(const double *partia
     }
     s = sqrt(grad_block_sum(s));
     if (threadIdx.x == 0) {
-        const double c = max_norm / (s + eps);
+        const double c = max_norm == INFINITY && s == INFINITY ? 1.0 : max_norm / (s + eps);
         norm[0] = (float)s;
         coef[0] = c > 1.0 ? 1.f : (float)c;             // (a norm that is not a number: neither comparison holds, NaN goes through)
     }

@@ -703,7 +703,7 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     a.stream = p->B * p->N * p->C * vq_elem_bytes(p->dtype) > (64 << 20);
     a.S = (int)S; a.rows = rows; a.eps = p->eps;
     a.pair = (float2 *)p->workspace; a.joined = a.pair + p->B * S * p->groups; a.chan = (float *)(a.joined + p->B * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
-    if (S * p->groups <= GN_JOIN) a.joined = nullptr;
+    if (S == 1 || S * p->groups <= GN_JOIN) a.joined = nullptr;           // (more chunks than one: B <= 256)
     return a;
 }
 

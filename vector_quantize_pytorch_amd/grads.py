@@ -51,7 +51,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
 
     grads: contiguous float32 / bfloat16 / float16 tensors of one device; out: contiguous tensors of the same types and numbers of
     elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that
-    is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  No gradient passes through."""
+    is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  max_norm inf: the norm alone
+    (nothing is scaled unless it is NaN).  No gradient passes through."""
     grads = list(grads)
     if not max_norm >= 0.0:
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")
@@ -73,7 +74,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     return out, norm
 
 
-def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
+def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, *, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Clips the gradients of `parameters` in place to a global 2-norm of max_norm and returns the norm before (0-dim float32, on the
     device; nothing is read back unless error_if_nonfinite asks).  Parameters without a gradient are passed over; a gradient that is not
     contiguous is clipped through a contiguous copy."""
