@@ -28,20 +28,36 @@ def _clip(first, table, max_norm):
     return norm
 
 
-def _table(grads, out):
-    """the checked rows of vqhip_grad_t; out None: the norm alone"""
-    codes, dev, flat = L._ELEM_CODES, grads[0].get_device(), []
-    for g, o in zip(grads, out if out is not None else grads):          # (one pass: a model has hundreds)
-        dt, n = g.dtype, g.numel()
-        if dt not in codes:
-            L._elem_code(g, "clip_grads")
+def _check(grads, out):
+    """raises what is wrong with a tensor or its result, if anything is"""
+    dev = grads[0].get_device()
+    for g, o in zip(grads, out):
+        L._elem_code(g, "clip_grads")
         if not g.is_contiguous():
             raise L.VQHipError(f"clip_grads: tensor {tuple(g.shape)} with strides {g.stride()}, expected a contiguous one")
         if g.get_device() != dev:
             raise L.VQHipError(f"clip_grads: tensors on different devices ({grads[0].device} and {g.device})")
-        if o is not g and (o.numel() != n or o.dtype != dt or not o.is_contiguous() or o.get_device() != dev):
-            raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {n} contiguous elements of {dt} on {g.device}")
-        flat += (g.data_ptr(), o.data_ptr() if out is not None else 0, n, codes[dt])
+        if o.numel() != g.numel() or o.dtype != g.dtype or not o.is_contiguous() or o.get_device() != dev:
+            raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {g.numel()} contiguous elements of {g.dtype} on {g.device}")
+
+
+def _table(grads, out):
+    """the checked rows of vqhip_grad_t; out None: the norm alone.  A pass over all tensors for each property: a model has hundreds, and
+    `map` takes two thirds of the time of a loop over them (311 tensors with results of their own: a call 205 us instead of 250)"""
+    T, codes = torch.Tensor, L._ELEM_CODES
+    dtypes, sizes = [t.dtype for t in grads], list(map(T.numel, grads))
+    fine = all(map(T.is_contiguous, grads)) and len(set(map(T.get_device, grads))) == 1 and all(map(codes.__contains__, set(dtypes)))
+    if out is not None and out is not grads:
+        fine = fine and sizes == list(map(T.numel, out)) and dtypes == [t.dtype for t in out] and all(map(T.is_contiguous, out)) \
+            and set(map(T.get_device, out)) == {grads[0].get_device()}
+    if not fine:
+        _check(grads, grads if out is None else out)
+    flat = [0] * (4 * len(grads))
+    flat[::4] = map(T.data_ptr, grads)
+    if out is not None:
+        flat[1::4] = map(T.data_ptr, out)
+    flat[2::4] = sizes
+    flat[3::4] = [codes[d] for d in dtypes]
     return array.array("q", flat)
 
 
