@@ -69,7 +69,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that
     is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  max_norm inf: the norm alone
     (nothing is scaled unless it is NaN).  No gradient passes through."""
-    grads = list(grads)
+    given, grads = grads, list(grads)
     if not max_norm >= 0.0:
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")
     if not grads:
@@ -80,7 +80,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
         out = [torch.empty_like(g) for g in grads]
         table[1::4] = array.array("q", [o.data_ptr() for o in out])
     else:
-        out = list(out)
+        out = grads if out is given else list(out)
         if len(out) != len(grads):
             raise L.VQHipError(f"clip_grads: {len(out)} results for {len(grads)} tensors")
         table = _table(grads, out)
