@@ -49,7 +49,8 @@ def make(b, j, v, dtype, seed=0, spread=2.0):
 
 SIZES = [(1, 1, 1, 1), (3, 1, 7, 7), (5, 4, 4, 4), (2, 3, 1, 2), (2, 8, 8, 64), (1, 64, 3, 5), (4, 7, 33, 13), (3, 5, 257, 5), (2, 2, 1024, 64),
          (2, 6, 1023, 6), (1, 3, 2049, 8), (2, 3, 5001, 16), (1, 2, 32003, 33), (1, 1, 100001, 4), (1, 4, 131072, 8), (67, 4, 4, 4), (300, 2, 65, 3),
-         (1030, 1, 130, 2), (2, 64, 64, 64)]
+         (1030, 1, 130, 2), (2, 64, 64, 64), (9, 16, 16, 16), (5, 13, 19, 13), (300, 1, 65, 64), (3, 9, 57, 20), (7, 32, 32, 32), (2, 33, 47, 40), (2, 64, 32, 64),
+         (3, 4, 1024, 64), (2, 5, 819, 7), (2, 64, 65, 64), (1, 64, 700, 64), (1, 40, 5000, 64)]
 
 
 @pytest.mark.gpu
@@ -64,7 +65,7 @@ def test_select(dev, b, j, v, k, normalize, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("b,j,v,k", [(4, 4, 5, 7), (3, 5, 40, 9), (2, 6, 1000, 6), (2, 3, 9000, 64), (1, 4, 70001, 5), (70, 8, 9000, 8)])
+@pytest.mark.parametrize("b,j,v,k", [(4, 4, 5, 7), (3, 5, 40, 9), (3, 9, 90, 12), (3, 8, 500, 33), (2, 6, 1000, 6), (2, 3, 9000, 64), (1, 4, 70001, 5), (70, 8, 9000, 8)])
 @pytest.mark.parametrize("kind", ["lowest", "infinite", "one", "first", "finished", "masked"])
 def test_select_scores_that_hide_logits(dev, b, j, v, k, kind, dtype):
     """scores beside which 64 bits do not see the logits: all continuations of such a beam are equal, and their places decide.  one: only
@@ -101,7 +102,7 @@ def test_select_logits_that_scores_hide(dev, v, k):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("b,j,v,k", [(3, 4, 4, 5), (2, 5, 1000, 6), (2, 3, 40009, 9)])
+@pytest.mark.parametrize("b,j,v,k", [(3, 4, 4, 5), (2, 5, 1000, 6), (2, 3, 40009, 9), (3, 5, 50, 6), (4, 5, 100, 6), (2, 7, 250, 20), (2, 5, 800, 9)])
 @pytest.mark.parametrize("kind", ["row", "shared", "each", "beam", "nothing"])
 def test_select_masked(dev, b, j, v, k, kind):
     """what the mask leaves out holds NaN and infinities; `nothing`: one beam, and one whole entry, have no continuation"""
@@ -123,7 +124,7 @@ def test_select_masked(dev, b, j, v, k, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("v", [5, 700, 33333])
+@pytest.mark.parametrize("v", [5, 40, 300, 700, 33333])
 def test_select_dead_finished_and_not_a_number(dev, v):
     import vector_quantize_pytorch_amd as A
     b, j, k, end = 4, 6, 9, v // 2
@@ -149,7 +150,7 @@ def test_select_dead_finished_and_not_a_number(dev, v):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("j,v,k", [(3, 5, 15), (4, 1500, 64), (2, 50000, 64), (5, 9001, 7)])
+@pytest.mark.parametrize("j,v,k", [(3, 5, 15), (4, 1500, 64), (2, 50000, 64), (5, 9001, 7), (16, 16, 16), (4, 100, 7), (8, 120, 64), (7, 250, 64), (5, 800, 64), (64, 64, 3)])
 def test_select_ties(dev, j, v, k):
     """equal continuations survive by ascending place: a constant table, few values, runs in ascending and descending order"""
     import vector_quantize_pytorch_amd as A

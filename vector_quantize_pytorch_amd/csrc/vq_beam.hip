@@ -12,7 +12,7 @@
 // Within a row c grows with l, so the K best of a row are the K largest l (where 64 bits tell their c apart, see sel_places).  Two
 // launches: vq_beam_rows_kernel reads every logit once (its tile stays in registers), and leaves of each tile the log-sum's maximum and
 // sum and its K largest logits; vq_beam_merge_kernel joins the tiles of a batch entry's rows.  Bound by the read of the logits.
-// vq_beam_small_kernel does small entries in one launch.
+// vq_beam_small_kernel and vq_beam_entry_kernel do entries of up to 64 and SEL_ENTRY continuations in one launch.
 struct SelArgs {
     const void *logits; int64_t lb, lj;                 // element strides of batch and beam
     int dtype;
@@ -99,11 +99,10 @@ __device__ __forceinline__ unsigned sel_order(float f)       // ascending like f
 
 __device__ __forceinline__ float sel_value(unsigned u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
 
-// a value that at least K (<= 64) of the wave's 64 values are not below, the K-th largest cut to its upper 20 bits: bisection over the
-// ordered bits, a ballot each.  -inf where fewer than K are above it.
-__device__ __forceinline__ float sel_kth(float f, int K)
+// a value that at least K (<= 64) of the wave's 64 values (sel_order's bits) are not below, the K-th largest cut to its upper 20 bits:
+// bisection over the bits, a ballot each.  -inf where fewer than K are above it.
+__device__ __forceinline__ float sel_kth(unsigned mine, int K)
 {
-    const unsigned mine = sel_order(f);
     unsigned kth = 0;
 #pragma unroll
     for (int bit = 31; bit >= 12; --bit) {
@@ -117,6 +116,205 @@ __device__ __forceinline__ float sel_kth(float f, int K)
 // is off by 5 steps of fp32, e^-5 of one in the sum.  Measured on normal logits of deviation 1 to 4, 1000 to 131071 of them: log-sums off
 // by 2e-8 to 5e-8 rms, most of it the same for every row (the rounding of log2 e).
 __device__ __forceinline__ float sel_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// i / of and i % of along i, i + step, ...: the divisions once
+struct SelWalk {
+    int q, r, dq, dr, of;
+    __device__ SelWalk(int i, int of_, int step) : q(i / of_), r(i - q * of_), dq(step / of_), dr(step - dq * of_), of(of_) {}
+    __device__ __forceinline__ void next() { q += dq; r += dr; if (r >= of) { r -= of; ++q; } }
+};
+
+// like sel_order in 64 bits, for scores
+__device__ __forceinline__ unsigned long long sel_order64(double c)
+{
+    const unsigned long long u = (unsigned long long)__double_as_longlong(c + 0.0);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// Where too many scores reach a first bound: a cut (value, last place among those equal to it) that at least K and at most `cap` (> K)
+// are not behind.  Bisection over the ordered bits until that holds, among equal ones over the places (`places` in all).
+// count(pred): how many of the workgroup's scores above -inf fulfil pred(ordered bits, place).
+struct SelCut { unsigned long long value; int place; };
+template <typename Count> __device__ __forceinline__ SelCut sel_cut(int K, int cap, int places, Count &&count)
+{
+    SelCut cut{0, 0x7fffffff};
+#pragma unroll 1
+    for (int bit = 63; bit >= 0; --bit) {
+        const unsigned long long want = cut.value | 1ull << bit;
+        const int n = count([&](unsigned long long o, int) { return o >= want; });
+        if (n >= K) {
+            cut.value = want;
+            if (n <= cap) return cut;
+        }
+    }
+    const unsigned long long kth = cut.value;
+    const int above = count([&](unsigned long long o, int) { return o > kth; });
+    int lo = 0, hi = places - 1;
+    while (lo < hi) {                                         // the least place with `above` + (equal ones up to it) >= K
+        const int mid = lo + (hi - lo) / 2;
+        if (above + count([&](unsigned long long o, int p) { return o == kth && p <= mid; }) >= K) hi = mid; else lo = mid + 1;
+    }
+    cut.place = lo;
+    return cut;
+}
+__device__ __forceinline__ bool sel_within(const SelCut &cut, unsigned long long o, int place) { return o > cut.value || (o == cut.value && place <= cut.place); }
+
+// the sum of c over a workgroup of NT threads, for all of them; `red` holds NT / 64 ints
+template <int NT> __device__ __forceinline__ int sel_count(int c, int *red)
+{
+    c = vq_wave_sum(c);
+    if (NT == 64) return c;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) c += red[w];
+    return c;
+}
+
+// ---- entries of up to NT * E continuations in one launch ------------------------------------------------------------------------------
+// A workgroup (a wave for up to 1024) holds an entry's continuations, i = u * NT + t of thread t, as 64-bit scores; for the rows' log-sums the
+// logits lie in LDS once, where lanes of a power of two sum a row.  The K best by a bound from 64 groups, sel_cut where more than CAP reach it,
+// and ranks.  Bound by instructions and the latency of its steps, so few waves an entry: 8192 entries of 32 x 32 fp32 with log-sums 36 us with 16
+// a lane of one wave, 45 and 54 with 2 and 4 waves; 16384 of 16 x 16 28 us with 4 a lane, 33 with 8.  In two launches as below, 8192 entries:
+// 16 x 16 141 us (here 18), 4 x 1024 129 (90), 8 x 512 82 (93).
+#define SEL_ENTRY 4096
+template <typename T, int NT, int E> __global__ void __launch_bounds__(NT) vq_beam_entry_kernel(const SelArgs a)
+{
+    constexpr int CAP = NT == 64 ? 128 : 256;
+    __shared__ float tile[NT * E + NT * E / 32];              // (a word more every 32: rows of 32 logits lie in different banks)
+    __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], cs[CAP];
+    __shared__ float group_max[64];
+    __shared__ int ps[CAP], red[NT / 64], found;
+    __shared__ uint8_t fin[VQHIP_BEAM_MAX];
+    const int t = threadIdx.x, J = a.J, V = a.V, K = a.K, total = J * V;
+    const SelWalk start(t, V, NT);
+    const int64_t b = blockIdx.x;
+    const T *lg = (const T *)a.logits + b * a.lb;
+    const uint8_t *mk = a.mask ? a.mask + b * a.mb : nullptr;
+    float x[E];
+    {
+        T raw[E];
+        bool live[E];
+        SelWalk at = start;
+#pragma unroll
+        for (int u = 0; u < E; ++u, at.next()) {              // loads without conditions; past the end, the first one again
+            const bool in = u * NT + t < total;
+            const int j = in ? at.q : 0, v = in ? at.r : 0;
+            raw[u] = lg[j * a.lj + v];
+            live[u] = in && (!mk || mk[j * a.mj + v]);
+        }
+#pragma unroll
+        for (int u = 0; u < E; ++u) x[u] = live[u] ? (float)raw[u] : -INFINITY;
+    }
+    if (a.normalize)
+#pragma unroll
+        for (int u = 0; u < E; ++u) {
+            const int i = u * NT + t;
+            if (i < total) tile[i + (i >> 5)] = x[u];
+        }
+    if (t == 0) found = 0;
+    __syncthreads();
+    int w = 64;                                               // lanes of a row
+    while (w > 1 && w * J > NT) w >>= 1;
+    for (int j = t / w; j < (J + NT / w - 1) / (NT / w) * (NT / w); j += NT / w) {
+        const bool row = j < J;
+        double lse = 0.0;
+        if (a.normalize) {
+            float top = -INFINITY;
+            double sum = 0.0;
+            if (row)
+#pragma unroll 8
+                for (int v = t % w; v < V; v += w) { const int i = j * V + v; top = fmaxf(top, tile[i + (i >> 5)]); }
+            for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            if (row)
+                for (int v = t % w; v < V; v += 8 * w) {      // 8 terms in 32 bits, the rest in 64
+                    float q = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = j * V + (v + k * w < V ? v + k * w : v);
+                        const float e = sel_exp(tile[i + (i >> 5)] - top);
+                        q += v + k * w < V ? e : 0.f;
+                    }
+                    sum += q;
+                }
+            for (int o = w >> 1; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            lse = (double)top + log(sum);                     // (no logit admitted, one of +inf or NaN: not finite)
+        }
+        if (row && t % w == 0) {
+            const double s = a.scores ? (double)a.scores[b * J + j] : 0.0;
+            const bool f = a.finished && a.finished[b * J + j];
+            fin[j] = f;
+            base[j] = f || (s > -INFINITY && lse > -INFINITY && lse < INFINITY) ? s : -INFINITY;
+            log_sum[j] = lse;
+            if (a.lse_out) a.lse_out[b * J + j] = lse;
+        }
+    }
+    __syncthreads();
+    double c[E], best = -INFINITY;
+    {
+        SelWalk at = start;
+#pragma unroll
+        for (int u = 0; u < E; ++u, at.next()) {
+            c[u] = -INFINITY;
+            if (u * NT + t < total) {
+                const double s = base[at.q];
+                if (fin[at.q]) c[u] = at.r == a.end_token ? sel_sum(s, 0.0) : -INFINITY;
+                else if (s > -INFINITY && x[u] > -INFINITY) c[u] = sel_sum(s, (double)x[u] - log_sum[at.q]);
+            }
+            best = fmax(best, c[u]);
+        }
+    }
+    float low = __double2float_rd(best);                      // (32 bits, rounded down: a bound need not be exact)
+    if (NT > 64) {
+#pragma unroll
+        for (int o = 1; o < NT / 64; o <<= 1) low = fmaxf(low, __shfl_xor(low, o, 64));
+        if (t % (NT / 64) == 0) group_max[t / (NT / 64)] = low;
+        __syncthreads();
+        low = group_max[t & 63];
+    }
+    const double bound = (double)sel_kth(sel_order(low), K);
+    auto collect = [&](auto &&pred) {
+#pragma unroll
+        for (int u = 0; u < E; ++u)
+            if (c[u] > -INFINITY && pred(c[u], u * NT + t)) {
+                const int at = atomicAdd(&found, 1);
+                if (at < CAP) { cs[at] = c[u]; ps[at] = u * NT + t; }
+            }
+    };
+    collect([&](double d, int) { return d >= bound; });
+    __syncthreads();
+    int n = found;
+    if (n > CAP) {
+        const SelCut cut = sel_cut(K, CAP, total, [&](auto &&pred) {
+            int k = 0;
+#pragma unroll
+            for (int u = 0; u < E; ++u) k += c[u] > -INFINITY && pred(sel_order64(c[u]), u * NT + t) ? 1 : 0;
+            return sel_count<NT>(k, red);
+        });
+        __syncthreads();
+        if (t == 0) found = 0;
+        __syncthreads();
+        collect([&](double d, int p) { return sel_within(cut, sel_order64(d), p); });
+        __syncthreads();
+        n = found;
+    }
+    for (int i = t; i < n; i += NT) {
+        const double d = cs[i];
+        const int p = ps[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) rank += sel_before(cs[k], ps[k], d, p) ? 1 : 0;
+        if (rank < K) {
+            a.scores_out[b * K + rank] = (float)d;
+            a.parents_out[b * K + rank] = p / V;
+            a.tokens_out[b * K + rank] = p % V;
+        }
+    }
+    __syncthreads();
+    if (t == 0 && n < K) sel_fill(a, b, n);
+}
 
 // NT threads hold a tile of NT * E logits in registers, 8 consecutive ones of every NT * 8 each.  The K best:
 //   1. a bound: the threads form 64 groups; the K-th largest of the groups' maxima has at least K logits at or above it;
@@ -186,7 +384,7 @@ template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bound
     gm = group_max[t & 63];
     const float mx = vq_wave_max(gm);
     if (t >> 6 == NW - 1) {
-        const float k = sel_kth(gm, K);
+        const float k = sel_kth(sel_order(gm), K);
         if ((t & 63) == 0) bound_s = k;
     }
     // the log-sum: 8 terms in 32 bits, the rest in 64; a logit of +inf or NaN makes it NaN
@@ -336,18 +534,17 @@ __device__ void sel_places(const SelArgs &a, int64_t b, double cut, int at, cons
 
 // ---- merge: one workgroup per batch entry -------------------------------------------------------------------------------------------
 // The rows' log-sums from their tiles (16 lanes a row), then the K best of J * tiles * K (and the finished beams') by the same bound and
-// ranks in 64 bits; where ties let more than SEL_CAP through, K rounds that each find the next one.  Bound by latency: the first
-// SEL_HELD list entries of a thread are on their way while the log-sums are formed, and stay in registers.
+// ranks in 64 bits; sel_cut where more than SEL_CAP reach the bound.  Bound by latency: the first SEL_HELD list entries of a thread are on
+// their way while the log-sums are formed, and stay in registers.
 #define SEL_HELD 4
 __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
 {
     __shared__ double base[VQHIP_BEAM_MAX], log_sum[VQHIP_BEAM_MAX], cs[SEL_CAP];       // base: a row's s, -inf: no continuation
-    __shared__ float group_max[64], ls[SEL_CAP];
-    __shared__ int ps[SEL_CAP], found;
+    __shared__ float ls[SEL_CAP];
+    __shared__ unsigned group_max[64];
+    __shared__ int ps[SEL_CAP], found, red[4];
     __shared__ double cut_s;
     __shared__ uint8_t fin[VQHIP_BEAM_MAX];
-    __shared__ double rc[4];
-    __shared__ int rp[4];
     const int t = threadIdx.x, J = a.J, S = a.tiles, K = a.K;
     const int64_t b = blockIdx.x;
     const int per = S * K, total = J * per;
@@ -380,126 +577,116 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
         }
     }
     if (t == 0) found = 0;
+    if (t < 64) group_max[t] = sel_order(-INFINITY);
     __syncthreads();
-    // candidate i: list entry i % per of row i / per; a finished beam's first entry is its only continuation
-    auto value = [&](int i, int2 q, int &place) -> double {
-        const int j = i / per;
+    // candidate i: list entry row.r of row row.q, a finished beam's first one is its only continuation; entry list.r of list list.q
+    SelWalk row(t, per, 256), list(t, K, 256);
+    auto value = [&](const SelWalk &row, int2 q, int &place) -> double {
+        const int j = row.q;
         const double s = base[j];
         if (fin[j]) {
             place = j * a.V + a.end_token;
-            return i == j * per ? sel_sum(s, 0.0) : -INFINITY;
+            return row.r == 0 ? sel_sum(s, 0.0) : -INFINITY;
         }
         const double l = (double)__int_as_float(q.x);
         place = j * a.V + q.y;
         return s > -INFINITY && l > -INFINITY ? sel_sum(s, l - log_sum[j]) : -INFINITY;
     };
-    double c_held[SEL_HELD], best = -INFINITY;
+    // 64 groups: lists and, where there are fewer than 64 of them, ranks modulo R.  A list falls, so its first R entries are the largest of
+    // their groups.  (32 bits, rounded down: a bound need not be exact)
+    const int R = J * S < 64 ? 64 / (J * S) : 1;
+    auto group = [&](double c) {
+        if (list.r < R && c > -INFINITY) atomicMax(&group_max[(list.q * R + list.r) & 63], sel_order(__double2float_rd(c)));
+    };
+    double c_held[SEL_HELD];
     int p_held[SEL_HELD], place;
 #pragma unroll
-    for (int h = 0; h < SEL_HELD; ++h) {
-        c_held[h] = h * 256 + t < total ? value(h * 256 + t, held[h], p_held[h]) : -INFINITY;
-        best = fmax(best, c_held[h]);
+    for (int h = 0; h < SEL_HELD; ++h, row.next(), list.next()) {
+        c_held[h] = h * 256 + t < total ? value(row, held[h], p_held[h]) : -INFINITY;
+        group(c_held[h]);
     }
-    for (int i = SEL_HELD * 256 + t; i < total; i += 256) best = fmax(best, value(i, lists[i], place));
-    // (32 bits, rounded down: a bound need not be exact)
-    float low = __double2float_rd(best);
-    low = fmaxf(low, __shfl_xor(low, 1, 64));
-    low = fmaxf(low, __shfl_xor(low, 2, 64));
-    if ((t & 3) == 0) group_max[t >> 2] = low;
+    const SelWalk behind = row;
+    for (int i = SEL_HELD * 256 + t; i < total; i += 256, row.next(), list.next())
+        if (list.r < R) group(value(row, lists[i], place));
     __syncthreads();
     const double bound = (double)sel_kth(group_max[t & 63], K);
-    auto offer = [&](double c, int p, int logit) {
-        if (c >= bound && c > -INFINITY) {
-            const int k = atomicAdd(&found, 1);
-            if (k < SEL_CAP) { cs[k] = c; ps[k] = p; ls[k] = __int_as_float(logit); }
+    auto each = [&](auto &&f) {                               // f(score, place, logit) of this thread's candidates above -inf
+#pragma unroll
+        for (int h = 0; h < SEL_HELD; ++h)
+            if (c_held[h] > -INFINITY) f(c_held[h], p_held[h], __int_as_float(held[h].x));
+        SelWalk row = behind;
+        for (int i = SEL_HELD * 256 + t; i < total; i += 256, row.next()) {
+            const int2 q = lists[i];
+            const double c = value(row, q, place);
+            if (c > -INFINITY) f(c, place, __int_as_float(q.x));
         }
     };
-#pragma unroll
-    for (int h = 0; h < SEL_HELD; ++h) offer(c_held[h], p_held[h], held[h].x);
-    for (int i = SEL_HELD * 256 + t; i < total; i += 256) {
-        const int2 q = lists[i];
-        const double c = value(i, q, place);
-        offer(c, place, q.x);
-    }
+    auto collect = [&](auto &&pred) {
+        each([&](double c, int p, float l) {
+            if (pred(c, p)) {
+                const int k = atomicAdd(&found, 1);
+                if (k < SEL_CAP) { cs[k] = c; ps[k] = p; ls[k] = l; }
+            }
+        });
+    };
+    collect([&](double c, int) { return c >= bound; });
     __syncthreads();
     // whether a logit below l, which no list may hold, has l's c (the cut's) too
     auto more = [&](int j, float l) { return !fin[j] && sel_sum(base[j], (double)nextafterf(l, -INFINITY) - log_sum[j]) == cut_s; };
-    bool open = false;
-    int n = found, above = 0;
-    if (n <= SEL_CAP) {
-        for (int i = t; i < n; i += 256) {
-            const double c = cs[i];
-            const int p = ps[i];
-            int rank = 0;
+    int n = found;
+    const bool many = n > SEL_CAP;
+    if (many) {
+        const SelCut cut = sel_cut(K, SEL_CAP, J * a.V, [&](auto &&pred) {
+            int k = 0;
+            each([&](double c, int p, float) { k += pred(sel_order64(c), p) ? 1 : 0; });
+            return sel_count<256>(k, red);
+        });
+        __syncthreads();
+        if (t == 0) found = 0;
+        __syncthreads();
+        collect([&](double c, int p) { return sel_within(cut, sel_order64(c), p); });
+        __syncthreads();
+        n = found;
+    }
+    for (int i = t; i < n; i += 256) {
+        const double c = cs[i];
+        const int p = ps[i];
+        int rank = 0;
 #pragma unroll 8
-            for (int k = 0; k < n; ++k) rank += sel_before(cs[k], ps[k], c, p) ? 1 : 0;
-            if (rank < K) {
-                a.scores_out[b * K + rank] = (float)c;
-                a.parents_out[b * K + rank] = p / a.V;
-                a.tokens_out[b * K + rank] = p % a.V;
-            }
-            if (rank == K - 1) cut_s = c;
+        for (int k = 0; k < n; ++k) rank += sel_before(cs[k], ps[k], c, p) ? 1 : 0;
+        if (rank < K) {
+            a.scores_out[b * K + rank] = (float)c;
+            a.parents_out[b * K + rank] = p / a.V;
+            a.tokens_out[b * K + rank] = p % a.V;
         }
-        __syncthreads();
-        if (n >= K) {
-            for (int i = t; i < n; i += 256) open |= cs[i] == cut_s && more(ps[i] / a.V, ls[i]);
-            open = __syncthreads_or(open);
-            if (open)
-                for (int k = 0; k < n; ++k) above += cs[k] > cut_s ? 1 : 0;
-            n = K;
-        }
-    } else {
-        double last = INFINITY;
-        int lastp = -1;
-        for (n = 0; n < K; ++n) {
-            double c = -INFINITY;
-            int p = 0x7fffffff;
-            for (int i = t; i < total; i += 256) {
-                const double d = value(i, lists[i], place);
-                if (sel_before(last, lastp, d, place) && d > -INFINITY && sel_before(d, place, c, p)) { c = d; p = place; }
-            }
-            for (int o = 32; o; o >>= 1) {
-                const double d = __shfl_xor(c, o, 64);
-                const int q = __shfl_xor(p, o, 64);
-                if (sel_before(d, q, c, p)) { c = d; p = q; }
-            }
-            if ((t & 63) == 0) { rc[t >> 6] = c; rp[t >> 6] = p; }
-            __syncthreads();
-            for (int w = 0; w < 4; ++w)
-                if (sel_before(rc[w], rp[w], c, p)) { c = rc[w]; p = rp[w]; }
-            __syncthreads();
-            if (!(c > -INFINITY)) break;
-            if (c < last) above = n;
-            last = c; lastp = p;
-            if (t == 0) {
-                cut_s = c;
-                a.scores_out[b * K + n] = (float)c;
-                a.parents_out[b * K + n] = p / a.V;
-                a.tokens_out[b * K + n] = p % a.V;
-            }
-        }
-        __syncthreads();
-        if (n == K)
-            for (int i = t; i < total; i += 256) {
-                const int2 q = lists[i];
-                open |= value(i, q, place) == cut_s && more(i / per, __int_as_float(q.x));
-            }
-        open = __syncthreads_or(open);
+        if (rank == K - 1) cut_s = c;
     }
     __syncthreads();
-    if (open) sel_places(a, b, cut_s, above, base, log_sum, fin, rp);
-    else if (t == 0 && n < K) sel_fill(a, b, n);
+    if (n < K) {
+        if (t == 0) sel_fill(a, b, n);
+        return;
+    }
+    bool open = false;
+    if (many) each([&](double c, int p, float l) { open |= c == cut_s && more(p / a.V, l); });
+    else
+        for (int i = t; i < n; i += 256) open |= cs[i] == cut_s && more(ps[i] / a.V, ls[i]);
+    if (__syncthreads_or(open)) {
+        int above = 0;
+        for (int k = 0; k < n; ++k) above += cs[k] > cut_s ? 1 : 0;
+        sel_places(a, b, cut_s, above, base, log_sum, fin, red);
+    }
 }
 
 #define SEL_MOST_SMALL ((1 << 26) - 1)
 #define SEL_MOST_TILES ((1 << 24) - 1)
 
-// tiles of the rows: one wave for rows of up to 512 logits; 8192 logits a workgroup where that gives each CU two, else 2048.  Rows and
+// small: 1 a lane, 2 a wave or a workgroup an entry.  Tiles of the rows: one wave for rows of up to 512 logits; 8192 logits a workgroup where that gives each CU two, else 2048.  Rows and
 // merge with 8192 and 2048: 128 rows of 131071 bf16 14.6 + 6.5 and 21.0 + 15.9 us, 160 rows of 8193 masked 8.2 + 5.3 and 5.4 + 6.0.
 struct SelPlan { int small, threads, per_thread, tiles; };
 static SelPlan sel_plan(int64_t B, int64_t J, int64_t V)
 {
     if (J * V <= 64) return SelPlan{1, 0, 0, 0};
+    if (J * V <= SEL_ENTRY) return SelPlan{2, 0, 0, 0};
     if (V <= 512) return SelPlan{0, 64, 8, 1};
     const bool big = B * J * ((V + 8191) / 8192) >= 512;
     return SelPlan{0, 256, big ? 32 : 8, (int)(big ? (V + 8191) / 8192 : (V + 2047) / 2048)};
@@ -515,6 +702,17 @@ template <typename T> static void sel_rows(const SelArgs &a, const SelPlan &p, h
     } else {
         if (a.mask) vq_beam_rows_kernel<T, 256, 32, true><<<grid, 256, 0, st>>>(a); else vq_beam_rows_kernel<T, 256, 32, false><<<grid, 256, 0, st>>>(a);
     }
+}
+
+template <typename T> static void sel_entries(const SelArgs &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)a.B);
+    const int n = a.J * a.V;
+    if (n <= 256) vq_beam_entry_kernel<T, 64, 4><<<grid, 64, 0, st>>>(a);
+    else if (n <= 512) vq_beam_entry_kernel<T, 64, 8><<<grid, 64, 0, st>>>(a);
+    else if (n <= 1024) vq_beam_entry_kernel<T, 64, 16><<<grid, 64, 0, st>>>(a);
+    else if (n <= 2048) vq_beam_entry_kernel<T, 128, 16><<<grid, 128, 0, st>>>(a);
+    else vq_beam_entry_kernel<T, 256, 16><<<grid, 256, 0, st>>>(a);
 }
 
 static int sel_check(const vqhip_beam_select_t *p, const char *what)
@@ -553,6 +751,12 @@ extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
     a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.end_token = (int)p->end_token; a.normalize = p->normalize != 0;
     const SelPlan plan = sel_plan(p->B, p->J, p->V);
     hipStream_t st = (hipStream_t)stream;
+    if (plan.small == 2) {
+        if (p->dtype == VQHIP_F32) sel_entries<float>(a, st);
+        else if (p->dtype == VQHIP_BF16) sel_entries<__bf16>(a, st);
+        else sel_entries<_Float16>(a, st);
+        return vq_launch_status("vqhip_beam_select");
+    }
     if (plan.small) {
         int W = 1;
         while (W < a.J * a.V) W <<= 1;
