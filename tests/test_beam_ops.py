@@ -184,7 +184,7 @@ def test_select_layouts(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("normalize", [True, False])
-@pytest.mark.parametrize("b,j,v,k", [(1, 1, 1, 1), (3, 4, 4, 6), (2, 5, 257, 9), (2, 3, 9001, 16), (1, 2, 40003, 64)])
+@pytest.mark.parametrize("b,j,v,k", [(1, 1, 1, 1), (3, 4, 4, 6), (2, 5, 257, 9), (2, 3, 9001, 16), (1, 2, 40003, 64), (70, 16, 16, 16), (3, 64, 64, 64), (3, 7, 130, 33)])
 def test_select_gradient(dev, b, j, v, k, normalize, dtype):
     """Against the formula in 64 bits.  The softmax carries 2^-19 of itself (the log-sum's 2^-20 and a 32-bit exp), the sum over the
     kept ones k steps of 2^-24, the result is rounded once to its type."""
@@ -471,8 +471,7 @@ def test_select_refusals():
             ("survivors", lambda: A.beam_select(lg, sc, 31)),
             ("survivors", lambda: A.beam_select(torch.zeros(1, 1, 1000), None, 65)),
             ("survivors", lambda: A.beam_select(torch.zeros(1, 65, 10), None, 4)),
-            ("survivors", lambda: A.beam_select(torch.zeros(1, 2, 0), None, 1)),
-            ("its gradient takes", lambda: A.beam_select(torch.zeros(1).expand(1 << 22, 4, 4).requires_grad_(), None, 1))]:
+            ("survivors", lambda: A.beam_select(torch.zeros(1, 2, 0), None, 1))]:
         with pytest.raises(VQHipError, match=match):
             call()
 

@@ -144,8 +144,6 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     for d in lead:
         n *= d
     grad = torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad))
-    if grad and n * j * (-(-v // 4096)) >= 1 << 24:
-        raise L.VQHipError(f"beam_select: {n} x {j} x {v} continuations are more than its gradient takes (2^24 tiles of 4096)")
     L._need_gpu(logits, scores, mask, finished)
     beam_size = int(beam_size)
     lg = _table(logits, n, j, v)
