@@ -8,7 +8,9 @@ the beams' states (`beam_reorder`), both differentiable.  `ResidualVQ.forward(be
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import math
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -178,6 +180,9 @@ def _collapse(sizes, strides):
 
 def _layout(t: torch.Tensor, nlead: int):
     """t [*lead, beams, ...] -> (t or its contiguous copy, batch stride, beam stride, pieces, piece stride, elements of a piece)"""
+    if t.is_contiguous():
+        run = math.prod(t.shape[nlead + 1:])
+        return t, run * t.shape[nlead], run, 1, 0, run
     shape, strides = t.shape, t.stride()
     lead = _collapse(shape[:nlead], strides[:nlead])
     inner, inner_st = list(shape[nlead + 1:]), list(strides[nlead + 1:])
@@ -200,19 +205,25 @@ def _extent(t):
 @L._on_device
 def _reorder(parents, states, outs):
     nlead, k = parents.ndim - 1, parents.shape[-1]
-    n = parents.numel() // k
-    keep, table, j = [], [], states[0].shape[nlead]
+    n, j = parents.numel() // k, states[0].shape[nlead]
+    keep, flat, last = [], [], None                          # flat: vqhip_beam_state_t rows
     for s, o in zip(states, outs):
         if s.numel() == 0:
             continue
-        t, sb, sj, pieces, ps, run = _layout(s, nlead)
-        keep.append(t)
-        es = t.element_size()
-        table.append((t.data_ptr(), o.data_ptr(), sb * es, sj * es, pieces, ps * es, run * es))
-    for i in range(0, len(table), _STATES):
-        part = table[i:i + _STATES]
-        arr = (_State * len(part))(*part)
-        L._check(L.lib().vqhip_beam_reorder(arr, len(part), _addr(parents), n, j, k, L._stream()), "vqhip_beam_reorder")
+        key = s.shape, s.stride(), s.dtype
+        if key == last:                                      # the caches of a model's layers: one layout for all
+            t = s
+        else:
+            t, sb, sj, pieces, ps, run = _layout(s, nlead)
+            es = t.element_size()
+            form = sb * es, sj * es, pieces, ps * es, run * es
+            last = key if t is s else None
+            keep.append(t)
+        flat += (t.data_ptr(), o.data_ptr(), *form)
+    table = array.array("q", flat)
+    for i in range(0, len(flat), 7 * _STATES):
+        L._check(L.lib().vqhip_beam_reorder(table.buffer_info()[0] + 8 * i, min(_STATES, (len(flat) - i) // 7), _addr(parents), n, j, k, L._stream()),
+                 "vqhip_beam_reorder")
 
 
 @L._on_device
@@ -231,11 +242,22 @@ def _reorder_bwd(parents, j, grads):
     return outs
 
 
+def _results(parents, states):
+    """new tensors for the reordered states"""
+    outs, nlead, last, lead, device = [], parents.ndim - 1, None, tuple(parents.shape), parents.device
+    for s in states:
+        if s.shape != last:
+            last = s.shape
+            shape = lead + last[nlead + 1:]
+        outs.append(torch.empty(shape, dtype=s.dtype, device=device))
+    return outs
+
+
 class _ReorderFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, parents, *states):
         nlead, k = parents.ndim - 1, parents.shape[-1]
-        outs = tuple(torch.empty(*parents.shape, *s.shape[nlead + 1:], dtype=s.dtype, device=s.device) for s in states)
+        outs = tuple(_results(parents, states))
         _reorder(parents, states, outs)
         ctx.save_for_backward(parents)
         ctx.beams = states[0].shape[nlead]
@@ -267,11 +289,14 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         return []
     nlead = parents.ndim - 1
     j = states[0].shape[nlead] if states[0].ndim > nlead else 0
+    device, fits = parents.get_device(), None                # fits: a shape that does
     for s in states:
-        if s.device != parents.device:
+        if s.get_device() != device:
             raise L.VQHipError(f"beam_reorder: tensors on different devices ({parents.device} and {s.device})")
-        if s.ndim <= nlead or s.shape[:nlead] != parents.shape[:-1] or s.shape[nlead] != j or j < 1:
-            raise L.VQHipError(f"beam_reorder: state {tuple(s.shape)}, expected {tuple(parents.shape[:-1])} + ({j or 'beams'}, ...)")
+        if s.shape != fits:
+            if s.ndim <= nlead or s.shape[:nlead] != parents.shape[:-1] or s.shape[nlead] != j or j < 1:
+                raise L.VQHipError(f"beam_reorder: state {tuple(s.shape)}, expected {tuple(parents.shape[:-1])} + ({j or 'beams'}, ...)")
+            fits = s.shape
     grad = torch.is_grad_enabled() and any(s.requires_grad for s in states)
     if out is None:
         if grad:
@@ -282,7 +307,9 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         parents = parents.contiguous()
         if grad:
             return list(_ReorderFn.apply(parents, *states))
-        out = [torch.empty(*parents.shape, *s.shape[nlead + 1:], dtype=s.dtype, device=s.device) for s in states]
+        out = _results(parents, states)
+        if parents.numel():
+            _reorder(parents, states, out)
     else:
         out = list(out)
         if grad:
@@ -302,7 +329,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             end_out = max(end_out, behind) if is_out else end_out
         L._need_gpu(parents, *states)
         parents = parents.contiguous()
-    if parents.numel():
-        _reorder(parents, states, out)
-        L._written(out)
+        if parents.numel():
+            _reorder(parents, states, out)
+            L._written(out)
     return out
