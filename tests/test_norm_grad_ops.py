@@ -174,6 +174,36 @@ def test_norm_far_from_zero(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("n", [64, 20000])
+@pytest.mark.parametrize("value", [1.0, 1000.0, 30000.0])
+def test_norm_flat_far_from_zero(dev, value, n, act, dtype):
+    """Groups of one value: its 64-bit mean is the value, a 32-bit number, so xh is 0 and the result the activated bias, whatever the value and the
+    number of rows.  The activation takes 2^-21 of it (exp2 of a rounded argument, a reciprocal, two products), then one rounding.
+    Nearly flat (one row a step up): xh carries the mean's rounding, 2^-24 |mean| rstd, and the roundings of rstd, 2^-20 of |xh| + |mean| rstd 2^-20 |xh|
+    (the lanes' means are rounded like the whole mean is, so the variance is off by 2 |mean| 2^-24 a deviation)"""
+    import vector_quantize_pytorch_amd as A
+    b, c, groups = 2, 32, 4
+    g = torch.Generator().manual_seed(n)
+    w, q = (1 + 0.3 * torch.randn(c, generator=g)).cuda(), (0.3 * torch.randn(c, generator=g)).cuda()
+    x = torch.full((b, n, c), value).to(DT[dtype])
+    y = A.group_norm(x.cuda(), groups, w, q, activation=act).cpu().double()
+    want = q.cpu().double().expand(b, n, c)
+    want = want * torch.sigmoid(want) if act else want
+    assert ((y - want).abs() <= (half_step(DT[dtype]) + 2.0 ** -21) * want.abs()).all()
+    x[:, n // 3] = torch.nextafter(x[:, n // 3].float(), torch.tensor(torch.inf)) if dtype == "fp32" else x[:, n // 3] * (1 + 2 * half_step(DT[dtype]))
+    want = norm_ref(x, groups, w, q, act=act)
+    t = x.double().view(b, n, groups, c // groups)
+    t = t - t.mean((1, 3), keepdim=True)
+    r = 1.0 / ((t * t).mean((1, 3), keepdim=True) + 1e-5).sqrt()
+    xh, off = (t * r).abs(), x.double().abs().max() * r
+    err = ((off * 2.0 ** -24 + xh * 2.0 ** -20 * (1 + off)).expand_as(t) * w.cpu().double().abs().view(groups, -1)).reshape(b, n, c)
+    y = A.group_norm(x.cuda(), groups, w, q, activation=act).cpu().double()
+    assert ((y - want).abs() <= half_step(DT[dtype]) * want.abs() + 1.1 * err * (1 + half_step(DT[dtype])) + 2.0 ** -21 * (want.abs() + err) + (2.0 ** -25 if dtype == "fp16" else 0)).all()
+
+
+@pytest.mark.gpu
 def test_norm_layouts_and_module(dev):
     import vector_quantize_pytorch_amd as A
     torch.manual_seed(0)

@@ -320,9 +320,8 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
     const T *x = (const T *)a.x + b * a.xb;
     const uint8_t *mask = MASKED ? a.mask + b * a.N : nullptr;
     T *y = (T *)a.y + b * a.N * a.C;
-    // 16-bit rows: x scale + (bias - mean scale) in one step, its rounding is far below theirs.  32-bit rows subtract the mean first: a mean
-    // far from zero then costs nothing.
-    constexpr bool FOLD = sizeof(T) == 2;
+    // (x - mean) scale + bias, the mean first: bias - mean scale would round a number |mean| rstd times the result's size, and flat rows far from
+    // zero would lose their bias to it (values of 1000 and a bias of 0.2: 0.212).  6 x 65536 x 128 bf16 57 us a call either way
     for (int col = t % sh.width; col < sh.cols; col += sh.width) {
         float mean[VEC], scale[VEC], shift[VEC];
         gn_params<VEC>(a.weight, a.wdtype, col * VEC, 1.f, scale);
@@ -331,9 +330,8 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
 #pragma unroll
         for (int i = 0; i < VEC; ++i, of.next()) {
             const float2 st = stat[of.g];
-            mean[i] = FOLD ? 0.f : st.x;
+            mean[i] = st.x;
             scale[i] *= st.y;
-            if (FOLD) shift[i] = fmaf(-st.x, scale[i], shift[i]);
         }
         const T *xc = x + (int64_t)col * VEC;
         T *yc = y + (int64_t)col * VEC;
@@ -353,7 +351,7 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
                 VqVec<T, VEC> o;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    float z = fmaf(FOLD ? (float)v[u].v[i] : (float)v[u].v[i] - mean[i], scale[i], shift[i]);
+                    float z = fmaf((float)v[u].v[i] - mean[i], scale[i], shift[i]);
                     if (SILU) z *= gn_sigmoid(z);
                     o.v[i] = !MASKED || live[u] ? (T)z : (T)0.f;
                 }
