@@ -450,6 +450,44 @@ def test_residual_beam_search_needs_losses(dev):
         r.eval()(torch.randn(1, 8, 32, device="cuda"))
 
 
+@pytest.mark.gpu
+def test_reorder_of_conjugated_and_negated_states(dev):
+    """torch's conj() and imag of it leave memory as it is and set a flag: the results are the tensors' values"""
+    import vector_quantize_pytorch_amd as A
+    z = torch.randn(3, 4, 6, 5, dtype=torch.complex64, device="cuda")
+    par = torch.tensor([[1, 1, 3], [0, 2, -1], [3, 0, 0]], device="cuda")
+    states = [z.conj(), z.conj().imag, z.conj()[..., 1:4], z.transpose(2, 3).conj(), torch._neg_view(z.real.contiguous()), z, z.mH]
+    for s, n in zip(states, A.beam_reorder(states, par)):
+        assert torch.equal(n.cpu(), reorder_ref(s.resolve_conj().resolve_neg(), par))
+    out = [torch.empty(3, 3, *s.shape[2:], dtype=s.dtype, device="cuda") for s in states]
+    A.beam_reorder(states, par, out=out)
+    for s, o in zip(states, out):
+        assert torch.equal(o.cpu(), reorder_ref(s.resolve_conj().resolve_neg(), par))
+    im = torch.randn(3, 4, 7, device="cuda", requires_grad=True)
+    new, = A.beam_reorder([torch.complex(im, im).conj().imag], par)
+    w = torch.randn(3, 3, 7, device="cuda")
+    assert torch.equal(new.detach().cpu(), reorder_ref(-im, par))
+    got, = torch.autograd.grad(new, im, torch._neg_view(w), retain_graph=True)
+    back, = torch.autograd.grad(new, im, w)
+    assert torch.equal(got, -back) and back.abs().sum() > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [1, 6, 300, 9000])
+def test_select_of_negated_tensors(dev, v):
+    import vector_quantize_pytorch_amd as A
+    lg, sc = make(3, 4, v, "fp32", seed=v)
+    k = min(5, 4 * v)
+    ref = select_ref(lg, sc, k)
+    for a, b in ((torch._neg_view(-lg), sc), (lg, torch._neg_view(-sc)), (torch.complex(lg, -lg).conj().imag, torch.complex(sc, -sc).conj().imag)):
+        check_select(A.beam_select(a, b, k), ref)
+    lg.requires_grad_(True)
+    w = torch.randn(3, k, device="cuda")
+    step = A.beam_select(lg, sc, k)
+    got, = torch.autograd.grad(step.scores, lg, torch._neg_view(-w), retain_graph=True)
+    assert torch.equal(got, torch.autograd.grad(step.scores, lg, w)[0])
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A
@@ -535,3 +573,13 @@ def test_c_entry_refusals():
     assert L.vqhip_beam_reorder_bwd(st, None, 1, 8, 1, 2, 2, None) == -1
     odd = (_State * 1)((8, 8, 32, 16, 1, 0, 15))
     assert L.vqhip_beam_reorder_bwd(odd, (ctypes.c_int64 * 1)(1), 1, 8, 1, 2, 2, None) == -1
+
+
+def test_reorder_refuses_flagged_results():
+    """a result with a pending conjugation or negation would hold something else than what is written into its memory"""
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    z, par = torch.zeros(2, 3, 8, dtype=torch.complex64), torch.zeros(2, 4, dtype=torch.int64)
+    for s, o in ((z, torch.zeros(2, 4, 8, dtype=torch.complex64).conj()), (z.real, torch._neg_view(torch.zeros(2, 4, 8)))):
+        with pytest.raises(VQHipError, match="pending"):
+            A.beam_reorder([s], par, out=[o])

@@ -450,6 +450,43 @@ def test_training_step_of_a_tokenizer(dev, dtype):
         assert far[torch.arange(n, device="cuda")[None] < lens[:, None]].max().item() <= 0.0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,c,groups", [(9, 16, 4), (20000, 16, 4), (5, 1, 1)])
+def test_norm_of_negated_tensors(dev, n, c, groups):
+    """torch leaves a negation (the imaginary part of a conjugate, say) pending in a flag: rows, parameters and gradients count with it"""
+    import vector_quantize_pytorch_amd as A
+    ts = norm_inputs(2, n, c, "fp32", "fp32")
+
+    def step(x, w, q, grad):
+        x, w, q = (t.detach().requires_grad_(True) for t in (x, w, q))
+        y = A.group_norm(x, groups, w, q, activation="silu")
+        return (y, *torch.autograd.grad(y, (x, w, q), grad))
+
+    want = step(*ts)
+    for i in range(4):
+        for flagged in (torch._neg_view(-ts[i]), torch.complex(ts[i], -ts[i]).conj().imag):
+            assert flagged.is_neg() and all(torch.equal(a, b) for a, b in zip(step(*ts[:i], flagged, *ts[i + 1:]), want))
+
+
+@pytest.mark.gpu
+def test_clip_of_negated_tensors(dev):
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    g = torch.complex(*[torch.full((1,), 3.0, device="cuda")] * 2).conj().imag       # -3, contiguous, memory of +3
+    h = torch.full((1,), 4.0, device="cuda")
+    (a, b), norm = A.clip_grads([g, h], 2.5)
+    assert norm.item() == 5.0 and abs(a.item() + 1.5) < 1e-6 and abs(b.item() - 2.0) < 1e-6
+    o = [torch.empty(1, device="cuda") for _ in range(2)]
+    A.clip_grads([g, h], 2.5, out=o)
+    assert abs(o[0].item() + 1.5) < 1e-6 and abs(o[1].item() - 2.0) < 1e-6
+    p = torch.nn.Parameter(torch.zeros(1, device="cuda"))
+    p.grad = g
+    A.clip_grad_norm_([p], 1.5)
+    assert abs(p.grad.item() + 1.5) < 1e-6
+    with pytest.raises(VQHipError, match="pending"):
+        A.clip_grads([h], 1.0, out=[torch.complex(h, h).conj().imag])
+
+
 # ---- refusals (host side: no GPU) -------------------------------------------------------------------------------------------------------
 def test_norm_refusals():
     import vector_quantize_pytorch_amd as A

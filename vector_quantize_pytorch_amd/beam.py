@@ -102,7 +102,7 @@ class _SelectFn(torch.autograd.Function):
         if grad is None:
             return (None,) * 7
         logits, mask, finished, out, parents, tokens, lse = ctx.saved_tensors
-        d_logits, d_scores = _select_bwd(grad.contiguous(), logits, mask, finished, ctx.end_token, ctx.normalize, out, parents, tokens, lse,
+        d_logits, d_scores = _select_bwd(grad.resolve_neg().contiguous(), logits, mask, finished, ctx.end_token, ctx.normalize, out, parents, tokens, lse,
                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return d_logits, d_scores, None, None, None, None, None
 
@@ -148,7 +148,8 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     grad = torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad))
     L._need_gpu(logits, scores, mask, finished)
     beam_size = int(beam_size)
-    lg = _table(logits, n, j, v)
+    lg = _table(logits.resolve_neg(), n, j, v)              # (the library reads memory, where torch leaves a negation pending in a flag)
+    scores = None if scores is None else scores.resolve_neg()
     sc = scores if scores is None or (len(lead) == 1 and scores.is_contiguous()) else scores.reshape(n, j).contiguous()
     mk = None if mask is None else _table(mask, n, j, v).view(torch.uint8)
     fin = None if finished is None else finished.reshape(n, j).contiguous().view(torch.uint8)
@@ -196,6 +197,15 @@ def _layout(t: torch.Tensor, nlead: int):
     return t, lead[1], strides[nlead], pieces[0], pieces[1], run
 
 
+def _flagged(tensors):
+    """whether a tensor's values are not what its memory holds: conj(), and the imaginary part of its result, only set a flag"""
+    return any(map(torch.Tensor.is_conj, tensors)) or any(map(torch.Tensor.is_neg, tensors))
+
+
+def _resolved(states):
+    return [s.resolve_conj().resolve_neg() for s in states] if _flagged(states) else states
+
+
 def _extent(t):
     """[first byte, behind the last byte) of a tensor's memory"""
     span = sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
@@ -231,7 +241,7 @@ def _reorder_bwd(parents, j, grads):
     nlead, k = parents.ndim - 1, parents.shape[-1]
     n = parents.numel() // k
     lead = parents.shape[:-1]
-    grads = [None if g is None else g.contiguous() for g in grads]
+    grads = [None if g is None else g.resolve_neg().contiguous() for g in grads]
     outs = [None if g is None else torch.empty(*lead, j, *g.shape[nlead + 1:], dtype=g.dtype, device=g.device) for g in grads]
     some = [(g, o) for g, o in zip(grads, outs) if g is not None and o.numel()]
     for i in range(0, len(some), _STATES):
@@ -304,7 +314,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
                 if s.requires_grad:
                     L._elem_code(s, "beam_reorder: state with a gradient")
         L._need_gpu(parents, *states)
-        parents = parents.contiguous()
+        parents, states = parents.contiguous(), _resolved(states)
         if grad:
             return list(_ReorderFn.apply(parents, *states))
         out = _results(parents, states)
@@ -320,6 +330,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             if o.shape != (*parents.shape, *s.shape[nlead + 1:]) or o.dtype != s.dtype or o.device != s.device or not o.is_contiguous():
                 raise L.VQHipError(f"beam_reorder: out {tuple(o.shape)} {o.dtype}, expected contiguous "
                                    f"{(*parents.shape, *s.shape[nlead + 1:])} {s.dtype} on {s.device}")
+        if _flagged(out):
+            raise L.VQHipError("beam_reorder: out with a pending conjugation or negation")
         taken = sorted([(*_extent(t), w) for w, ts in ((0, [*states, parents]), (1, out)) for t in ts if t.numel()])
         end = end_out = -1                                       # behind the last byte of any tensor, of any result so far
         for first, behind, is_out in taken:
@@ -328,7 +340,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             end = max(end, behind)
             end_out = max(end_out, behind) if is_out else end_out
         L._need_gpu(parents, *states)
-        parents = parents.contiguous()
+        parents, states = parents.contiguous(), _resolved(states)
         if parents.numel():
             _reorder(parents, states, out)
             L._written(out)

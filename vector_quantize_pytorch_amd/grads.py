@@ -41,11 +41,26 @@ def _check(grads, out):
             raise L.VQHipError(f"clip_grads: out {tuple(o.shape)} {o.dtype}, expected {g.numel()} contiguous elements of {g.dtype} on {g.device}")
 
 
+def _unflagged(grads, out):
+    """grads with a pending negation carried out where the result has none (the imaginary part of a conjugate only sets a flag; its strides are
+    even, so of contiguous tensors single elements alone have one)"""
+    grads = list(grads)
+    for i, g in enumerate(grads):
+        if out is not None and out[i].is_neg() and not g.is_neg():
+            raise L.VQHipError("clip_grads: out with a pending negation")
+        if g.is_neg() and (out is None or not out[i].is_neg()):
+            grads[i] = g.resolve_neg()
+    return grads
+
+
 def _table(grads, out):
-    """the checked rows of vqhip_grad_t; out None: the norm alone.  A pass over all tensors for each property: a model has hundreds, and
-    `map` takes two thirds of the time of a loop over them (311 tensors with results of their own: a call 205 us instead of 250)"""
+    """the checked rows of vqhip_grad_t, and the tensors that they point to; out None: the norm alone.  A pass over all tensors for each
+    property: a model has hundreds, and `map` takes two thirds of the time of a loop over them (311 tensors with results of their own: a
+    call 205 us instead of 250)"""
     T, codes = torch.Tensor, L._ELEM_CODES
     dtypes, sizes = [t.dtype for t in grads], list(map(T.numel, grads))
+    if 1 in sizes and out is not grads:
+        grads = _unflagged(grads, out)
     fine = all(map(T.is_contiguous, grads)) and len(set(map(T.get_device, grads))) == 1 and all(map(codes.__contains__, set(dtypes)))
     if out is not None and out is not grads:
         fine = fine and sizes == list(map(T.numel, out)) and dtypes == [t.dtype for t in out] and all(map(T.is_contiguous, out)) \
@@ -58,7 +73,7 @@ def _table(grads, out):
         flat[1::4] = map(T.data_ptr, out)
     flat[2::4] = sizes
     flat[3::4] = [codes[d] for d in dtypes]
-    return array.array("q", flat)
+    return array.array("q", flat), grads
 
 
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[Sequence[torch.Tensor]] = None):
@@ -75,7 +90,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     if not grads:
         return [], torch.zeros((), dtype=torch.float32)
     if out is None:
-        table = _table(grads, None)
+        table, grads = _table(grads, None)
         L._need_gpu(grads[0])
         out = [torch.empty_like(g) for g in grads]
         table[1::4] = array.array("q", [o.data_ptr() for o in out])
@@ -83,7 +98,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
         out = grads if out is given else list(out)
         if len(out) != len(grads):
             raise L.VQHipError(f"clip_grads: {len(out)} results for {len(grads)} tensors")
-        table = _table(grads, out)
+        table, grads = _table(grads, out)
         L._need_gpu(grads[0])
     norm = _clip(grads[0], table, float(max_norm))
     L._written(out)
@@ -99,7 +114,7 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, *, erro
     grads = list({id(p.grad): p.grad.detach() for p in parameters if p.grad is not None}.values())      # a shared one counts once
     work = [g if g.is_contiguous() else g.contiguous() for g in grads]
     if error_if_nonfinite and work:
-        table = _table(work, None)
+        table, _ = _table(work, None)
         L._need_gpu(work[0])
         if not torch.isfinite(_clip(work[0], table, 0.0)).item():
             raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")

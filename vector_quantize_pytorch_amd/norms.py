@@ -74,7 +74,7 @@ class _GroupNormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, weight, bias, lens, mask, stats = ctx.saved_tensors
-        dx, dw, db = _backward(grad.contiguous(), x, weight, bias, lens, mask, *ctx.args, stats, *ctx.needs_input_grad[:3])
+        dx, dw, db = _backward(grad.resolve_neg().contiguous(), x, weight, bias, lens, mask, *ctx.args, stats, *ctx.needs_input_grad[:3])
         return dx, dw, db, None, None, None, None, None
 
 
@@ -109,6 +109,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     if lens is not None and (x.ndim != 3 or lens.dtype not in (torch.int64, torch.int32) or tuple(lens.shape) != (b,)):
         raise L.VQHipError(f"group_norm: lens {tuple(lens.shape)} {lens.dtype} for x {tuple(x.shape)}, expected integers [b] for [b, n, c]")
     L._need_gpu(x, weight, bias, mask, lens)
+    x = x.resolve_neg()                                     # (the library reads memory, where torch leaves a negation pending in a flag)
+    weight, bias = (None if p is None else p.resolve_neg() for p in (weight, bias))
     rows = x if x.ndim == 3 else x.flatten(1, -2) if x.ndim > 3 else x[:, None]
     if rows.stride(-1) != 1 and c > 1:
         rows = rows.contiguous()
