@@ -583,3 +583,25 @@ def test_reorder_refuses_flagged_results():
     for s, o in ((z, torch.zeros(2, 4, 8, dtype=torch.complex64).conj()), (z.real, torch._neg_view(torch.zeros(2, 4, 8)))):
         with pytest.raises(VQHipError, match="pending"):
             A.beam_reorder([s], par, out=[o])
+
+
+def test_forward_mode_is_refused():
+    """a dual tensor's tangent would be lost: no entry point has a forward-mode derivative (host side: no GPU)"""
+    import torch.autograd.forward_ad as fwad
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    lg, sc, st, par = torch.zeros(2, 3, 10), torch.zeros(2, 3), torch.zeros(2, 3, 8), torch.zeros(2, 4, dtype=torch.int64)
+    with fwad.dual_level():
+        def dual(t):
+            return fwad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: A.beam_select(dual(lg), sc, 4), lambda: A.beam_select(lg, dual(sc), 4), lambda: A.beam_reorder([st, dual(st)], par),
+                     lambda: A.beam_reorder([dual(st)], par, out=[torch.zeros(2, 4, 8)]), lambda: A.beam_reorder([st], par, out=[dual(torch.zeros(2, 4, 8))]),
+                     lambda: A.beam_select(dual(lg.clone().requires_grad_()), sc, 4)):
+            with pytest.raises(VQHipError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(VQHipError, match="forward-mode"):
+                call()
+        with pytest.raises(VQHipError, match="no CPU fallback"):             # a level without a tangent is no hindrance
+            A.beam_select(lg, sc, 4)
+    with pytest.raises(VQHipError, match="forward-mode"):
+        torch.func.jvp(lambda t: A.beam_select(t, sc, 4).scores, (lg,), (lg,))

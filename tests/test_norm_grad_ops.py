@@ -573,3 +573,23 @@ def test_c_entry_refusals():
                  ((64, 128, 4, 0), (256, 140, 4, 0)), ((64, 128, 8, 0), (140, 256, 4, 0)), ((64, 64, 8, 0), (95, 95, 4, 0))]:
         args = ((_Grad * 2)(*pair), 2, 1.0, 1e-6, 8, 16, many)
         assert L.vqhip_clip_grads(*args, None) == -1
+
+
+def test_forward_mode_is_refused():
+    """a dual tensor's tangent would be lost: no entry point has a forward-mode derivative (host side: no GPU)"""
+    import torch.autograd.forward_ad as fwad
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    x, w = torch.zeros(2, 5, 16), torch.ones(16)
+    with fwad.dual_level():
+        def dual(t):
+            return fwad.make_dual(t, torch.ones_like(t))
+        p = torch.nn.Parameter(torch.zeros(4))
+        p.grad = dual(torch.ones(4))
+        for call in (lambda: A.group_norm(dual(x), 4), lambda: A.group_norm(x, 4, dual(w)), lambda: A.group_norm(x, 4, w, dual(w)),
+                     lambda: A.GroupNorm(4, 16)(dual(x)), lambda: A.clip_grads([x, dual(x)], 1.0), lambda: A.clip_grads([x], 1.0, out=[dual(x.clone())]),
+                     lambda: A.clip_grad_norm_([p], 1.0)):
+            with pytest.raises(VQHipError, match="forward-mode"):
+                call()
+        with pytest.raises(VQHipError, match="no CPU fallback"):             # a level without a tangent is no hindrance
+            A.group_norm(x, 4)

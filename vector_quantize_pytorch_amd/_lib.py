@@ -11,6 +11,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("VQHIP_SO", os.path.join(_HERE, "csrc", "libvqhip.so"))   # VQHIP_SO: A/B experiments only
@@ -253,6 +254,14 @@ def _need_gpu(*ts):
         if t is not None and not t.is_cuda:
             raise VQHipError("vector_quantize_pytorch_amd runs on MI355X only: got a CPU tensor "
                              "(there is no CPU fallback; move the module and input to 'cuda')")
+
+
+def _no_tangent(what: str, tensors):
+    """refuses tensors with a forward-mode tangent, which a call outside of autograd would drop (the differentiated ones have no such rule)"""
+    if forward_ad._current_level >= 0:                       # (inside a dual_level or torch.func.jvp)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise VQHipError(f"{what}: no forward-mode derivative")
 
 
 def _written(tensors):

@@ -119,7 +119,7 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     finished  bool [..., beams]: such a beam is kept as it is, as its own only continuation `end_token`
     A score that is not a number counts as -inf: a beam whose logits hold NaN or +inf, or whose mask leaves nothing, has no
     continuation (normalize=True).  Where fewer than beam_size continuations are left, the last survivors have a score of -inf.
-    Gradients reach logits and scores through the returned scores; survivors of score -inf pass none on."""
+    Gradients reach logits and scores through the returned scores (backward mode); survivors of score -inf pass none on."""
     L._elem_code(logits, "beam_select")
     if logits.ndim < 2:
         raise L.VQHipError(f"beam_select: logits {tuple(logits.shape)}, expected [..., beams, vocabulary]")
@@ -145,6 +145,7 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     n = 1
     for d in lead:
         n *= d
+    L._no_tangent("beam_select", (logits, scores))
     grad = torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad))
     L._need_gpu(logits, scores, mask, finished)
     beam_size = int(beam_size)
@@ -307,6 +308,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             if s.ndim <= nlead or s.shape[:nlead] != parents.shape[:-1] or s.shape[nlead] != j or j < 1:
                 raise L.VQHipError(f"beam_reorder: state {tuple(s.shape)}, expected {tuple(parents.shape[:-1])} + ({j or 'beams'}, ...)")
             fits = s.shape
+    L._no_tangent("beam_reorder", states)
     grad = torch.is_grad_enabled() and any(s.requires_grad for s in states)
     if out is None:
         if grad:
@@ -330,6 +332,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             if o.shape != (*parents.shape, *s.shape[nlead + 1:]) or o.dtype != s.dtype or o.device != s.device or not o.is_contiguous():
                 raise L.VQHipError(f"beam_reorder: out {tuple(o.shape)} {o.dtype}, expected contiguous "
                                    f"{(*parents.shape, *s.shape[nlead + 1:])} {s.dtype} on {s.device}")
+        L._no_tangent("beam_reorder", out)
         if _flagged(out):
             raise L.VQHipError("beam_reorder: out with a pending conjugation or negation")
         taken = sorted([(*_extent(t), w) for w, ts in ((0, [*states, parents]), (1, out)) for t in ts if t.numel()])

@@ -83,12 +83,14 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     grads: contiguous float32 / bfloat16 / float16 tensors of one device; out: contiguous tensors of the same types and numbers of
     elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that
     is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  max_norm inf: the norm alone
-    (nothing is scaled unless it is NaN).  No gradient passes through."""
+    (nothing is scaled unless it is NaN).  No gradient passes through, and a forward-mode
+    tangent is refused."""
     given, grads = grads, list(grads)
     if not max_norm >= 0.0:
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")
     if not grads:
         return [], torch.zeros((), dtype=torch.float32)
+    L._no_tangent("clip_grads", grads)
     if out is None:
         table, grads = _table(grads, None)
         L._need_gpu(grads[0])
@@ -98,6 +100,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
         out = grads if out is given else list(out)
         if len(out) != len(grads):
             raise L.VQHipError(f"clip_grads: {len(out)} results for {len(grads)} tensors")
+        L._no_tangent("clip_grads", out)
         table, grads = _table(grads, out)
         L._need_gpu(grads[0])
     norm = _clip(grads[0], table, float(max_norm))
@@ -111,6 +114,8 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, *, erro
     contiguous is clipped through a contiguous copy."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
+    parameters = list(parameters)
+    L._no_tangent("clip_grad_norm_", [p.grad for p in parameters])
     grads = list({id(p.grad): p.grad.detach() for p in parameters if p.grad is not None}.values())      # a shared one counts once
     work = [g if g.is_contiguous() else g.contiguous() for g in grads]
     if error_if_nonfinite and work:

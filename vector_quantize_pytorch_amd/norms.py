@@ -108,6 +108,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         raise L.VQHipError(f"group_norm: mask {tuple(mask.shape)} {mask.dtype} for x {tuple(x.shape)}, expected bool [b, n] for [b, n, c]")
     if lens is not None and (x.ndim != 3 or lens.dtype not in (torch.int64, torch.int32) or tuple(lens.shape) != (b,)):
         raise L.VQHipError(f"group_norm: lens {tuple(lens.shape)} {lens.dtype} for x {tuple(x.shape)}, expected integers [b] for [b, n, c]")
+    L._no_tangent("group_norm", (x, weight, bias))
     L._need_gpu(x, weight, bias, mask, lens)
     x = x.resolve_neg()                                     # (the library reads memory, where torch leaves a negation pending in a flag)
     weight, bias = (None if p is None else p.resolve_neg() for p in (weight, bias))
