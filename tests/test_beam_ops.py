@@ -488,6 +488,24 @@ def test_select_of_negated_tensors(dev, v):
     assert torch.equal(got, torch.autograd.grad(step.scores, lg, w)[0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead,j,v", [((3,), 4, 4), ((3,), 4, 3000), ((2, 2), 5, 50)])
+def test_tokens_may_be_edited_between_selection_and_backward(dev, lead, j, v):
+    """parents, tokens and scores are tensors of their own: the backward of a reordering needs the parents alone"""
+    import vector_quantize_pytorch_amd as A
+    lg = torch.randn(*lead, j, v, device="cuda")
+    state = torch.randn(*lead, j, 6, device="cuda", requires_grad=True)
+    step = A.beam_select(lg, None, 4)
+    assert len({t.data_ptr() for t in step}) == 3 and all(t.is_contiguous() for t in step)
+    new, = A.beam_reorder([state], step.parents)
+    parents = step.parents.clone()
+    step.tokens.masked_fill_(step.tokens == v - 1, 0)
+    step.scores.zero_()
+    new.sum().backward()
+    want = torch.zeros(*lead, j, device="cuda").scatter_add_(-1, parents, torch.ones(*lead, 4, device="cuda"))
+    assert torch.equal(state.grad, want[..., None].expand_as(state))
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A

@@ -59,7 +59,8 @@ def _select(logits, scores, mask, finished, beam_size, end_token, normalize, wan
     dev = logits.device
     lib = L.lib()
     out = torch.empty((b, beam_size), dtype=torch.float32, device=dev)
-    parents, tokens = torch.empty((2, b, beam_size), dtype=torch.int64, device=dev).unbind(0)
+    # (tensors of their own: views of one would share its version, and an edit of the tokens would stop the backward of a reordering)
+    parents, tokens = (torch.empty((b, beam_size), dtype=torch.int64, device=dev) for _ in range(2))
     lse = torch.empty((b, j), dtype=torch.float64, device=dev) if want_lse else None
     nws = lib.vqhip_beam_select_workspace_bytes(b, j, v, beam_size)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
