@@ -553,8 +553,7 @@ int vqhip_row_sumsq(const void *x, int x_dtype, int64_t N, int D, int64_t ldx, f
  *   scores   nullable (zeros) [B, J] fp32        mask      nullable [B, J, V] bytes at byte strides mask_stride_b / _j (0: shared)
  *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out: the log-sums, which the backward reads
  *   out_scores / parents / tokens  [B, K]        workspace vqhip_beam_select_workspace_bytes(B, J, V, K) bytes, 16-byte aligned
- * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B * J * ceil(V / 2048) < 2^24, or B < 2^26 where J * V <= 64
- * (VQHIP_EDIM beyond).
+ * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B < 2^31 (VQHIP_EDIM beyond; batches that one launch cannot hold go in several).
  * vqhip_beam_select_bwd: the gradients of out_scores (grad [B, K]) with the fields of the forward call, its outputs among them:
  *   d_scores[b, j] (nullable [B, J] fp32) = sum of grad over the kept continuations of beam j,
  *   d_logits (nullable [B, J, V] contiguous, dtype) = sum of grad over those with token v - (normalize) d_scores softmax(logits).

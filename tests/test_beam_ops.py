@@ -506,6 +506,35 @@ def test_tokens_may_be_edited_between_selection_and_backward(dev, lead, j, v):
     assert torch.equal(state.grad, want[..., None].expand_as(state))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,j,v,k", [(2 ** 23 + 5, 2, 2, 3), (2 ** 23 + 5, 1, 65, 2), (2 ** 23 + 5, 3, 30, 4), (2 ** 18 + 1, 64, 64, 64), (2 ** 17 + 1, 64, 65, 3), (2 ** 20 + 1, 8, 513, 5)])
+def test_select_of_large_batches(dev, b, j, v, k):
+    """batches that take several launches, or more entries than a launch has tiles: the entries on either side of every border, forward and
+    backward, against the same entries alone (their tiles differ, so the log-sums' last bits may)"""
+    import vector_quantize_pytorch_amd as A
+    g = torch.Generator(device="cuda").manual_seed(j)
+    lg = torch.empty(b, j, v, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    sc = torch.randn(b, j, generator=g, device="cuda")
+    mask = torch.rand(b, 1, v, generator=g, device="cuda") < 0.8
+    fin = torch.rand(b, j, generator=g, device="cuda") < 0.1
+    some = sorted({n for per in (1, j, 2 * j) for m in (1, 2) for n in (0, 1, 2 ** 23 // per * m - 1, 2 ** 23 // per * m, b - 1) if n < b})
+    some = torch.tensor(some, device="cuda")
+    lg.requires_grad_(True)
+    sc.requires_grad_(True)
+    step = A.beam_select(lg, sc, k, mask=mask, finished=fin, end_token=v - 1)
+    w = torch.randn(b, k, generator=g, device="cuda")
+    dl, ds = torch.autograd.grad(step.scores, (lg, sc), w)
+    l1, s1 = lg.detach()[some].requires_grad_(True), sc.detach()[some].requires_grad_(True)
+    alone = A.beam_select(l1, s1, k, mask=mask[some], finished=fin[some], end_token=v - 1)
+    d1, e1 = torch.autograd.grad(alone.scores, (l1, s1), w[some])
+    check_select(alone, select_ref(l1, s1, k, mask=mask[some], finished=fin[some], end=v - 1))
+    assert torch.equal(step.parents[some], alone.parents) and torch.equal(step.tokens[some], alone.tokens) and torch.equal(ds[some], e1)
+    real = alone.scores > NEG
+    assert torch.equal(step.scores[some] > NEG, real) and ((step.scores[some] - alone.scores)[real].abs() <= 2.0 ** -20 * (1 + alone.scores[real].abs())).all()
+    assert ((dl[some].float() - d1.float()).abs() <= 2.0 ** -7 * d1.float().abs()).all()       # (one step of bf16)
+    assert not ((step.parents < 0) | (step.parents >= j) | (step.tokens < 0) | (step.tokens >= v)).any()
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A
@@ -623,3 +652,16 @@ def test_forward_mode_is_refused():
             A.beam_select(lg, sc, 4)
     with pytest.raises(VQHipError, match="forward-mode"):
         torch.func.jvp(lambda t: A.beam_select(t, sc, 4).scores, (lg,), (lg,))
+
+
+def test_c_entry_takes_large_batches():
+    """what a launch cannot hold goes in several: the batch has no limit below 2^31.  Sizes are checked before the workspace, whose alignment
+    (-3) is checked before anything is launched"""
+    from vector_quantize_pytorch_amd import _lib
+    from vector_quantize_pytorch_amd.beam import _Select
+    L = _lib.lib()
+    for b, j, v in [(2 ** 20, 16, 16), (2 ** 19, 32, 32), (2 ** 18, 64, 64), (2 ** 31 - 1, 1, 1), (2 ** 26, 8, 8), (2 ** 25, 1, 4096), (2 ** 18, 64, 65), (2 ** 25, 2, 5000)]:
+        nws = L.vqhip_beam_select_workspace_bytes(b, j, v, 4)
+        assert nws < 2 ** 34
+        s = _Select(logits=8, dtype=1, B=b, J=j, V=v, stride_b=j * v, stride_j=v, normalize=0, K=min(4, j * v), out_scores=8, parents=8, tokens=8, workspace=24, workspace_bytes=nws)
+        assert L.vqhip_beam_select(ctypes.byref(s), None) == -3, (b, j, v)

@@ -677,12 +677,13 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
     }
 }
 
-#define SEL_MOST_SMALL ((1 << 26) - 1)
-#define SEL_MOST_TILES ((1 << 24) - 1)
+// Workgroups of a launch, which takes fewer than 2^32 threads; larger batches go in several, one after the other with the same workspace.  An
+// entry has at most 2^19 + 64 tiles.
+#define SEL_LAUNCH (1 << 23)
 
 // small: 1 a lane, 2 a wave or a workgroup an entry.  Tiles of the rows: one wave for rows of up to 512 logits; 8192 logits a workgroup where that gives each CU two, else 2048.  Rows and
 // merge with 8192 and 2048: 128 rows of 131071 bf16 14.6 + 6.5 and 21.0 + 15.9 us, 160 rows of 8193 masked 8.2 + 5.3 and 5.4 + 6.0.
-struct SelPlan { int small, threads, per_thread, tiles; };
+struct SelPlan { int small, threads, per_thread, tiles; };           // (tiles: of a row)
 static SelPlan sel_plan(int64_t B, int64_t J, int64_t V)
 {
     if (J * V <= 64) return SelPlan{1, 0, 0, 0};
@@ -691,6 +692,9 @@ static SelPlan sel_plan(int64_t B, int64_t J, int64_t V)
     const bool big = B * J * ((V + 8191) / 8192) >= 512;
     return SelPlan{0, 256, big ? 32 : 8, (int)(big ? (V + 8191) / 8192 : (V + 2047) / 2048)};
 }
+
+// batch entries of a launch with `per` workgroups an entry
+static int64_t sel_most(int64_t B, int64_t per) { return B < SEL_LAUNCH / per ? B : SEL_LAUNCH / per; }
 
 template <typename T> static void sel_rows(const SelArgs &a, const SelPlan &p, hipStream_t st)
 {
@@ -720,10 +724,8 @@ static int sel_check(const vqhip_beam_select_t *p, const char *what)
     if (!p) VQ_FAIL(VQHIP_EINVAL, "%s: null argument", what);
     if (!vq_elem_bytes(p->dtype)) VQ_FAIL(VQHIP_EINVAL, "%s: dtype %lld", what, (long long)p->dtype);
     if (p->B < 0 || p->J < 1 || p->V < 1 || p->K < 1) VQ_FAIL(VQHIP_EINVAL, "%s: B %lld, J %lld, V %lld, K %lld", what, (long long)p->B, (long long)p->J, (long long)p->V, (long long)p->K);
-    // (a launch takes fewer than 2^32 threads: 256 a row of a tile, 64 an entry of up to 64 continuations)
-    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->V > (1 << 30) / p->J || p->K > p->J * p->V ||
-        p->B > (p->J * p->V <= 64 ? SEL_MOST_SMALL : SEL_MOST_TILES / p->J / ((p->V + 2047) / 2048)))
-        VQ_FAIL(VQHIP_EDIM, "%s: %lld entries, %lld kept of %lld x %lld continuations: at most %d beams, %d kept, 2^30 continuations an entry, 2^24 tiles in all",
+    if (p->J > VQHIP_BEAM_MAX || p->K > VQHIP_BEAM_MAX || p->V > (1 << 30) / p->J || p->K > p->J * p->V || p->B > 0x7fffffff)
+        VQ_FAIL(VQHIP_EDIM, "%s: %lld entries, %lld kept of %lld x %lld continuations: fewer than 2^31 entries, at most %d beams, %d kept, 2^30 continuations an entry",
                 what, (long long)p->B, (long long)p->K, (long long)p->J, (long long)p->V, VQHIP_BEAM_MAX, VQHIP_BEAM_MAX);
     if (p->finished && (p->end_token < 0 || p->end_token >= p->V)) VQ_FAIL(VQHIP_EINVAL, "%s: end token %lld outside [0, %lld)", what, (long long)p->end_token, (long long)p->V);
     if (p->B > 0 && (!p->logits || !p->parents || !p->tokens || !p->out_scores)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
@@ -732,8 +734,9 @@ static int sel_check(const vqhip_beam_select_t *p, const char *what)
 
 extern "C" size_t vqhip_beam_select_workspace_bytes(int64_t B, int64_t J, int64_t V, int64_t K)
 {
-    if (B <= 0 || J <= 0 || V <= 0 || K <= 0 || J > VQHIP_BEAM_MAX || V > (1 << 30) / J) return 0;
-    return (size_t)(B * J * sel_plan(B, J, V).tiles) * (size_t)(8 * K + 12);
+    if (B <= 0 || J <= 0 || V <= 0 || K <= 0 || B > 0x7fffffff || J > VQHIP_BEAM_MAX || V > (1 << 30) / J) return 0;
+    const int64_t per = J * sel_plan(B, J, V).tiles;
+    return per ? (size_t)(sel_most(B, per) * per) * (size_t)(8 * K + 12) : 0;
 }
 
 extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
@@ -745,34 +748,40 @@ extern "C" int vqhip_beam_select(const vqhip_beam_select_t *p, void *stream)
     if (p->workspace_bytes < need || (need && !p->workspace)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select: workspace of %zu bytes, needs %zu", p->workspace_bytes, need);
     if ((uintptr_t)p->workspace & 15) VQ_FAIL(VQHIP_EALIGN, "vqhip_beam_select: workspace not 16-byte aligned");
     SelArgs a;
-    a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.dtype = (int)p->dtype; a.scores = p->scores;
-    a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j; a.finished = p->finished;
-    a.scores_out = p->out_scores; a.parents_out = p->parents; a.tokens_out = p->tokens; a.lse_out = p->lse;
-    a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.end_token = (int)p->end_token; a.normalize = p->normalize != 0;
+    a.lb = p->stride_b; a.lj = p->stride_j; a.dtype = (int)p->dtype; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j;
+    a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.end_token = (int)p->end_token; a.normalize = p->normalize != 0;
     const SelPlan plan = sel_plan(p->B, p->J, p->V);
     hipStream_t st = (hipStream_t)stream;
-    if (plan.small == 2) {
-        if (p->dtype == VQHIP_F32) sel_entries<float>(a, st);
-        else if (p->dtype == VQHIP_BF16) sel_entries<__bf16>(a, st);
-        else sel_entries<_Float16>(a, st);
-        return vq_launch_status("vqhip_beam_select");
+    const int64_t most = sel_most(p->B, plan.small ? 1 : p->J * plan.tiles);
+    for (int64_t b = 0; b < p->B; b += most) {
+        a.B = p->B - b < most ? p->B - b : most;
+        a.logits = (const char *)p->logits + b * p->stride_b * vq_elem_bytes(p->dtype);
+        a.scores = p->scores ? p->scores + b * p->J : nullptr;
+        a.mask = p->mask ? p->mask + b * p->mask_stride_b : nullptr;
+        a.finished = p->finished ? p->finished + b * p->J : nullptr;
+        a.scores_out = p->out_scores + b * p->K; a.parents_out = p->parents + b * p->K; a.tokens_out = p->tokens + b * p->K;
+        a.lse_out = p->lse ? p->lse + b * p->J : nullptr;
+        if (plan.small == 2) {
+            if (p->dtype == VQHIP_F32) sel_entries<float>(a, st);
+            else if (p->dtype == VQHIP_BF16) sel_entries<__bf16>(a, st);
+            else sel_entries<_Float16>(a, st);
+        } else if (plan.small) {
+            int W = 1;
+            while (W < a.J * a.V) W <<= 1;
+            const dim3 grid((unsigned)((a.B * W + 255) / 256));
+            if (p->dtype == VQHIP_F32) vq_beam_small_kernel<float><<<grid, 256, 0, st>>>(a, W);
+            else if (p->dtype == VQHIP_BF16) vq_beam_small_kernel<__bf16><<<grid, 256, 0, st>>>(a, W);
+            else vq_beam_small_kernel<_Float16><<<grid, 256, 0, st>>>(a, W);
+        } else {
+            const int64_t lists = most * a.J * plan.tiles;
+            a.tiles = plan.tiles;
+            a.part = (int2 *)p->workspace; a.part_sum = (double *)(a.part + lists * a.K); a.part_max = (float *)(a.part_sum + lists);
+            if (p->dtype == VQHIP_F32) sel_rows<float>(a, plan, st);
+            else if (p->dtype == VQHIP_BF16) sel_rows<__bf16>(a, plan, st);
+            else sel_rows<_Float16>(a, plan, st);
+            vq_beam_merge_kernel<<<dim3((unsigned)a.B), 256, 0, st>>>(a);
+        }
     }
-    if (plan.small) {
-        int W = 1;
-        while (W < a.J * a.V) W <<= 1;
-        const dim3 grid((unsigned)((a.B * W + 255) / 256));
-        if (p->dtype == VQHIP_F32) vq_beam_small_kernel<float><<<grid, 256, 0, st>>>(a, W);
-        else if (p->dtype == VQHIP_BF16) vq_beam_small_kernel<__bf16><<<grid, 256, 0, st>>>(a, W);
-        else vq_beam_small_kernel<_Float16><<<grid, 256, 0, st>>>(a, W);
-        return vq_launch_status("vqhip_beam_select");
-    }
-    const int64_t lists = a.B * a.J * plan.tiles;
-    a.tiles = plan.tiles;
-    a.part = (int2 *)p->workspace; a.part_sum = (double *)(a.part + lists * a.K); a.part_max = (float *)(a.part_sum + lists);
-    if (p->dtype == VQHIP_F32) sel_rows<float>(a, plan, st);
-    else if (p->dtype == VQHIP_BF16) sel_rows<__bf16>(a, plan, st);
-    else sel_rows<_Float16>(a, plan, st);
-    vq_beam_merge_kernel<<<dim3((unsigned)a.B), 256, 0, st>>>(a);
     return vq_launch_status("vqhip_beam_select");
 }
 
@@ -947,16 +956,26 @@ extern "C" int vqhip_beam_select_bwd(const vqhip_beam_select_t *p, const float *
     if (rc) return rc;
     if (p->B == 0 || (!d_logits && !d_scores)) return 0;
     if (!grad || (p->normalize && d_logits && !p->lse)) VQ_FAIL(VQHIP_EINVAL, "vqhip_beam_select_bwd: null pointer");
+    const int eb = vq_elem_bytes(p->dtype);
     SelBwdArgs a;
-    a.logits = p->logits; a.lb = p->stride_b; a.lj = p->stride_j; a.mask = p->mask; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j;
-    a.finished = p->finished; a.lse = p->lse; a.scores_out = p->out_scores; a.parents = p->parents; a.tokens = p->tokens; a.grad = grad;
-    a.d_logits = d_logits; a.d_scores = d_scores;
-    a.B = p->B; a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.normalize = p->normalize != 0;
+    a.lb = p->stride_b; a.lj = p->stride_j; a.mb = p->mask_stride_b; a.mj = p->mask_stride_j;
+    a.J = (int)p->J; a.V = (int)p->V; a.K = (int)p->K; a.normalize = p->normalize != 0;
     a.tiles = d_logits ? (a.V + SEL_BWD - 1) / SEL_BWD : 1;
     hipStream_t st = (hipStream_t)stream;
-    if (p->dtype == VQHIP_F32) sel_bwd<float>(a, st);
-    else if (p->dtype == VQHIP_BF16) sel_bwd<__bf16>(a, st);
-    else sel_bwd<_Float16>(a, st);
+    const int64_t most = sel_most(p->B, p->J * p->V <= SEL_ENTRY ? 1 : p->J * a.tiles);
+    for (int64_t b = 0; b < p->B; b += most) {
+        a.B = p->B - b < most ? p->B - b : most;
+        a.logits = (const char *)p->logits + b * p->stride_b * eb;
+        a.mask = p->mask ? p->mask + b * p->mask_stride_b : nullptr;
+        a.finished = p->finished ? p->finished + b * p->J : nullptr;
+        a.lse = p->lse ? p->lse + b * p->J : nullptr;
+        a.scores_out = p->out_scores + b * p->K; a.parents = p->parents + b * p->K; a.tokens = p->tokens + b * p->K; a.grad = grad + b * p->K;
+        a.d_logits = d_logits ? (char *)d_logits + b * p->J * p->V * eb : nullptr;
+        a.d_scores = d_scores ? d_scores + b * p->J : nullptr;
+        if (p->dtype == VQHIP_F32) sel_bwd<float>(a, st);
+        else if (p->dtype == VQHIP_BF16) sel_bwd<__bf16>(a, st);
+        else sel_bwd<_Float16>(a, st);
+    }
     return vq_launch_status("vqhip_beam_select_bwd");
 }
 
