@@ -575,7 +575,8 @@ int vqhip_beam_select_bwd(const vqhip_beam_select_t *step, const float *grad, vo
 /* ---- beam search: the states follow their beams ------------------------------------------------------
  * dst[b, i] = src[b, parents[b, i]] for n <= VQHIP_BEAM_STATES states in one launch (`pick`, the gathers of rvq.py:533-562).  A state's row is
  * `pieces` runs of piece_bytes contiguous bytes, piece_stride bytes apart; rows lie stride_j, batch entries stride_b bytes apart; dst is
- * contiguous [B, K, pieces * piece_bytes] and overlaps no src; less than 2^24 workgroups of 16 KB in all.  parents [B, K] int64; one outside [0, J) gives a row of zeros.
+ * contiguous [B, K, pieces * piece_bytes] and overlaps no src.  parents [B, K] int64; one outside [0, J) gives a row of zeros.
+ * B * K < 2^31, and less than 2^24 workgroups of 16 KB in all (VQHIP_EDIM beyond), here and in the backward.
  * vqhip_beam_reorder_bwd: dst[b, j] = sum of src[b, i] over parents[b, i] == j, summed in fp32 by ascending i and rounded once; src
  * (the gradients [B, K, row]) and dst ([B, J, row]) contiguous, element types dtypes[n] F32 / BF16 / F16; the strides are not read. */
 #define VQHIP_BEAM_STATES 32

@@ -535,6 +535,23 @@ def test_select_of_large_batches(dev, b, j, v, k):
     assert not ((step.parents < 0) | (step.parents >= j) | (step.tokens < 0) | (step.tokens >= v)).any()
 
 
+@pytest.mark.gpu
+def test_reorder_of_more_than_2_31_rows(dev):
+    """the continuations of a residual beam search: 2^19 entries of 64 x 64; parents that differ, so that every gradient lies alone"""
+    import vector_quantize_pytorch_amd as A
+    b, j = 2 ** 19 + 3, 4096
+    g = torch.Generator(device="cuda").manual_seed(0)
+    s = torch.empty(b, j, dtype=torch.bfloat16, device="cuda").normal_(generator=g).requires_grad_(True)
+    par = torch.randint(0, j // 2, (b, 2), generator=g, device="cuda")
+    par[:, 1] += j // 2
+    par[-1] = torch.tensor([j - 1, 0])
+    n, = A.beam_reorder([s], par)
+    assert torch.equal(n, s.detach().gather(1, par))
+    w = torch.rand(b, 2, generator=g, device="cuda").bfloat16() + 1
+    d, = torch.autograd.grad(n, s, w)
+    assert torch.equal(d.gather(1, par), w) and int(torch.count_nonzero(d)) == 2 * b
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A
@@ -665,3 +682,16 @@ def test_c_entry_takes_large_batches():
         assert nws < 2 ** 34
         s = _Select(logits=8, dtype=1, B=b, J=j, V=v, stride_b=j * v, stride_j=v, normalize=0, K=min(4, j * v), out_scores=8, parents=8, tokens=8, workspace=24, workspace_bytes=nws)
         assert L.vqhip_beam_select(ctypes.byref(s), None) == -3, (b, j, v)
+
+
+def test_reorder_takes_many_rows():
+    """sizes are checked before the states' pointers: -1 here is the null pointer"""
+    from vector_quantize_pytorch_amd import _lib
+    from vector_quantize_pytorch_amd.beam import _State
+    L = _lib.lib()
+    nul = (_State * 1)((None, 8, 4096 * 4, 4, 1, 0, 4))
+    dts = (ctypes.c_int64 * 1)(0)
+    for b, j, k in [(2 ** 19, 4096, 64), (2 ** 20, 4096, 1), (2 ** 31 - 1, 64, 1)]:
+        assert L.vqhip_beam_reorder(nul, 1, 8, b, j, k, None) == -1
+        assert L.vqhip_beam_reorder_bwd(nul, dts, 1, 8, b, j, k, None) == -1
+    assert L.vqhip_beam_reorder(nul, 1, 8, 2 ** 25, 1, 64, None) == -2

@@ -1066,8 +1066,8 @@ struct ReorderBwdArgs {
 template <typename T, int N> __device__ __forceinline__ void reo_sum(const ReorderBwdArgs &a, const ReorderBwdState &s)
 {
     const int64_t rows = a.B * a.J;
-    const int64_t id0 = (int64_t)(blockIdx.x - s.first) * REO_UNITS, row0 = id0 / s.per_row;
-    const unsigned off0 = (unsigned)(id0 - row0 * s.per_row);
+    const int64_t id0 = (int64_t)(blockIdx.x - s.first) * REO_UNITS, row0 = id0 / s.per_row, b0 = row0 / a.J;
+    const unsigned off0 = (unsigned)(id0 - row0 * s.per_row), j0 = (unsigned)(row0 - b0 * a.J);
 #pragma unroll
     for (int u = 0; u < REO_PER_THREAD; ++u) {
         const unsigned off = off0 + u * 256 + threadIdx.x, skip = off / s.per_row, in_row = off - skip * s.per_row;
@@ -1075,8 +1075,8 @@ template <typename T, int N> __device__ __forceinline__ void reo_sum(const Reord
         if (row >= rows) break;
         int64_t at = (int64_t)in_row * N;
         at = at + N <= s.row ? at : s.row - N;
-        const unsigned b = (unsigned)row / (unsigned)a.J;
-        const int64_t j = row - (int64_t)b * a.J, k0 = (int64_t)b * a.K;
+        const unsigned further = (j0 + skip) / (unsigned)a.J;
+        const int64_t j = (int64_t)(j0 + skip - further * (unsigned)a.J), k0 = (b0 + further) * a.K;
         const T *g = (const T *)s.grad + k0 * s.row + at;
         float d[N];
 #pragma unroll
@@ -1117,7 +1117,8 @@ __global__ void __launch_bounds__(256) vq_beam_reorder_bwd_kernel(const ReorderB
 static int reorder_check(int64_t n, const void *states, const int64_t *parents, int64_t B, int64_t J, int64_t K, const char *what)
 {
     if (n < 0 || n > VQHIP_BEAM_STATES || B < 0 || J < 1 || K < 1) VQ_FAIL(VQHIP_EINVAL, "%s: %lld states (at most %d), B %lld, J %lld, K %lld", what, (long long)n, VQHIP_BEAM_STATES, (long long)B, (long long)J, (long long)K);
-    if (J > 0x7fffffff || K > 0x7fffffff || B > 0x7fffffff / J || B > 0x7fffffff / K) VQ_FAIL(VQHIP_EDIM, "%s: %lld x %lld rows from %lld x %lld", what, (long long)B, (long long)K, (long long)B, (long long)J);
+    if (J > 0x7fffffff || K > 0x7fffffff || B > 0x7fffffff / K)          // (B * J: a state's units are counted, reorder_blocks)
+        VQ_FAIL(VQHIP_EDIM, "%s: %lld x %lld rows from %lld x %lld", what, (long long)B, (long long)K, (long long)B, (long long)J);
     if (n > 0 && B > 0 && (!states || !parents)) VQ_FAIL(VQHIP_EINVAL, "%s: null pointer", what);
     return 0;
 }
