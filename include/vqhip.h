@@ -551,7 +551,8 @@ int vqhip_row_sumsq(const void *x, int x_dtype, int64_t N, int D, int64_t ldx, f
  * continuations are above -inf, -inf ones follow, by ascending j * V + v.  c is compared in 64 bits and returned rounded to fp32.
  *   logits   [B, J, V] of dtype F32 / BF16 / F16, continuations contiguous, beams stride_j and batch entries stride_b elements apart
  *   scores   nullable (zeros) [B, J] fp32        mask      nullable [B, J, V] bytes at byte strides mask_stride_b / _j (0: shared)
- *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out: the log-sums, which the backward reads
+ *   finished nullable [B, J] bytes               lse       nullable [B, J] doubles out (normalize): the log-sums, which the backward reads;
+ *            not finite for a beam without a continuation, NaN for a finished one and one whose score is not above -inf
  *   out_scores / parents / tokens  [B, K]        workspace vqhip_beam_select_workspace_bytes(B, J, V, K) bytes, 16-byte aligned
  * J, K <= VQHIP_BEAM_MAX, J * V <= 2^30, K <= J * V, B < 2^31 (VQHIP_EDIM beyond; batches that one launch cannot hold go in several).
  * vqhip_beam_select_bwd: the gradients of out_scores (grad [B, K]) with the fields of the forward call, its outputs among them:

@@ -552,6 +552,31 @@ def test_reorder_of_more_than_2_31_rows(dev):
     assert torch.equal(d.gather(1, par), w) and int(torch.count_nonzero(d)) == 2 * b
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("j,v", [(4, 5), (4, 300), (4, 3000), (5, 20011)])
+def test_select_log_sums(dev, j, v):
+    """the C entry's log-sums: the admitted logits' own, NaN for beams whose logits are not used (finished, or without a score), not finite where
+    nothing is left -- also in memory that held numbers before"""
+    from vector_quantize_pytorch_amd.beam import _select
+    lg, sc = make(3, j, v, "fp32", seed=v)
+    mask = torch.rand(3, j, v, generator=torch.Generator().manual_seed(1)).cuda() < 0.7
+    mask[..., 0] = True
+    mask[2, 1] = False
+    fin = torch.zeros(3, j, dtype=torch.bool, device="cuda")
+    fin[0, 1] = fin[1, 0] = True
+    sc[0, 2], sc[1, 3] = NEG, float("nan")
+    for _ in range(2):
+        held = [torch.full((n,), 1.0, dtype=torch.float64, device="cuda") for n in (3 * j, 64, 3 * j * 70)]
+        del held
+        *_, lse = _select(lg, sc, mask.view(torch.uint8), fin.view(torch.uint8), 4, v - 1, True, True)
+        dead = fin | ~(sc > NEG)
+        assert lse.shape == (3, j) and lse[dead].isnan().all()
+        want = lg.double().masked_fill(~mask, NEG).logsumexp(-1)
+        none = ~mask.any(-1)
+        assert not torch.isfinite(lse[none]).any()
+        assert ((lse - want)[~dead & ~none].abs() <= 2.0 ** -20).all()
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A

@@ -31,6 +31,9 @@ __device__ __forceinline__ double sel_sum(double score, double x)
     return c != c ? -INFINITY : c;
 }
 
+// the log-sum as it is handed out: none for a beam whose logits are not used (no tile of it need have been summed)
+__device__ __forceinline__ double sel_lse(double lse, double score, bool finished) { return !finished && score > -INFINITY ? lse : (double)NAN; }
+
 __device__ __forceinline__ bool sel_before(double c, int i, double d, int k) { return c > d || (c == d && i < k); }
 
 // the entry's last survivors where fewer than K continuations are above -inf: the first places, by number, that are not among the `found`
@@ -74,7 +77,7 @@ template <typename T> __global__ void __launch_bounds__(256) vq_beam_small_kerne
         const double mine = exp(x - m);
         for (int t = 0; t < V; ++t) e += __shfl(mine, row + t, 64);
         const double lse = m + log(e);
-        if (in && v == 0 && a.lse_out) a.lse_out[bb * J + j] = lse;
+        if (in && v == 0 && a.lse_out) a.lse_out[bb * J + j] = sel_lse(lse, s, fin);
         x -= lse;
     }
     if (fin) x = v == a.end_token ? 0.0 : -INFINITY;
@@ -248,7 +251,7 @@ template <typename T, int NT, int E> __global__ void __launch_bounds__(NT) vq_be
             fin[j] = f;
             base[j] = f || (s > -INFINITY && lse > -INFINITY && lse < INFINITY) ? s : -INFINITY;
             log_sum[j] = lse;
-            if (a.lse_out) a.lse_out[b * J + j] = lse;
+            if (a.lse_out) a.lse_out[b * J + j] = sel_lse(lse, s, f);
         }
     }
     __syncthreads();
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(256) vq_beam_merge_kernel(const SelArgs a)
             fin[j] = f;
             base[j] = f ? s : live && lse > -INFINITY && lse < INFINITY ? s : -INFINITY;
             log_sum[j] = lse;
-            if (a.lse_out) a.lse_out[row] = lse;
+            if (a.lse_out) a.lse_out[row] = sel_lse(lse, s, f);
         }
     }
     if (t == 0) found = 0;
