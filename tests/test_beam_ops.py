@@ -720,3 +720,16 @@ def test_reorder_takes_many_rows():
         assert L.vqhip_beam_reorder(nul, 1, 8, b, j, k, None) == -1
         assert L.vqhip_beam_reorder_bwd(nul, dts, 1, 8, b, j, k, None) == -1
     assert L.vqhip_beam_reorder(nul, 1, 8, 2 ** 25, 1, 64, None) == -2
+
+
+def test_reorder_refuses_results_that_require_a_gradient():
+    """their history would stay as it was beside other values: s + s, say, would go on passing gradients to s"""
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    st, par = torch.zeros(2, 3, 8), torch.zeros(2, 4, dtype=torch.int64)
+    leaf = torch.zeros(2, 4, 8, requires_grad=True)
+    for o in (leaf, leaf + leaf):
+        with pytest.raises(VQHipError, match="requires a gradient"):
+            A.beam_reorder([st], par, out=[o])
+        with torch.no_grad(), pytest.raises(VQHipError, match="no CPU fallback"):          # (as torch's own out= takes them there)
+            A.beam_reorder([st], par, out=[o])

@@ -292,7 +292,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     use, `cache[..., :length, :]`), otherwise from a contiguous copy.
 
     out: contiguous tensors that take the results (the other half of a double buffer); they may not share memory with a state or with
-    each other, and no state may require a gradient.  Without it, gradients reach float32, bfloat16 and float16 states: beams continued
+    each other, and neither a state nor a result may require a gradient.  Without it, gradients reach float32, bfloat16 and float16 states: beams continued
     by several rows get the sum, accumulated in 32 bits."""
     states = list(states)
     if parents.dtype != torch.int64 or parents.ndim < 1 or parents.shape[-1] < 1:
@@ -327,6 +327,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         out = list(out)
         if grad:
             raise L.VQHipError("beam_reorder: out= with states that require a gradient")
+        if torch.is_grad_enabled() and any(o.requires_grad for o in out):
+            raise L.VQHipError("beam_reorder: a result that requires a gradient")
         if len(out) != len(states):
             raise L.VQHipError(f"beam_reorder: {len(out)} results for {len(states)} states")
         for s, o in zip(states, out):
