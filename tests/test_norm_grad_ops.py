@@ -487,6 +487,17 @@ def test_clip_of_negated_tensors(dev):
         A.clip_grads([h], 1.0, out=[torch.complex(h, h).conj().imag])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("b,n,c,groups", [(2100, 2, 256, 32), (2100, 2, 64, 8), (2100, 3, 96, 4), (300, 16, 256, 8), (5, 3000, 64, 8), (20, 1024, 128, 32), (60, 256, 128, 32), (4, 8192, 32, 8)])
+def test_norm_many_maps(dev, b, n, c, groups, dtype):
+    """batches on either side of where one launch gives way to two"""
+    import vector_quantize_pytorch_amd as A
+    x, w, q, _ = norm_inputs(b, n, c, dtype, "fp32", seed=n)
+    y = A.group_norm(x, groups, w, q, activation="silu")
+    check_forward(y, norm_ref(x, groups, w, q, act="silu"), x.dtype, x.abs().max().item(), 317.0 if n * c // groups < 64 else 4.0)
+
+
 # ---- refusals (host side: no GPU) -------------------------------------------------------------------------------------------------------
 def test_norm_refusals():
     import vector_quantize_pytorch_amd as A

@@ -705,8 +705,15 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     return a;
 }
 
-// the span of vq_gn_one_kernel and its rows a thread; U 0: the slab does not fit.  The widest of up to 128 bytes that leaves a workgroup to
-// every CU, else the narrowest: a small map wants its rows over as many CUs as there are.  16 x 1024 x 256 fp32: 14.5 us, 7.0 + 8.8 in two launches.
+// the span of vq_gn_one_kernel and its rows a thread; U 0: two launches.  The widest of up to 128 bytes that leaves a workgroup to every CU,
+// else the narrowest: a small map wants its rows over as many CUs as there are.  One launch and two, us a call, C channels in G groups:
+//   a launch saved, all small maps       1 x 256 x 512 / 32 bf16 14.1 and 16.6, 16 x 1024 x 256 / 32 fp32 14.5 and 16.9
+//   x read once from HBM                 122 x 256 x 512 / 32 fp32 24 and 36, 4096 x 256 x 64 / 8 fp32 104 and 162
+//   a thread of more than 64 values      122 x 1024 x 256 / 32 bf16 45 and 37: not taken
+//   stripes of less than half a line     122 x 4096 x 64 / 8 fp32 (32 bytes) 126 and 66, threads whose channels lie in several groups 1953 x 64 x
+//                                        128 / 32 bf16 70 and 47: taken up to 4 MB, what an XCD's L2 holds
+//   many small workgroups                3906 x 16 x 256 / 32 bf16 (2 KB each) 109 and 71: not taken, beyond what the CUs hold at once, below 32 KB
+//                                        each and where two spans do not make a row (7812 x 16 x 64 / 8 bf16 57 and 140)
 struct GnOne { int span, U; };
 static GnOne gn_one(int64_t B, int64_t N, int C, int G, int elem)
 {
@@ -721,6 +728,9 @@ static GnOne gn_one(int64_t B, int64_t N, int C, int G, int elem)
         if (rows > 16) break;
         best = GnOne{span, rows <= 1 ? 1 : rows <= 4 ? 4 : 16};
     }
+    if (!best.span) return best;
+    const int64_t slab = N * best.span * elem, slabs = B * (C / best.span);
+    if (best.U * vec > 64 || (slabs * slab > (4 << 20) && (best.span * elem < 64 || cg % vec)) || (slabs > 2048 && slab < 32768 && 2 * best.span < C)) best.U = 0;
     return best;
 }
 
@@ -740,7 +750,7 @@ template <typename T> static void gn_one_rows(const GnArgs &a, const GnOne &o, h
     constexpr int VEC = 16 / sizeof(T);
     if (o.U == 1) gn_one_launch<T, VEC, 1>(a, o.span, st);
     else if (o.U == 4) gn_one_launch<T, VEC, 4>(a, o.span, st);
-    else gn_one_launch<T, VEC, 16>(a, o.span, st);
+    else if constexpr (sizeof(T) == 4) gn_one_launch<T, VEC, 16>(a, o.span, st);
 }
 
 extern "C" size_t vqhip_group_norm_workspace_bytes(int64_t B, int64_t N, int64_t C, int64_t groups)
