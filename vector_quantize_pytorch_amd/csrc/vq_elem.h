@@ -11,18 +11,6 @@ template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) 
 template <typename T, int N> __device__ __forceinline__ VqVec<T, N> vq_ldv(const T *p) { return *(const VqVec<T, N> *)p; }
 template <typename T, int N> __device__ __forceinline__ void vq_stv(T *p, const VqVec<T, N> &v) { *(VqVec<T, N> *)p = v; }
 
-// the same past the caches: results that this kernel and the next do not read
-template <typename T, int N> __device__ __forceinline__ void vq_stv_nt(T *p, const VqVec<T, N> &v)
-{
-    if constexpr (sizeof(v) % 4 == 0) {
-        typedef unsigned U __attribute__((ext_vector_type(sizeof(v) / 4), aligned(sizeof(T))));
-        U u;
-        __builtin_memcpy(&u, &v, sizeof(v));
-        __builtin_nontemporal_store(u, (U *)p);
-    } else
-        vq_stv<T, N>(p, v);
-}
-
 static inline int vq_elem_bytes(int64_t dtype) { return dtype == VQHIP_F32 ? 4 : (dtype == VQHIP_BF16 || dtype == VQHIP_F16) ? 2 : 0; }
 
 // Reductions over the 64 lanes of a full wave by DPP: each row of 16 to its last lane, then rows 0 -> 1, 2 -> 3, then 1 -> 3; lane 63 holds

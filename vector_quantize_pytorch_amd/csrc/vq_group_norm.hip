@@ -27,7 +27,6 @@ struct GnArgs {
     const void *grad; void *dx, *dweight, *dbias;       // backward: grad and dx contiguous
     float2 *pair, *joined; float *chan, *live;          // per chunk: [B * S, G] pairs, (backward) [B * S, 2, C] sums, [B * S] live rows; joined [B, G] or null
     int64_t N, B, rows; int C, G, act, wdtype, S;       // S chunks of `rows` rows
-    int stream;                                         // results past the caches
     double eps;
 };
 
@@ -69,11 +68,6 @@ __device__ __forceinline__ int64_t gn_len(const GnArgs &a, int64_t b)
 }
 
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
-
-template <typename T, int N> __device__ __forceinline__ void gn_store(T *p, const VqVec<T, N> &v, int stream)
-{
-    if (stream) vq_stv_nt<T, N>(p, v); else vq_stv<T, N>(p, v);
-}
 
 // what a thread visits: rows first + lane, + step, ...; VEC channels from vector column col0 + (t % width), pass after pass of `width` columns
 struct GnShape { int cols, width, lanes; };
@@ -355,7 +349,7 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
                     if (SILU) z *= gn_sigmoid(z);
                     o.v[i] = !MASKED || live[u] ? (T)z : (T)0.f;
                 }
-                gn_store<T, VEC>(yc + at * a.C, o, a.stream);
+                vq_stv<T, VEC>(yc + at * a.C, o);
             }
         }
         gn_zero_rows<T, VEC>(yc, (r0 > len ? r0 : len) + lane, end, sh.lanes, a.C);
@@ -645,7 +639,7 @@ template <typename T, int VEC, bool SILU, bool MASKED> __global__ void __launch_
                     const float xh = ((float)v[u].v[i] - mean[i]) * rstd[i], dz = gn_dz<SILU>((float)d[u].v[i], xh, w[i], bias[i]);
                     o.v[i] = !MASKED || live[u] ? (T)(rstd[i] * (fmaf(dz, w[i], -m1[i]) - xh * m2[i])) : (T)0.f;
                 }
-                gn_store<T, VEC>(dx + at * a.C + (int64_t)col * VEC, o, a.stream);
+                vq_stv<T, VEC>(dx + at * a.C + (int64_t)col * VEC, o);
             }
         }
         gn_zero_rows<T, VEC>(dx + (int64_t)col * VEC, (r0 > len ? r0 : len) + lane, end, sh.lanes, a.C);
@@ -697,8 +691,6 @@ static GnArgs gn_args(const vqhip_group_norm_t *p)
     a.x = p->x; a.xb = p->stride_b; a.xn = p->stride_n; a.weight = p->weight; a.bias = p->bias; a.lens = p->lens; a.mask = p->mask;
     a.y = nullptr; a.mean = p->mean; a.rstd = p->rstd; a.grad = nullptr; a.dx = a.dweight = a.dbias = nullptr;
     a.N = p->N; a.B = p->B; a.C = (int)p->C; a.G = (int)p->groups; a.act = (int)p->activation; a.wdtype = (int)p->param_dtype;
-    // results of more than a quarter of the 256 MB memory-side cache go past it: 6 x 65536 x 128 bf16 90 -> 80 us with x still in it
-    a.stream = p->B * p->N * p->C * vq_elem_bytes(p->dtype) > (64 << 20);
     a.S = (int)S; a.rows = rows; a.eps = p->eps;
     a.pair = (float2 *)p->workspace; a.joined = a.pair + p->B * S * p->groups; a.chan = (float *)(a.joined + p->B * p->groups); a.live = a.chan + p->B * S * 2 * p->C;
     if (S == 1 || S * p->groups <= GN_JOIN) a.joined = nullptr;           // (more chunks than one: B <= 256)
