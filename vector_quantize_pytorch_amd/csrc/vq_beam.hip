@@ -178,10 +178,13 @@ template <int NT> __device__ __forceinline__ int sel_count(int c, int *red)
 
 // ---- entries of up to NT * E continuations in one launch ------------------------------------------------------------------------------
 // A workgroup (a wave for up to 1024) holds an entry's continuations, i = u * NT + t of thread t, as 64-bit scores; for the rows' log-sums the
-// logits lie in LDS once, where lanes of a power of two sum a row.  The K best by a bound from 64 groups, sel_cut where more than CAP reach it,
-// and ranks.  Bound by instructions and the latency of its steps, so few waves an entry: 8192 entries of 32 x 32 fp32 with log-sums 36 us with 16
-// a lane of one wave, 45 and 54 with 2 and 4 waves; 16384 of 16 x 16 28 us with 4 a lane, 33 with 8.  In two launches as below, 8192 entries:
-// 16 x 16 141 us (here 18), 4 x 1024 129 (90), 8 x 512 82 (93).
+// logits lie in LDS once, where lanes of a power of two sum a row.  The K best by a bound from 64 groups, sel_cut where more than CAP reach it
+// (K near 64: 300 of 1024 or more do, and almost every entry of one wave takes it), and ranks.  Bound by instructions and the latency of its
+// steps, so few waves an entry: 8192 entries of 32 x 32 fp32 with log-sums, K 32, 36 us with 16 a lane of one wave, 45 and 54 with 2 and 4 waves;
+// 16384 of 16 x 16, K 16, 28 us with 4 a lane, 33 with 8.  Here and in two launches as below, us a call, 8192 entries:
+//   16 x 16 K 16 17 and 143     32 x 32 K 32 40 and 323     4 x 1024 K 4 90 and 134, K 64 274 and 1056
+//   8 x 512 K 4 88 and 77, K 16 99 and 95, K 32 118 and 140     2 x 2048 K 4 97 and 88, K 16 108 and 99, K 64 284 and 349
+// and 256 entries of each with K up to 16 14.6 and 19.8: a launch saved where entries are few, a tenth lost where many have rows that fit a tile.
 #define SEL_ENTRY 4096
 template <typename T, int NT, int E> __global__ void __launch_bounds__(NT) vq_beam_entry_kernel(const SelArgs a)
 {
@@ -321,7 +324,7 @@ template <typename T, int NT, int E> __global__ void __launch_bounds__(NT) vq_be
 
 // NT threads hold a tile of NT * E logits in registers, 8 consecutive ones of every NT * 8 each.  The K best:
 //   1. a bound: the threads form 64 groups; the K-th largest of the groups' maxima has at least K logits at or above it;
-//   2. what reaches the bound is collected (on unordered data about K + K^2 / 128);
+//   2. what reaches the bound is collected: on unordered data the sum of 64 / (64 - i) over i < K on average, 4 for K 4, 18 for 16, 44 for 32, 304 for 64;
 //   3. where more than SEL_CAP do (ties, runs), the K-th largest is found by bisection over value and place, and exactly K collected;
 //   4. each collected one's rank is the number of those before it.
 template <typename T, int NT, int E, bool MASKED> __global__ void __launch_bounds__(NT) vq_beam_rows_kernel(const SelArgs a)

@@ -35,7 +35,8 @@ __device__ double grad_block_sum(double v)
     return v;
 }
 
-// 16-byte loads, four in flight a thread; what is left of a tensor's end one by one
+// 16-byte loads, four in flight a thread (of a chunk's 512 vectors of a 16-bit type two are a thread's own, the other two read its first again);
+// what is left of a tensor's end one by one
 template <typename T> __device__ double grad_sumsq(const T *src, int64_t n)
 {
     constexpr int N = 16 / sizeof(T);
