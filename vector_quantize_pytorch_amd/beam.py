@@ -50,6 +50,8 @@ def _table(t: torch.Tensor, b: int, j: int, v: int) -> torch.Tensor:
     """t [..., j, v] as [b, j, v] with contiguous continuations, without a copy where the layout allows it"""
     if t.ndim != 3:
         t = t.reshape(b, j, v)
+    if t.is_contiguous():
+        return t
     return t if t.stride(-1) == 1 or v == 1 else t.contiguous()
 
 
@@ -60,7 +62,7 @@ def _select(logits, scores, mask, finished, beam_size, end_token, normalize, wan
     lib = L.lib()
     out = torch.empty((b, beam_size), dtype=torch.float32, device=dev)
     # (tensors of their own: views of one would share its version, and an edit of the tokens would stop the backward of a reordering)
-    parents, tokens = (torch.empty((b, beam_size), dtype=torch.int64, device=dev) for _ in range(2))
+    parents, tokens = torch.empty((b, beam_size), dtype=torch.int64, device=dev), torch.empty((b, beam_size), dtype=torch.int64, device=dev)
     lse = torch.empty((b, j), dtype=torch.float64, device=dev) if want_lse else None
     nws = lib.vqhip_beam_select_workspace_bytes(b, j, v, beam_size)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
@@ -125,9 +127,9 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     if logits.ndim < 2:
         raise L.VQHipError(f"beam_select: logits {tuple(logits.shape)}, expected [..., beams, vocabulary]")
     *lead, j, v = logits.shape
-    rows = tuple(logits.shape[:-1])
-    if scores is not None and (tuple(scores.shape) != rows or scores.dtype != torch.float32):
-        raise L.VQHipError(f"beam_select: scores {tuple(scores.shape)} {scores.dtype}, expected {rows} float32")
+    rows = logits.shape[:-1]
+    if scores is not None and (scores.shape != rows or scores.dtype != torch.float32):
+        raise L.VQHipError(f"beam_select: scores {tuple(scores.shape)} {scores.dtype}, expected {tuple(rows)} float32")
     if mask is not None:
         if mask.dtype != torch.bool:
             raise L.VQHipError(f"beam_select: mask of {mask.dtype}, expected bool")
@@ -136,23 +138,22 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
         except RuntimeError:
             raise L.VQHipError(f"beam_select: mask {tuple(mask.shape)} does not broadcast to {tuple(logits.shape)}") from None
     if finished is not None:
-        if tuple(finished.shape) != rows or finished.dtype != torch.bool:
-            raise L.VQHipError(f"beam_select: finished {tuple(finished.shape)} {finished.dtype}, expected {rows} bool")
+        if finished.shape != rows or finished.dtype != torch.bool:
+            raise L.VQHipError(f"beam_select: finished {tuple(finished.shape)} {finished.dtype}, expected {tuple(rows)} bool")
         if end_token is None or not 0 <= end_token < v:
             raise L.VQHipError(f"beam_select: finished beams need an end_token in [0, {v}), got {end_token}")
     if j < 1 or v < 1 or j > BEAM_MAX or not 1 <= beam_size <= min(BEAM_MAX, j * v):
         raise L.VQHipError(f"beam_select: {beam_size} survivors of {j} x {v} continuations: takes 1 to {BEAM_MAX} beams and survivors, "
                            "no more survivors than continuations")
-    n = 1
-    for d in lead:
-        n *= d
+    n = lead[0] if len(lead) == 1 else math.prod(lead)
     L._no_tangent("beam_select", (logits, scores))
     grad = torch.is_grad_enabled() and (logits.requires_grad or (scores is not None and scores.requires_grad))
     L._need_gpu(logits, scores, mask, finished)
     beam_size = int(beam_size)
     lg = _table(logits.resolve_neg(), n, j, v)              # (the library reads memory, where torch leaves a negation pending in a flag)
-    scores = None if scores is None else scores.resolve_neg()
-    sc = scores if scores is None or (len(lead) == 1 and scores.is_contiguous()) else scores.reshape(n, j).contiguous()
+    sc = None if scores is None else scores.resolve_neg().contiguous()
+    if sc is not None and len(lead) != 1:
+        sc = sc.view(n, j)
     mk = None if mask is None else _table(mask, n, j, v).view(torch.uint8)
     fin = None if finished is None else finished.reshape(n, j).contiguous().view(torch.uint8)
     end = 0 if finished is None else int(end_token)
@@ -210,8 +211,9 @@ def _resolved(states):
 
 def _extent(t):
     """[first byte, behind the last byte) of a tensor's memory"""
-    span = sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-    return t.data_ptr(), t.data_ptr() + span * t.element_size()
+    n, first = t.numel(), t.data_ptr()
+    span = n if n == 0 or t.is_contiguous() else sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1
+    return first, first + span * t.element_size()
 
 
 @L._on_device

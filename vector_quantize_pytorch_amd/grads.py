@@ -115,7 +115,7 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, *, erro
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     parameters = list(parameters)
-    L._no_tangent("clip_grad_norm_", [p.grad for p in parameters])
+    L._no_tangent("clip_grad_norm_", (p.grad for p in parameters))
     grads = list({id(p.grad): p.grad.detach() for p in parameters if p.grad is not None}.values())      # a shared one counts once
     work = [g if g.is_contiguous() else g.contiguous() for g in grads]
     if error_if_nonfinite and work:

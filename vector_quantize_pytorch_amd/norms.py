@@ -98,7 +98,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     if not eps >= 0.0:
         raise L.VQHipError(f"group_norm: eps {eps}")
     for p in (weight, bias):
-        if p is not None and (tuple(p.shape) != (c,) or p.dtype not in (torch.float32, x.dtype)):
+        if p is not None and (p.shape != (c,) or p.dtype not in (torch.float32, x.dtype)):
             raise L.VQHipError(f"group_norm: parameter {tuple(p.shape)} {p.dtype}, expected ({c},) float32 or {x.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise L.VQHipError(f"group_norm: weight of {weight.dtype}, bias of {bias.dtype}")
@@ -111,14 +111,13 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     L._no_tangent("group_norm", (x, weight, bias))
     L._need_gpu(x, weight, bias, mask, lens)
     x = x.resolve_neg()                                     # (the library reads memory, where torch leaves a negation pending in a flag)
-    weight, bias = (None if p is None else p.resolve_neg() for p in (weight, bias))
     rows = x if x.ndim == 3 else x.flatten(1, -2) if x.ndim > 3 else x[:, None]
     if rows.stride(-1) != 1 and c > 1:
         rows = rows.contiguous()
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    if weight is not None:
+        weight = weight.resolve_neg().contiguous()
+    if bias is not None:
+        bias = bias.resolve_neg().contiguous()
     mk = None if mask is None else mask.contiguous().view(torch.uint8)
     ln = None if lens is None else lens.to(torch.int64).contiguous()
     args = (rows, weight, bias, ln, mk, num_groups, float(eps), _ACTIVATIONS[activation])
