@@ -118,7 +118,8 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     scores `scores[j] + log_softmax(logits[j])[v]`, or `scores[j] + logits[j, v]` with normalize=False (negative errors of codes, say).
     -> BeamStep(scores, parents, tokens), each [..., beam_size], best first; equal scores by ascending beam, then ascending token.
 
-    mask      bool, broadcastable to logits: False leaves a continuation out -- of the softmax as well; its logits may hold anything
+    mask      bool, broadcastable to logits: False leaves a continuation out -- of the softmax as well; its logits may hold anything (one that
+              is broadcast over the vocabulary is copied to that size)
     finished  bool [..., beams]: such a beam is kept as it is, as its own only continuation `end_token`
     A score that is not a number counts as -inf: a beam whose logits hold NaN or +inf, or whose mask leaves nothing, has no
     continuation (normalize=True).  Where fewer than beam_size continuations are left, the last survivors have a score of -inf.

@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(VQS_WAVES * 64, 8 / VQS_WAVES) vq_screen16_ker
                 const f32x4 w = *(const f32x4 *)(nh + 32 + 8 * q);
                 if (METRIC != 0) { v.x = v.x < -1e38f ? v.x : 0.f; v.y = v.y < -1e38f ? v.y : 0.f;
                                    v.z = v.z < -1e38f ? v.z : 0.f; v.w = v.w < -1e38f ? v.w : 0.f; }
-                // two scores per instruction (v_pk_mul_f32 / v_pk_fma_f32: written as 2-vectors, the SLP vectoriser is off -- csrc/Makefile)
+                // two scores a line (2-vectors, issued half by half: packed fp32 is off -- csrc/Makefile)
                 const f32x2 vp[2] = {f32x2{v.x, v.y}, f32x2{v.z, v.w}}, wp[2] = {f32x2{w.x, w.y}, f32x2{w.z, w.w}};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {

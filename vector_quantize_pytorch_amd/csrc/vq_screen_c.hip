@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(256, 2) vq_screenc_kernel(const ScreenArgs a, 
     // PLAIN mode (chosen per launch from the codebook alone): while the largest code norm is within 4 x of the smallest, charging every
     // code OTHER than the two best with the largest norm costs little -- the winner / runner-up decision keeps both codes' own
     // allowances, only the "nobody else comes close" test (best vs third) is looser, i.e. some pair rows become open rows -- and the
-    // sweep can track the plain scores: one start vector -||c||^2 / 2 for both row blocks and all lanes, 8 packed multiplies per tile
-    // instead of 8 + 16 packed FMAs (which cost the cfg-2 search 4 %).  Codebooks with a wider norm spread keep the upper-bound scores
+    // sweep can track the plain scores: one start vector -||c||^2 / 2 for both row blocks and all lanes, 16 multiplies per tile
+    // instead of 16 + 32 FMAs (which cost the cfg-2 search 4 %).  Codebooks with a wider norm spread keep the upper-bound scores
     // (one large code must not raise every row's threshold).
     const float y2max_c = __uint_as_float(a.scalars[0]), y2min_c = __uint_as_float(~a.scalars[4]);
 #ifdef VQC_FORCE_UPPER      // dev builds: the upper-bound sweep whatever the codebook (A/B runs of the two sweeps on one workload)
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(256, 2) vq_screenc_kernel(const ScreenArgs a, 
                         const f32x4 w = *(const f32x4 *)(nh + 32 + 8 * q);
                         if (METRIC != 0) { v.x = v.x < -1e38f ? v.x : 0.f; v.y = v.y < -1e38f ? v.y : 0.f;
                                            v.z = v.z < -1e38f ? v.z : 0.f; v.w = v.w < -1e38f ? v.w : 0.f; }
-                        // two scores per instruction (v_pk_mul_f32 / v_pk_fma_f32, explicit 2-vectors: the SLP vectoriser is off)
+                        // two scores a line (2-vectors, issued half by half: packed fp32 is off)
                         const f32x2 vp[2] = {f32x2{v.x, v.y}, f32x2{v.z, v.w}}, wp[2] = {f32x2{w.x, w.y}, f32x2{w.z, w.w}};
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {

@@ -464,7 +464,7 @@ __device__ __forceinline__ void mfma_sweep_tile(const f32x4 *ap, const float (&x
 // lanes, so every VALU instruction of either resident wave takes ~7 cycles AWAY from the MFMA stream -- VALU work is
 // not hidden behind fp32 MFMAs, it is serialised with them.  The epilogue is therefore written for minimum VALU
 // instruction COUNT (about 90 per tile; the first version, one wave-level branch per element, had ~190 + 16 branches):
-//   1. s = (x2 + y2) + (-2 xy)          v_pk_add_f32 + v_pk_fma_f32, two codes per instruction  (vqp.py:62, one
+//   1. s = (x2 + y2) + (-2 xy)          v_add_f32 + v_fma_f32  (vqp.py:62, one
 //                                        rounding per operation exactly like the reference; the product by -2 is exact)
 //   2. s_min                             v_min3_f32 tree; clamp(min=1e-8) applied to the minimum only (monotone)
 //   3. skip the tile (wave-uniform) unless some lane has s_min < s_best: sqrt is monotone, it cannot win
@@ -532,7 +532,7 @@ template <int DT>
 __device__ __forceinline__ float x2_aten_order(const float (&xr)[DT / 2], int j)
 {
     constexpr int NG = DT / 8;
-    // two chains per v_pk_mul_f32 / v_pk_add_f32 (each component rounds exactly like the scalar op)
+    // two chains as 2-vectors (each component rounds exactly like the scalar op)
     f32x2 ch[4][2];
 #pragma unroll
     for (int mm = 0; mm < 4; ++mm) { ch[mm][0] = f32x2{0.f, 0.f}; ch[mm][1] = f32x2{0.f, 0.f}; }

@@ -78,7 +78,7 @@ def _table(grads, out):
 
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[Sequence[torch.Tensor]] = None):
     """-> (clipped, norm): norm = the 2-norm over all elements of all tensors (a 0-dim float32 tensor, summed in 64 bits), clipped =
-    every tensor times min(1, max_norm / (norm + 1e-6)), rounded once to its type.
+    every tensor times min(1, max_norm / (norm + 1e-6)), the factor in 32 bits, the product rounded to the tensor's type.
 
     grads: contiguous float32 / bfloat16 / float16 tensors of one device; out: contiguous tensors of the same types and numbers of
     elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that

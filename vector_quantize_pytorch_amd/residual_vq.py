@@ -573,7 +573,7 @@ class ResidualVQ(nn.Module):
             elif max(J, keep) <= BEAM_MAX:
                 scores, parents, tokens = beam_select(total, None, keep, normalize=False)
                 at = parents * K + tokens
-            else:
+            else:                                                   # (more beams than a selection takes)
                 scores, at = total.flatten(-2).topk(keep, dim=-1)
                 parents = at // K
             if want_inputs:
