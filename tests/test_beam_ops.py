@@ -577,6 +577,21 @@ def test_select_log_sums(dev, j, v):
         assert ((lse - want)[~dead & ~none].abs() <= 2.0 ** -20).all()
 
 
+@pytest.mark.gpu
+def test_forward_mode_through_the_backward_is_refused(dev):
+    """a gradient with a tangent (forward over backward): the backward's result would come without one"""
+    import torch.autograd.forward_ad as fwad
+    import vector_quantize_pytorch_amd as A
+    from vector_quantize_pytorch_amd._lib import VQHipError
+    lg, x = torch.randn(2, 3, 10, device="cuda", requires_grad=True), torch.randn(2, 3, 8, device="cuda", requires_grad=True)
+    for y, t in ((A.beam_select(lg, None, 4).scores, lg), (A.beam_reorder([x], torch.zeros(2, 4, dtype=torch.int64, device="cuda"))[0], x), (A.group_norm(x, 2), x)):
+        with fwad.dual_level():
+            g = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(VQHipError, match="forward-mode"):
+                torch.autograd.grad(y, t, g, retain_graph=True)
+        assert torch.autograd.grad(y, t, torch.ones_like(y))[0].shape == t.shape
+
+
 # ---- refusals (host side: no GPU) ---------------------------------------------------------------------------------------------------
 def test_select_refusals():
     import vector_quantize_pytorch_amd as A

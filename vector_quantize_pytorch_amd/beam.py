@@ -104,6 +104,7 @@ class _SelectFn(torch.autograd.Function):
     def backward(ctx, grad, _parents, _tokens):
         if grad is None:
             return (None,) * 7
+        L._no_tangent("beam_select's backward", (grad,))
         logits, mask, finished, out, parents, tokens, lse = ctx.saved_tensors
         d_logits, d_scores = _select_bwd(grad.resolve_neg().contiguous(), logits, mask, finished, ctx.end_token, ctx.normalize, out, parents, tokens, lse,
                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1])
@@ -123,7 +124,8 @@ def beam_select(logits: torch.Tensor, scores: Optional[torch.Tensor], beam_size:
     finished  bool [..., beams]: such a beam is kept as it is, as its own only continuation `end_token`
     A score that is not a number counts as -inf: a beam whose logits hold NaN or +inf, or whose mask leaves nothing, has no
     continuation (normalize=True).  Where fewer than beam_size continuations are left, the last survivors have a score of -inf.
-    Gradients reach logits and scores through the returned scores (backward mode); survivors of score -inf pass none on."""
+    Gradients reach logits and scores through the returned scores (backward mode); survivors of score -inf pass none on.  The backward reads the
+    returned tensors: where one follows, edit copies of them."""
     L._elem_code(logits, "beam_select")
     if logits.ndim < 2:
         raise L.VQHipError(f"beam_select: logits {tuple(logits.shape)}, expected [..., beams, vocabulary]")
@@ -284,6 +286,7 @@ class _ReorderFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         parents, = ctx.saved_tensors
+        L._no_tangent("beam_reorder's backward", grads)
         need = ctx.needs_input_grad[1:]
         return (None, *_reorder_bwd(parents, ctx.beams, [g if w else None for g, w in zip(grads, need)]))
 

@@ -74,6 +74,7 @@ class _GroupNormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, weight, bias, lens, mask, stats = ctx.saved_tensors
+        L._no_tangent("group_norm's backward", (grad,))
         dx, dw, db = _backward(grad.resolve_neg().contiguous(), x, weight, bias, lens, mask, *ctx.args, stats, *ctx.needs_input_grad[:3])
         return dx, dw, db, None, None, None, None, None
 
