@@ -298,8 +298,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     use, `cache[..., :length, :]`), otherwise from a contiguous copy.
 
     out: contiguous tensors that take the results (the other half of a double buffer); they may not share memory with a state or with
-    each other, and neither a state nor a result may require a gradient.  Without it, gradients reach float32, bfloat16 and float16 states: beams continued
-    by several rows get the sum, accumulated in 32 bits."""
+    each other, and neither a state nor a result may require a gradient.  Without it, gradients reach float32, bfloat16 and float16 states:
+    beams continued by several rows get the sum, accumulated in 32 bits."""
     states = list(states)
     if parents.dtype != torch.int64 or parents.ndim < 1 or parents.shape[-1] < 1:
         raise L.VQHipError(f"beam_reorder: parents {tuple(parents.shape)} {parents.dtype}, expected int64 [..., k]")

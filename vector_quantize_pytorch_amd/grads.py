@@ -83,8 +83,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[
     grads: contiguous float32 / bfloat16 / float16 tensors of one device; out: contiguous tensors of the same types and numbers of
     elements that take the result -- a gradient itself, or memory that no other tensor of the call shares; None: new tensors.  A norm that
     is not finite is not hidden: infinite, it makes every finite gradient 0, NaN makes all of them NaN.  max_norm inf: the norm alone
-    (nothing is scaled unless it is NaN).  No gradient passes through, and a forward-mode
-    tangent is refused."""
+    (nothing is scaled unless it is NaN).  No gradient passes through, and a forward-mode tangent is refused."""
     given, grads = grads, list(grads)
     if not max_norm >= 0.0:
         raise L.VQHipError(f"clip_grads: max_norm {max_norm}")

@@ -85,7 +85,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     """x [b, ..., c] (float32 / bfloat16 / float16), channels last -> act(norm(x) * weight + bias), contiguous, x's shape and type.
 
     Mean and variance of each of the `num_groups` channel groups over all positions of a batch entry, in 32 bits or more, whatever x's
-    type; activation None or 'silu'.  At most 2^22 entries and 8192 channels.  weight, bias [c]: both of one type, float32 or x's, either may be left out.
+    type; activation None or 'silu'.  weight, bias [c]: both of one type, float32 or x's, either may be left out.  At most 2^22 entries and 8192
+    channels.
     mask / lens: as in VectorQuantize.forward for x [b, n, c] -- bool [b, n], or the number of live rows [b] (integers; more than n counts as
     n, less than 1 as none).  Padding rows take no part in the statistics, may hold anything, and give zeros, gradients as well."""
     L._elem_code(x, "group_norm")
